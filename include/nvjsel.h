@@ -253,6 +253,96 @@ int nvjsel_derive_keys_table(const int32_t* slots, int batch, int32_t* counter_t
                              uint32_t* keys, void* stream);
 
 /*
+ * LM head with 4-bit weights and group scales (no counterpart in the
+ * reference): w[v,k] = scale[v,G] * (q[v,k] - zero[v,G]), G = k / group, q in 0..15,
+ * zero = 8 where there are no zero points.  group is 32, 64 or 128 and divides
+ * hidden_dim; any vocab.  Scales are bf16 or f16.
+ *
+ * nvjsel_w4_quantize rounds weight(v, k) (element strides row_stride along v,
+ * col_stride along k; f32, bf16 or f16) to the plain form: qweight
+ * uint8 [vocab, hidden_dim / 2] with k even in the low nibble, scales
+ * [vocab, hidden_dim / group] of scale_dtype, zeros uint8 of the same shape
+ * (0..15), or null for codes around 8.  nvjsel_w4_pack lays a plain form out
+ * for the kernels, once: packed, nvjsel_w4_packed_size() bytes (0 for a shape
+ * that is not served), 16-byte aligned.
+ */
+size_t nvjsel_w4_packed_size(int vocab, int hidden_dim, int group, int has_zeros);
+
+int nvjsel_w4_quantize(const void* weight, int weight_dtype, int64_t row_stride, int64_t col_stride, int vocab,
+                       int hidden_dim, int group, int scale_dtype, void* qweight, void* scales, void* zeros,
+                       void* stream);
+
+int nvjsel_w4_pack(const void* qweight, const void* scales, const void* zeros, int vocab, int hidden_dim, int group,
+                   void* packed, size_t packed_bytes, void* stream);
+
+/*
+ * nvjsel_lm_head_top1 and nvjsel_lm_head_logits with such a weight: hidden
+ * [batch, hidden_dim] f32, bf16 or f16, fp32 accumulation, the same workspace
+ * (nvjsel_lm_head_workspace_size) and the same order of ids.  scale_dtype,
+ * has_zeros and group as packed.  A hidden row that holds a NaN or an infinity
+ * gets NaN for every logit.
+ */
+int nvjsel_lm_head_w4_top1(const void* hidden, int hidden_dtype, const void* packed, size_t packed_bytes,
+                           int scale_dtype, int has_zeros, int group, int batch, int hidden_dim, int vocab,
+                           int reduce_cast, int32_t* out_ids, float* out_best, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+int nvjsel_lm_head_w4_logits(const void* hidden, int hidden_dtype, const void* packed, size_t packed_bytes,
+                             int scale_dtype, int has_zeros, int group, int batch, int hidden_dim, int vocab,
+                             int reduce_cast, void* out_logits, int out_dtype, int64_t out_row_stride, void* stream);
+
+/*
+ * Beam search's selection (no counterpart in the reference).  Request b's
+ * candidates are
+ *   scores[b,w] + log_softmax(logits[b,w,:])[v]   for every beam w and token v;
+ * the k best of them, by value descending and, among equal values, by w * vocab + v
+ * ascending, give out_scores f32 [batch, k], out_parents int32 (w) and out_tokens
+ * int32 (v).  logits [batch, beams, vocab] of dtype, batch_stride and
+ * beam_stride elements apart; scores f32 [batch, beams].  1 <= beams, k <= 64,
+ * vocab <= 2^26.
+ *
+ * A beam whose score is -inf is not live: it has no candidates and its logits
+ * are not looked at.  A beam with finished[b,w] != 0 (nullable) has one
+ * candidate, end_token at its own score; its logits are not looked at either.  A
+ * candidate of -inf is none (masked tokens; a row of only -inf has none): where
+ * fewer than k are left the rest is -inf, parent -1, token -1.  A NaN or +inf
+ * among a live beam's logits, or as its score, makes its candidates NaN, and
+ * NaN comes before every number, in order of place.
+ * Workspace: nvjsel_beam_select_workspace_size() bytes of scratch, 16-byte
+ * aligned, any contents on entry.
+ */
+size_t nvjsel_beam_select_workspace_size(int dtype, int batch, int beams, int vocab, int k);
+
+int nvjsel_beam_select(const void* logits, int dtype, int batch, int beams, int vocab, int64_t batch_stride,
+                       int64_t beam_stride, const float* scores, const uint8_t* finished, int end_token, int k,
+                       float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
+ * Reordering of the beams' states after a selection, in place (no counterpart
+ * in the reference): for every tensor, row slot(b,w) receives what row
+ * slot(b, parents[b,w]) held before the call.  A tensor is `rows` rows, row_bytes
+ * apart, each of outer x length x token_bytes contiguous bytes.  lengths (nullable)
+ * int32 [batch]: only the first lengths[b] of `length` positions move, the rest
+ * stays as it is.  slots (nullable: row b * beams + w) int32 [batch, beams], the
+ * slots of a call distinct; parents rows are parent_stride apart.  A beam
+ * whose parent is itself or outside 0..beams-1, or whose own or parent's slot is
+ * outside 0..rows-1, stays as it is.  beams <= 64, batch <= 65535.  The descriptions
+ * are read before the call returns.
+ */
+typedef struct {
+  void* data;
+  int64_t row_bytes;
+  int64_t length;
+  int64_t token_bytes;
+  int32_t outer;
+  int32_t rows;
+} nvjsel_state;
+
+int nvjsel_reorder_states(const nvjsel_state* states, int count, const int32_t* parents, int64_t parent_stride,
+                          const int32_t* slots, const int32_t* lengths, int batch, int beams, void* stream);
+
+/*
  * Diagnostic (no counterpart in the reference): the Gumbel draw of every
  * 23-bit uniform mantissa m in [first, first + n), i.e. random bits
  * (m << 9), two ways -- fast[i] with the hardware fp32 log the kernels use to

@@ -42,9 +42,24 @@ SIGNATURES = {
     "nvjsel_derive_keys_table": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "nvjsel_topk_workspace_size": (_sz, [_i, _i]),
     "nvjsel_topk": (_i, [_vp, _i, _i, _i, _i64, _i, _vp, _vp, _vp, _sz, _vp]),
+    "nvjsel_w4_packed_size": (_sz, [_i, _i, _i, _i]),
+    "nvjsel_w4_quantize": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "nvjsel_w4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "nvjsel_lm_head_w4_top1": (_i, [_vp, _i, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "nvjsel_lm_head_w4_logits": (_i, [_vp, _i, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _i64, _vp]),
+    "nvjsel_beam_select_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "nvjsel_beam_select": (_i, [_vp, _i, _i, _i, _i, _i64, _i64, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nvjsel_reorder_states": (_i, [_vp, _i, _vp, _i64, _vp, _vp, _i, _i, _vp]),
     "nvjsel_debug_gumbel_draws": (_i, [ctypes.c_uint32, _i, _vp, _vp, _vp]),
     "nvjsel_debug_sample_topp": (_i, [_vp, _i, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
+
+
+class State(ctypes.Structure):
+    """nvjsel_state: one tensor of nvjsel_reorder_states."""
+
+    _fields_ = [("data", _vp), ("row_bytes", _i64), ("length", _i64), ("token_bytes", _i64),
+                ("outer", ctypes.c_int32), ("rows", ctypes.c_int32)]
 
 
 class NvjselError(RuntimeError):

@@ -1,0 +1,63 @@
+"""What the entry points share: dtype codes, device checks, the stream and the
+zero-filled workspaces."""
+from __future__ import annotations
+
+import threading
+from contextlib import nullcontext
+
+import torch
+
+from . import _lib
+
+_TORCH_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _dtype_code(t: torch.Tensor, what: str) -> int:
+    try:
+        return _TORCH_DTYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"unsupported {what} dtype: {t.dtype}") from None
+
+
+def _require_cuda(*ts: torch.Tensor) -> torch.device:
+    dev = ts[0].device
+    for t in ts:
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise ValueError("nvjsel kernels take device tensors (got a CPU tensor)")
+        if t.device != dev:
+            raise ValueError("all tensors must live on one device")
+    return dev
+
+
+def _stream_handle(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _WorkspacePool:
+    """Zero-filled scratch buffers per (device, stream, kind).
+
+    Each entry point leaves its workspace zero-filled when it returns, so a
+    buffer is zeroed once at allocation and reused in stream order."""
+
+    def __init__(self):
+        self._bufs: dict = {}
+        self._lock = threading.Lock()
+
+    def get(self, device: torch.device, stream: int, kind: str, nbytes: int) -> torch.Tensor:
+        key = (device.index, stream, kind)
+        with self._lock:
+            buf = self._bufs.get(key)
+            if buf is None or buf.numel() < nbytes:
+                buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
+                self._bufs[key] = buf
+            return buf
+
+
+_WS = _WorkspacePool()
+
+
+def _on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch, where it is not already."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)

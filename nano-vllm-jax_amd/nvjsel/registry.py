@@ -72,6 +72,9 @@ _SPECS = {
             "sample_topk_topp",
             "derive_rng_keys",
             "lm_head_logits",
+            "lm_head_w4",
+            "beam_search_select",
+            "reorder_beam_states",
         ),
         implemented=True,
         description="Hand-written HIP kernels for gfx950 behind the libnvjsel C ABI.",

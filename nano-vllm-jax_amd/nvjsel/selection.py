@@ -15,62 +15,17 @@ Mirrors:
   ``sample_topk_topp(logits, temperature, top_k, top_p, rng_state) -> token_ids``.
 * ``derive_rng_keys``          <- the executor's key derivation
   (nanovllm_jax/engine/model_executor.py:2131, 2214-2219, 2231).
+
+The LM-head entry points also take a 4-bit weight (``w4.W4Weight``) in place of
+the weight tensor.
 """
 from __future__ import annotations
-
-import threading
 
 import torch
 
 from . import _lib
-
-_TORCH_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
-
-
-def _dtype_code(t: torch.Tensor, what: str) -> int:
-    try:
-        return _TORCH_DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"unsupported {what} dtype: {t.dtype}") from None
-
-
-def _require_cuda(*ts: torch.Tensor) -> torch.device:
-    dev = ts[0].device
-    for t in ts:
-        if t is None:
-            continue
-        if t.device.type != "cuda":
-            raise ValueError("nvjsel kernels take device tensors (got a CPU tensor)")
-        if t.device != dev:
-            raise ValueError("all tensors must live on one device")
-    return dev
-
-
-def _stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _WorkspacePool:
-    """Zero-filled scratch buffers per (device, stream, kind).
-
-    Each entry point leaves its workspace zero-filled when it returns, so a
-    buffer is zeroed once at allocation and reused in stream order."""
-
-    def __init__(self):
-        self._bufs: dict = {}
-        self._lock = threading.Lock()
-
-    def get(self, device: torch.device, stream: int, kind: str, nbytes: int) -> torch.Tensor:
-        key = (device.index, stream, kind)
-        with self._lock:
-            buf = self._bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
-                buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
-                self._bufs[key] = buf
-            return buf
-
-
-_WS = _WorkspacePool()
+from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _require_cuda, _stream_handle
+from .w4 import W4Weight, w4_greedy as _w4_greedy, w4_logits as _w4_logits
 
 
 def _keys_as_i32(rng_keys: torch.Tensor, batch: int) -> torch.Tensor:
@@ -153,6 +108,9 @@ def lm_head_greedy_top1_hip(hidden_norm: torch.Tensor, output_weight: torch.Tens
     casts to ``act_dtype`` (``lm_head_decode_act_dtype``) and multiplies, in
     one launch on the streaming and bf16 tile paths."""
     x = _flatten_hidden(hidden_norm, require_3d=False)
+    if isinstance(output_weight, W4Weight):
+        x = x if norm_weight is None else rms_norm_hip(x, norm_weight, rms_norm_eps, act_dtype)
+        return _w4_greedy(x, output_weight, weight_layout, reduce_cast, return_best)
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
     if batch <= 0 or hidden_dim <= 0 or output_weight.numel() == 0:
         raise ValueError("LM-head top1 requires non-empty dimensions")
@@ -258,6 +216,10 @@ def lm_head_sample_token_ids(hidden_norm: torch.Tensor, output_weight: torch.Ten
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
     if batch <= 0 or hidden_dim <= 0:
         raise ValueError("LM-head sampling requires non-empty dimensions")
+    if isinstance(output_weight, W4Weight):
+        x = x if norm_weight is None else rms_norm_hip(x, norm_weight, rms_norm_eps, act_dtype)
+        logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
+        return sample_token_ids(logits, temperatures, rng_keys, top_k=top_k, top_p=top_p)
     hd = _dtype_code(x, "hidden")
     wd = _dtype_code(output_weight, "weight")
     w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
@@ -316,6 +278,8 @@ def lm_head_logits_hip(hidden_norm: torch.Tensor, output_weight: torch.Tensor, *
     model.py:765-780): fp32 accumulation; bf16 x bf16 gives bf16 logits and f16 x f16 f16 logits (the
     reference's dot output), other operand types f32 logits."""
     x = _flatten_hidden(hidden_norm, require_3d=False)
+    if isinstance(output_weight, W4Weight):
+        return _w4_logits(x, output_weight, weight_layout, reduce_cast)
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
     if batch <= 0 or hidden_dim <= 0 or output_weight.numel() == 0:
         raise ValueError("LM-head logits require non-empty dimensions")
@@ -419,10 +383,14 @@ def lm_head_token_ids_and_topk(hidden: torch.Tensor, output_weight: torch.Tensor
         ids = lm_head_greedy_top1_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
                                       norm_weight=norm_weight, rms_norm_eps=rms_norm_eps, act_dtype=act_dtype)
         return ids.reshape(batch, width), None, None
-    w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
-    x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
-    rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
-    logits = _dense_logits(x.contiguous(), w, layout, vocab, rc)
+    if isinstance(output_weight, W4Weight):
+        x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
+        logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
+    else:
+        w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
+        x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
+        rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
+        logits = _dense_logits(x.contiguous(), w, layout, vocab, rc)
     values, indices = topk_hip(logits, int(top_k))
     ids = indices[:, 0].reshape(batch, width)
     return ids, values.reshape(batch, width, -1), indices.reshape(batch, width, -1)
@@ -438,7 +406,9 @@ def mtp_greedy_top1_token_ids(x_normed: torch.Tensor, output_weight: torch.Tenso
     if x_normed.ndim != 3:
         raise ValueError("HIP MTP greedy top1 expects hidden shape [B, T, H]")
     batch, seq_len, hidden_dim = (int(d) for d in x_normed.shape)
-    flat = x_normed.reshape(batch * seq_len, 1, hidden_dim).to(output_weight.dtype)
+    flat = x_normed.reshape(batch * seq_len, 1, hidden_dim)
+    if not isinstance(output_weight, W4Weight):  # a 4-bit weight takes the activations as they are
+        flat = flat.to(output_weight.dtype)
     ids = lm_head_greedy_top1_hip(flat, output_weight, weight_layout=weight_layout)
     return ids.reshape(batch, seq_len)
 
