@@ -9,39 +9,46 @@
 // exactly, so one shift and one and-or make two operands.  The accumulator of
 // a group starts at -(16 + z) times the group's sum of activations, so that
 // the offset is gone when the group ends; then it is scaled into the row's
-// total.  Sums are fp32 throughout (the activations' group sums fp64, rounded
-// once).  The offset is the smallest one that an exponent's mantissa holds: with
-// 128 + q (no shift for a quarter of the nibbles) the partial sums are six
-// times larger than the result's terms, and so is their rounding.
+// total.  Sums are fp32 throughout.  The offset is the smallest one that an
+// exponent's mantissa holds: with 128 + q (no shift for a quarter of the nibbles)
+// the partial sums are six times larger than the result's terms, and so is their
+// rounding.
 //
-// Packed layout (w4_pack_kernel): blocks of 16 vocabulary rows x 128 k, 1 KB
-// each, in the order in which a wave's 16-byte loads feed the matrix
-// instructions: lane l holds row l & 15, word j the eight k at 32 j + 8 (l >> 4),
-// the nibble of k = 2 p at bits 4 p, of 2 p + 1 at 16 + 4 p.  All k blocks of 16 rows lie
-// together, then the next 16 rows.  The scales follow, 16 rows x 128 / group
-// per block, and the zero points in the same order.  Rows past V and k past H
-// are zero with scale zero.
+// Packed layout (w4_pack_kernel): blocks of 32 vocabulary rows x 128 k, 2 KB
+// each, in the order in which a wave's 16-byte loads feed the 16x16x32 matrix
+// instructions: piece t (1 KB), lane l, word j hold row 16 t + (l & 15) and the
+// eight k at 32 j + 8 (l >> 4), the nibble of the even k = 2 p at bits 4 p, of 2 p + 1
+// at 16 + 4 p.  All k blocks of 32 rows lie together, then the next 32 rows.  The
+// scales follow, per block [row of 16][t][128 / group], and the zero points in the
+// same order.  Rows past V and k past H are zero with scale zero.
+//
+// What bounds it: the weights' stream (7 TB/s), and beside it the sum of vector
+// and matrix instructions, which overlap little on a SIMD: measured with two
+// waves, 2.5 clocks for a shift or an or, 4.5 for v_and_or_b32 or an fma, 17 for
+// the 16x16x32 product and 33 for the 32x32x16 one, so the smaller tile costs
+// half where up to 16 batch rows are there and nothing where there are more.
 #pragma once
 #include "lm_head_common.h"
 
 namespace nvjsel {
 
 static constexpr int kW4Waves = 8, kW4Threads = 64 * kW4Waves;
+static constexpr size_t kW4Lds = 150 * 1024;  // for the hidden and its groups' sums
 
 struct W4Layout {
-  int tiles, kblocks, ng;  // 16-row tiles, 128-wide k blocks, groups per k block
+  int tiles, kblocks, ng;  // 32-row tiles, 128-wide k blocks, groups per k block
   size_t scales, zeros, total;  // byte offsets of the parts, and the size
 };
 
 __host__ __device__ inline W4Layout w4_layout(int V, int H, int group, bool zeros) {
   W4Layout w;
-  w.tiles = (V + 15) / 16;
+  w.tiles = (V + 31) / 32;
   w.kblocks = (H + 127) / 128;
   w.ng = 128 / group;
   const size_t blocks = (size_t)w.tiles * w.kblocks;
-  w.scales = blocks * 1024;
-  w.zeros = w.scales + (blocks * 16 * w.ng * 2 + 255) / 256 * 256;
-  w.total = w.zeros + (zeros ? (blocks * 16 * w.ng + 255) / 256 * 256 : 0);
+  w.scales = blocks * 2048;
+  w.zeros = w.scales + (blocks * 32 * w.ng * 2 + 255) / 256 * 256;
+  w.total = w.zeros + (zeros ? (blocks * 32 * w.ng + 255) / 256 * 256 : 0);
   return w;
 }
 
@@ -52,7 +59,7 @@ struct W4Args {
   int scale_dtype;
   int zeros;   // zero points are there
   int V, H;
-  int B, rows;  // batch rows of this pass; their slots in LDS (a power of two up to 16, or 16 MB)
+  int B;       // batch rows of this pass
   int kc;      // k blocks of the hidden in LDS at a time
   int reduce_cast;
   unsigned long long* row_keys;
@@ -64,275 +71,480 @@ struct W4Args {
   long long out_stride;
 };
 
-// 16 + q of the eight nibbles of a packed word, as bf16 or f16 pairs.
+// 16 + q of the eight nibbles of a packed word, as bf16 or f16 pairs.  The mask and
+// the exponents are held in registers: as literals they take two instructions a
+// pair where v_and_or_b32 takes one (V = 248,320, H = 1024, one row 29.1 against 28.0 us).
+struct W4Consts {
+  uint32_t mask, base;
+};
 template <int FMT>
-__device__ __forceinline__ u32x4_t w4_unpack(uint32_t w) {
-  u32x4_t r;
+__device__ __forceinline__ W4Consts w4_consts() {
+  W4Consts c;
   if constexpr (FMT == DT_BF16) {  // mantissa bits 3..6
-    r.x = ((w << 3) & 0x00780078u) | 0x41804180u;
-    r.y = ((w >> 1) & 0x00780078u) | 0x41804180u;
-    r.z = ((w >> 5) & 0x00780078u) | 0x41804180u;
-    r.w = ((w >> 9) & 0x00780078u) | 0x41804180u;
+    asm("s_mov_b32 %0, 0x00780078" : "=s"(c.mask));
+    asm("v_mov_b32 %0, 0x41804180" : "=v"(c.base));
   } else {  // mantissa bits 6..9
-    r.x = ((w << 6) & 0x03C003C0u) | 0x4C004C00u;
-    r.y = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
-    r.z = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u;
-    r.w = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+    asm("s_mov_b32 %0, 0x03c003c0" : "=s"(c.mask));
+    asm("v_mov_b32 %0, 0x4c004c00" : "=v"(c.base));
+  }
+  return c;
+}
+template <int FMT>
+__device__ __forceinline__ u32x4_t w4_unpack(uint32_t w, const W4Consts& c) {
+  u32x4_t r;
+  if constexpr (FMT == DT_BF16) {
+    r.x = ((w << 3) & c.mask) | c.base;
+    r.y = ((w >> 1) & c.mask) | c.base;
+    r.z = ((w >> 5) & c.mask) | c.base;
+    r.w = ((w >> 9) & c.mask) | c.base;
+  } else {
+    r.x = ((w << 6) & c.mask) | c.base;
+    r.y = ((w << 2) & c.mask) | c.base;
+    r.z = ((w >> 2) & c.mask) | c.base;
+    r.w = ((w >> 6) & c.mask) | c.base;
   }
   return r;
 }
 
 // k blocks kb0 .. of the hidden into LDS, as the matrix instructions' operands:
-// 16-byte slots [(4 kb + j) MB TERMS + mb TERMS + t][k eighth][row].  Three terms: x =
-// the bf16 values that its leading, next and last eight bits make (exact); a
-// value that is not finite keeps its first term only.  Then the sums of each
-// group's activations, [group][16 MB].
-template <int FMT, int TERMS, int MB, int NG>
-__device__ __forceinline__ void w4_stage_hidden(const W4Args& a, int kb0, int nkb, u32x4_t* frag, float* xsum) {
-  const int lane = (int)threadIdx.x & 63, u = lane & 15, j = u >> 2, qd = u & 3;
-  const int items = a.rows * nkb;  // 16 lanes each
-  const int rt = a.rows < 16 ? a.rows : 16;
-  for (int it = (int)threadIdx.x >> 4; it < items; it += kW4Threads / 16) {
-    const int row = it % a.rows, kb = it / a.rows, k = (kb0 + kb) * 128 + 8 * u;
-    float x[8];
-    if (row < a.B && k < a.H) {
-      load8_as_f32(a.hidden, a.hidden_dtype, (size_t)row * a.H + k, x);
-    } else {
+// 16-byte slots [((4 kb + j) MB + mb) TERMS + t][k quarter][row of RT].  Three terms: x =
+// the bf16 values that its leading, next and last eight bits make (exact); a value
+// that is not finite keeps its first term only.  Then, by the matrix cores, the
+// groups' sums of activations times -1 (zero points) or -(16 + 8): xsum [group][16 MB].
+// first(): the loads that may be on their way while the weights' first ones are
+// requested; rest(): everything else.
+template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS>
+struct W4Stage {
+  static constexpr int U = TERMS == 1 ? 8 : 4, EACH = kW4Threads / 16, LD = TERMS == 1 ? 1 : 2;
+  u32x4_t v[U][LD];
+
+  __device__ __forceinline__ void load(const W4Args& a, int kb0, int items, int it0) {
+    const int u = (int)threadIdx.x & 15;  // eight k of a k block
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    }
-    const int mb = row >> 4, slot = row & 15;
-    u32x4_t* dst = frag + ((size_t)((kb * 4 + j) * MB + mb) * TERMS * 4 + qd) * rt + slot;
-    uint32_t h[TERMS][8];
+    for (int i = 0; i < U; ++i) {
+      const int it = it0 + i * EACH, row = it % (RT * MB), k = (kb0 + it / (RT * MB)) * 128 + 8 * u;
+      const bool in = it < items && row < a.B && k < a.H;
+      const size_t at = in ? (size_t)row * a.H + k : 0;  // always a load, of the first values where none is wanted
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (TERMS == 1) {
-        h[0][e] = FMT == DT_BF16 ? bf16_bits_rne(x[e]) : f16_bits(x[e]);
-      } else {
-        const uint32_t b = __float_as_uint(x[e]);
-        const bool fin = (b & 0x7F800000u) != 0x7F800000u;
-        h[0][e] = fin ? b >> 16 : bf16_bits_rne(x[e]);
-        const float r1 = x[e] - __uint_as_float(b & 0xFFFF0000u);
-        h[1][e] = fin ? __float_as_uint(r1) >> 16 : 0u;
-        const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xFFFF0000u);
-        h[2][e] = fin ? __float_as_uint(r2) >> 16 : 0u;
+      for (int h = 0; h < LD; ++h) {
+        if constexpr (TERMS == 1) v[i][h] = *(const u32x4_any_t*)((const uint16_t*)a.hidden + at);
+        else v[i][h] = *(const u32x4_any_t*)((const float*)a.hidden + at + 4 * h);
       }
     }
-#pragma unroll
-    for (int t = 0; t < TERMS; ++t)
-      dst[t * 4 * rt] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16,
-                                h[t][6] | h[t][7] << 16};
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += (double)x[e];
-#pragma unroll
-    for (int m = 1; m < 16 / NG; m <<= 1) sum += __shfl_xor(sum, m, 64);
-    if (u % (16 / NG) == 0) xsum[(kb * NG + u / (16 / NG)) * 16 * MB + row] = (float)sum;
   }
-}
+  __device__ __forceinline__ void store(const W4Args& a, int kb0, int items, int it0, u32x4_t* frag) {
+    const int u = (int)threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int it = it0 + i * EACH, row = it % (RT * MB), kb = it / (RT * MB), k = (kb0 + kb) * 128 + 8 * u;
+      if (it >= items) break;
+      const bool in = row < a.B && k < a.H;
+      u32x4_t* dst = frag + (((kb * 4 + (u >> 2)) * MB + row / RT) * TERMS * 4 + (u & 3)) * RT + row % RT;
+      if constexpr (TERMS == 1) {
+        *dst = in ? v[i][0] : u32x4_t{0u, 0u, 0u, 0u};
+      } else {
+        uint32_t h[3][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t b = in ? v[i][e >> 2][e & 3] : 0u;
+          const float x = __uint_as_float(b);
+          const bool fin = (b & 0x7F800000u) != 0x7F800000u;
+          h[0][e] = fin ? b >> 16 : bf16_bits_rne(x);
+          const float r1 = x - __uint_as_float(b & 0xFFFF0000u);
+          h[1][e] = fin ? __float_as_uint(r1) >> 16 : 0u;
+          const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xFFFF0000u);
+          h[2][e] = fin ? __float_as_uint(r2) >> 16 : 0u;
+        }
+#pragma unroll
+        for (int t = 0; t < 3; ++t)
+          dst[t * 4 * RT] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16,
+                                    h[t][6] | h[t][7] << 16};
+      }
+    }
+  }
+  __device__ __forceinline__ void first(const W4Args& a, int kb0, int nkb) {
+    load(a, kb0, RT * MB * nkb, (int)threadIdx.x >> 4);
+  }
+  __device__ __forceinline__ void rest(const W4Args& a, int kb0, int nkb, u32x4_t* frag, float* xsum) {
+    const int items = RT * MB * nkb;
+    store(a, kb0, items, (int)threadIdx.x >> 4, frag);
+    for (int it0 = ((int)threadIdx.x >> 4) + U * EACH; it0 < items; it0 += U * EACH) {
+      load(a, kb0, items, it0);
+      store(a, kb0, items, it0, frag);
+    }
+    __syncthreads();
+    const int lane = (int)threadIdx.x & 63;
+    const uint32_t one =
+        ZEROS ? (FMT == DT_BF16 ? 0xBF80BF80u : 0xBC00BC00u) : (FMT == DT_BF16 ? 0xC1C0C1C0u : 0xCE00CE00u);
+    const u32x4_t ones{one, one, one, one};
+    const u32x4_t* mine = frag + (lane >> 4) * RT + (lane & (RT - 1));
+    for (int g = (int)threadIdx.x >> 6; g < nkb * NG; g += kW4Waves) {
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        f32x4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4 / NG; ++j)
+#pragma unroll
+          for (int c = TERMS - 1; c >= 0; --c)
+            d = mfma16x16x32<FMT>(mine[(((g * (4 / NG) + j) * MB + m) * TERMS + c) * 4 * RT], ones, d);
+        if ((lane & 15) == 0) *(f32x4_t*)(xsum + (g * MB + m) * 16 + 4 * (lane >> 4)) = d;
+      }
+    }
+    __syncthreads();
+  }
+};
 
-// One block per CU, eight waves.  A wave takes NT adjacent tiles of 16
-// vocabulary rows at a time and runs over all of H, its next k blocks' 1 KB pieces
-// on the way in registers (DEPTH); the waves share the hidden in LDS, all of it
-// where it fits and kc k blocks at a time where not.  Matrix tile: M = batch
-// rows, N = vocabulary rows, so that a lane's four results share their scale.
-template <int FMT, int TERMS, int MB, int NT, int NG, int MODE>
+// One block per CU, eight waves.  A wave takes a block of 32 vocabulary rows at a
+// time and runs over all of H, its next k blocks' pieces on the way in registers
+// (DEPTH); the waves share the hidden in LDS, all of it where it fits, kc k blocks at
+// a time where not (STAGED).  Matrix tile: M = batch rows (MB tiles of 16), N =
+// vocabulary rows, so that a lane's results share their scale.  RT: batch rows that
+// have slots in LDS (4: the others repeat them).
+//
+// Rows go round all waves of the device while every wave gets some; what is left is
+// dealt to the blocks, and a block splits its rest by k blocks over its waves, which
+// join their parts through LDS at the end (V = 151,936, H = 2560, 8 rows: 46 us with
+// whole tiles only, 2.3 rounds of them, 42 split).  STAGED waves walk the k blocks
+// together and repeat the last tile instead.
+template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, bool STAGED, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int DEPTH = 3;
-  const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, a.zeros != 0);
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int KB = lay.kblocks, kc = a.kc, rt = a.rows < 16 ? a.rows : 16;
+  constexpr int DEPTH = 4, NT = 2;
+  const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int KB = lay.kblocks, kc = a.kc, col = lane & 15;
   u32x4_t* frag = (u32x4_t*)lds;
-  float* xsum = (float*)(lds + (size_t)kc * 4 * MB * TERMS * 4 * rt * 16);
-  const int supers = (lay.tiles + NT - 1) / NT;
-  const int step = (int)gridDim.x * kW4Waves;
-  const int first = (int)blockIdx.x * kW4Waves + wave;
-  const int rounds = (supers - (int)blockIdx.x * kW4Waves + step - 1) / step;  // of the block: some waves repeat the last tile
-  const int n = rounds * KB;
+  float* xsum = (float*)(lds + (size_t)kc * 256 * TERMS * RT * MB);
+  const u32x4_t* mine = frag + (lane >> 4) * RT + (lane & (RT - 1));
+  const float* xmine = xsum + 4 * (lane >> 4);
 
-  const u32x4_t* wq = (const u32x4_t*)a.packed;
-  const uint8_t* sc = a.packed + lay.scales;
-  const uint8_t* zp = a.packed + lay.zeros;
+  const int step = (int)gridDim.x * kW4Waves, first = (int)blockIdx.x * kW4Waves + wave;
+  const int full = STAGED ? (lay.tiles - (int)blockIdx.x * kW4Waves + step - 1) / step : lay.tiles / step;  // whole rounds
+  // the block's rest: tiles from rest0, its k blocks dealt to the waves
+  int rest0 = 0, nrest = 0;
+  if (!STAGED) {
+    const int rest = lay.tiles - full * step;
+    const int each = (int)((unsigned)rest / gridDim.x), more = rest - each * (int)gridDim.x, b = (int)blockIdx.x;
+    const int r0 = each * b + (b < more ? b : more), r1 = r0 + each + (b < more);
+    rest0 = full * step + r0;
+    nrest = (r1 - r0) * KB;
+  }
+  auto from = [&](int w) { return (int)((unsigned)(nrest * w) / kW4Waves); };  // first k block of wave w's part
+  const int p0 = from(wave), p1 = from(wave + 1);
+  const int n = full * KB + p1 - p0;
+  const int tail_tile = rest0 + p0 / KB, tail_kb = p0 % KB;
 
+  const W4Consts consts = w4_consts<FMT>();
+  const uint32_t bf16_mask = a.scale_dtype == DT_BF16 ? 0xFFFFFFFFu : 0u;
+  const uint32_t zoff = (uint32_t)(col * 2 * NG) & ~3u, zshift = NG == 1 ? (col & 1) * 16 : 0;
+
+  // Scales and zero points are loaded as the aligned words that hold them: a 16-bit
+  // load's extension would be waited for a round of the ring early.
   struct Item {
     u32x4_t w[NT];
-    uint32_t s[NT][(NG + 1) / 2];
-    uint32_t z[NT];
+    uint32_t s[NG];  // two 16-bit scales each: [t][g]
+    uint32_t z[(NG + 1) / 2];
   };
   Item ring[DEPTH];
 
-  // the item to be requested next
-  int lkb = 0, lsuper = first;
-  auto load = [&](auto D, int) NVJSEL_INLINE {
+  int lkb = full ? 0 : tail_kb, ltile = full ? first : tail_tile, lfull = full;  // the item to be requested next
+  auto load = [&](auto D) NVJSEL_INLINE {
     Item& it = ring[decltype(D)::value];
+    const int tile = ltile < lay.tiles ? ltile : lay.tiles - 1;
+    const size_t blk = (size_t)tile * KB + lkb;
+    const u32x4_t* wb = (const u32x4_t*)(a.packed + blk * 2048) + lane;
+    it.w[0] = __builtin_nontemporal_load(wb);
+    it.w[1] = __builtin_nontemporal_load(wb + 64);
+    const uint32_t* sb = (const uint32_t*)(a.packed + lay.scales + blk * (64 * NG)) + col * NG;
+    if constexpr (NG == 4) {
+      const u32x4_t v = *(const u32x4_t*)sb;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      int tile = lsuper * NT + t;
-      tile = tile < lay.tiles ? tile : lay.tiles - 1;
-      const size_t blk = (size_t)tile * KB + lkb;
-      it.w[t] = __builtin_nontemporal_load(wq + blk * 64 + lane);
-      const size_t m = blk * 16 + (lane & 15);
-      if constexpr (NG == 1) it.s[t][0] = ((const uint16_t*)sc)[m];
-      else if constexpr (NG == 2) it.s[t][0] = ((const uint32_t*)sc)[m];
-      else {
-        const uint64_t v = ((const uint64_t*)sc)[m];
-        it.s[t][0] = (uint32_t)v;
-        it.s[t][1] = (uint32_t)(v >> 32);
-      }
-      if (a.zeros) {
-        if constexpr (NG == 1) it.z[t] = zp[m];
-        else if constexpr (NG == 2) it.z[t] = ((const uint16_t*)zp)[m];
-        else it.z[t] = ((const uint32_t*)zp)[m];
-      } else it.z[t] = 0x08080808u;
+      for (int g = 0; g < 4; ++g) it.s[g] = v[g];
+    } else if constexpr (NG == 2) {
+      const uint64_t v = *(const uint64_t*)sb;
+      it.s[0] = (uint32_t)v;
+      it.s[1] = (uint32_t)(v >> 32);
+    } else it.s[0] = *sb;
+    if constexpr (ZEROS) {
+      const uint8_t* zb = a.packed + lay.zeros + blk * (32 * NG) + zoff;
+      if constexpr (NG == 4) {
+        const uint64_t v = *(const uint64_t*)zb;
+        it.z[0] = (uint32_t)v;
+        it.z[1] = (uint32_t)(v >> 32);
+      } else it.z[0] = *(const uint32_t*)zb;
     }
-    if (++lkb == KB) { lkb = 0; lsuper += step; }
+    if (++lkb == KB) {
+      --lfull;
+      lkb = lfull == 0 ? tail_kb : 0;
+      ltile = lfull == 0 ? tail_tile : lfull > 0 ? ltile + step : ltile + 1;
+    }
   };
 
-  f32x4_t total[NT][MB];
-  unsigned long long best[MB][4];
+  // greedy: the best so far of each row among this lane's columns; no index yet: ~0, beside a NaN
+  float total[NT][MB][4], bval[MB][4], foreign[NT][MB][4];
+  uint32_t bidx[MB][4];
 #pragma unroll
-  for (int m = 0; m < MB; ++m) {
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) best[m][i] = 0ull;
+    for (int i = 0; i < 4; ++i) {
+      bval[m][i] = NAN;
+      bidx[m][i] = 0xFFFFFFFFu;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) total[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
+      for (int t = 0; t < NT; ++t) total[t][m][i] = foreign[t][m][i] = 0.0f;
+    }
 
-  const int arow = (lane & 15) < rt ? (lane & 15) : rt - 1;
-  int kb = 0, kl = 0, super = first;  // the item in work; kl: its k block in LDS
-  auto body = [&](auto D, int) NVJSEL_INLINE {
-    if (kc < KB && kl == 0) {
+  // A tile's totals are whole: rounded, and scored or stored.
+  auto finish_tile = [&](int tile) NVJSEL_INLINE {
+    if (a.reduce_cast == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) total[t][m][i] = round_bf16(total[t][m][i]);
+    } else if (a.reduce_cast == 2) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) total[t][m][i] = round_f16(total[t][m][i]);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int v = tile * 32 + 16 * t + col;
+      const bool in = tile < lay.tiles && v < a.V;
+      if constexpr (MODE == MODE_GREEDY) {
+        bool up = false;  // seldom: a lane's best of so many tiles
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) up |= !(total[t][m][i] <= bval[m][i]);
+        if (__any(up && in)) {
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = total[t][m][i], y = bval[m][i];  // in order of index: equal ones stay, the first NaN too
+              if (in && (bidx[m][i] == 0xFFFFFFFFu || x > y || (x != x && y == y))) {
+                bval[m][i] = x;
+                bidx[m][i] = (uint32_t)v;
+              }
+            }
+        }
+      } else {
+        auto store = [&](auto* out) NVJSEL_INLINE {
+          typedef typename std::remove_reference<decltype(*out)>::type T;
+          T* p = out + v;
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int b = 16 * m + 4 * (lane >> 4) + i;
+              if (in && b < a.B) p[(size_t)b * (size_t)a.out_stride] = (T)total[t][m][i];
+            }
+        };
+        if (a.out_dtype == DT_F32) store((float*)a.out_logits);
+        else if (a.out_dtype == DT_BF16) store((__bf16*)a.out_logits);
+        else store((_Float16*)a.out_logits);
+      }
+    }
+  };
+
+  int kb = full ? 0 : tail_kb, tile = full ? first : tail_tile, left = full;  // the item in work
+  int kl = 0;  // its k block in LDS (STAGED)
+  auto body = [&](auto D) NVJSEL_INLINE {
+    if (STAGED && kl == 0) {
       __syncthreads();
-      w4_stage_hidden<FMT, TERMS, MB, NG>(a, kb, KB - kb < kc ? KB - kb : kc, frag, xsum);
-      __syncthreads();
+      W4Stage<FMT, TERMS, MB, RT, NG, ZEROS> st;
+      st.first(a, kb, KB - kb < kc ? KB - kb : kc);
+      st.rest(a, kb, KB - kb < kc ? KB - kb : kc, frag, xsum);
     }
     const Item& it = ring[decltype(D)::value];
+    const int kx = STAGED ? kl : kb;
+    const u32x4_t* fk = mine + kx * (4 * MB * TERMS * 4 * RT);
+    const float* xk = xmine + kx * (NG * MB * 16);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       f32x4_t acc[NT][MB];
 #pragma unroll
       for (int m = 0; m < MB; ++m) {
-        const f32x4_t xs = *(const f32x4_t*)(xsum + (kl * NG + g) * 16 * MB + 16 * m + 4 * (lane >> 4));
+        const f32x4_t xs = *(const f32x4_t*)(xk + (g * MB + m) * 16);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float z = -16.0f - (float)((it.z[t] >> (8 * g)) & 0xFFu);
-          acc[t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
+          if constexpr (ZEROS) {
+            const int zi = t * NG + g;  // byte of the block's zero points of this row
+            const float z = 16.0f + (float)((it.z[zi >> 2] >> (zshift + 8 * (zi & 3))) & 0xFFu);
+            acc[t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
+          } else acc[t][m] = xs;
         }
       }
 #pragma unroll
       for (int j = g * 4 / NG; j < (g + 1) * 4 / NG; ++j) {
         u32x4_t wf[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) wf[t] = w4_unpack<FMT>(it.w[t][j]);
+        for (int t = 0; t < NT; ++t) wf[t] = w4_unpack<FMT>(it.w[t][j], consts);
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int c = 0; c < TERMS; ++c) {
-            const u32x4_t xf = frag[((size_t)((kl * 4 + j) * MB + m) * TERMS * 4 + c * 4 + (lane >> 4)) * rt + arow];
+          for (int c = TERMS - 1; c >= 0; --c) {
+            const u32x4_t xf = fk[((j * MB + m) * TERMS + c) * 4 * RT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t][m] = mfma16x16x32<FMT>(xf, wf[t], acc[t][m]);
           }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint32_t sb = (it.s[t][g / 2] >> (16 * (g & 1))) & 0xFFFFu;
-        const float s = a.scale_dtype == DT_BF16 ? bf16_to_f32((uint16_t)sb) : f16_to_f32((uint16_t)sb);
+        const int si = t * NG + g;  // 16-bit scale of the block's scales of this row
+        const uint32_t sb = it.s[si >> 1] >> (16 * (si & 1));
+        const uint32_t fh = __float_as_uint(f16_to_f32((uint16_t)sb));
+        const float s = __uint_as_float((sb << 16 & bf16_mask) | (fh & ~bf16_mask));
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) total[t][m][i] = __builtin_fmaf(s, acc[t][m][i], total[t][m][i]);
       }
     }
-    if (++kl == kc) kl = 0;
+    ++kl;
+    if (STAGED && kl == kc) kl = 0;
     if (++kb < KB) return;
-    kb = kl = 0;
+    if (!STAGED && left == 0 && tile == tail_tile && tail_kb != 0) {  // the end of another wave's tile
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int tile = super * NT + t, v = tile * 16 + (lane & 15);
-      const bool in = tile < lay.tiles && v < a.V;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) foreign[t][m][i] = total[t][m][i];
+    } else {
+      finish_tile(tile);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int b = 16 * m + 4 * (lane >> 4) + i;
-          const float val = apply_cast(total[t][m][i], a.reduce_cast);
-          if constexpr (MODE == MODE_GREEDY) {
-            if (in && b < a.B) best[m][i] = max_u64(best[m][i], argmax_key(val, (uint32_t)v));
-          } else if (in && b < a.B) {
-            const size_t o = (size_t)b * (size_t)a.out_stride + (size_t)v;
-            if (a.out_dtype == DT_F32) ((float*)a.out_logits)[o] = val;
-            else if (a.out_dtype == DT_BF16) ((__bf16*)a.out_logits)[o] = (__bf16)val;
-            else ((_Float16*)a.out_logits)[o] = (_Float16)val;
-          }
-          total[t][m][i] = 0.0f;
-        }
-    }
-    super += step;
+        for (int i = 0; i < 4; ++i) total[t][m][i] = 0.0f;
+    kl = 0;
+    if (left > 0) --left;  // as the loads go
+    const bool to_tail = left == 0 && (tile < rest0 || STAGED);
+    kb = to_tail ? tail_kb : 0;
+    tile = to_tail ? tail_tile : left > 0 ? tile + step : tile + 1;
   };
 
-  ring_pipeline<DEPTH>(n, load, body, [&]() NVJSEL_INLINE {
-    if (kc >= KB) {
-      w4_stage_hidden<FMT, TERMS, MB, NG>(a, 0, KB, frag, xsum);
-      __syncthreads();
-    }
+  // Every load is unconditional (tiles past the end repeat the last one), so that the
+  // waits count the same requests on every path to a body: with bounds tests before
+  // the first loads each round of the ring waited for all of it.
+  {
+    W4Stage<FMT, TERMS, MB, RT, NG, ZEROS> st;
+    if (!STAGED) st.first(a, 0, KB);
+    static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE { load(D); });
+    if (!STAGED) st.rest(a, 0, KB, frag, xsum);
+  }
+  int i = 0;
+  for (; i + DEPTH <= n; i += DEPTH)
+    static_for<DEPTH>([&](auto D) NVJSEL_INLINE {
+      load(std::integral_constant<int, (decltype(D)::value + DEPTH - 1) % DEPTH>{});
+      body(D);
+    });
+  static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE {
+    if (i + decltype(D)::value < n) body(D);
   });
 
-  if constexpr (MODE == MODE_GREEDY) {
+  if (nrest) {  // block-uniform: the parts of tiles meet
     __syncthreads();  // the hidden in LDS has been read
+    float* part = (float*)lds;  // [wave][t][m][i][lane]
+    const int pend = p1 % KB != 0 && p1 > p0 ? p1 / KB : -1;  // this wave's last tile is not whole
+    const bool owns = pend >= 0 && pend * KB >= p0;           // and begins here
+    if (p1 > p0 && tail_kb != 0) {
+      const bool ended = (p0 / KB + 1) * KB <= p1;  // its part reaches the tile's end: set aside; else still in total
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            part[(((wave * NT + t) * MB + m) * 4 + i) * 64 + lane] = ended ? foreign[t][m][i] : total[t][m][i];
+    }
+    __syncthreads();
+    if (owns) {
+      for (int w = wave + 1; w < kW4Waves && from(w) < (pend + 1) * KB; ++w) {
+        if (from(w + 1) == from(w)) continue;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[t][m][i] += part[(((w * NT + t) * MB + m) * 4 + i) * 64 + lane];
+      }
+      finish_tile(rest0 + pend);
+    }
+  }
+
+  if constexpr (MODE == MODE_GREEDY) {
+    __syncthreads();  // LDS has been read
     unsigned long long* red = (unsigned long long*)lds;
 #pragma unroll
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        unsigned long long k = best[m][i];
+        unsigned long long k = bidx[m][i] == 0xFFFFFFFFu ? 0ull : argmax_key(bval[m][i], bidx[m][i]);
 #pragma unroll
         for (int x = 8; x >= 1; x >>= 1) k = max_u64(k, shfl_xor_u64(k, x));
-        if ((lane & 15) == 0) red[wave * 16 * MB + 16 * m + 4 * (lane >> 4) + i] = k;
+        if (col == 0) red[wave * 16 * MB + 16 * m + 4 * (lane >> 4) + i] = k;
       }
     block_commit<kW4Waves, 16 * MB>(red, a.B, a.row_keys);
     finish_rows(a.row_keys, a.counter, a.B, a.out_ids, a.out_best);
   }
 }
 
-template <int FMT, int TERMS, int MB, int NG, int MODE>
+template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, int MODE>
 static int launch_w4(W4Args a, hipStream_t stream) {
-  constexpr int NT = 2;
-  auto kern = lm_head_w4_kernel<FMT, TERMS, MB, NT, NG, MODE>;
-  const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, a.zeros != 0);
-  a.rows = 16 * MB;
-  if (MB == 1) {
-    a.rows = 1;
-    while (a.rows < a.B) a.rows *= 2;
-  }
-  const size_t per_kb = (size_t)a.rows * 256 * TERMS + (size_t)NG * 16 * MB * 4;
-  const size_t most = 150 * 1024, red = (size_t)kW4Waves * 16 * MB * 8;
+  const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
+  const size_t per_kb = (size_t)RT * MB * 256 * TERMS + (size_t)NG * 16 * MB * 4;
+  const size_t parts = (size_t)kW4Waves * MB * 2048;  // of the tiles that waves split; the rows' keys need less
   int chunks = 1;
-  while ((size_t)((lay.kblocks + chunks - 1) / chunks) * per_kb > most) ++chunks;
+  while ((size_t)((lay.kblocks + chunks - 1) / chunks) * per_kb > kW4Lds) ++chunks;
   a.kc = (lay.kblocks + chunks - 1) / chunks;
   size_t lds = a.kc * per_kb;
-  if (lds < red) lds = red;
+  if (lds < parts) lds = parts;
+  auto kern = chunks == 1 ? lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, false, MODE>
+                          : lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, true, MODE>;
   if (lds > 48 * 1024)
     NVJSEL_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  const int supers = (lay.tiles + NT - 1) / NT, cus = device_cu_count();
-  const int need = (supers + kW4Waves - 1) / kW4Waves;
+  const int cus = device_cu_count(), need = chunks == 1 ? lay.tiles : (lay.tiles + kW4Waves - 1) / kW4Waves;
   hipLaunchKernelGGL(kern, dim3(need < cus ? need : cus), dim3(kW4Threads), lds, stream, a);
   NVJSEL_CHECK_LAUNCH("lm_head_w4_kernel");
   return NVJSEL_OK;
 }
 
-template <int FMT, int TERMS, int MB, int MODE>
+template <int FMT, int TERMS, int MB, int RT, int MODE>
 static int launch_w4_group(const W4Args& a, int group, hipStream_t s) {
-  if (group == 128) return launch_w4<FMT, TERMS, MB, 1, MODE>(a, s);
-  if (group == 64) return launch_w4<FMT, TERMS, MB, 2, MODE>(a, s);
-  return launch_w4<FMT, TERMS, MB, 4, MODE>(a, s);
+  if (a.zeros) {
+    if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, true, MODE>(a, s);
+    if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, true, MODE>(a, s);
+    return launch_w4<FMT, TERMS, MB, RT, 4, true, MODE>(a, s);
+  }
+  if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, false, MODE>(a, s);
+  if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, false, MODE>(a, s);
+  return launch_w4<FMT, TERMS, MB, RT, 4, false, MODE>(a, s);
 }
 
-// The passes by mode and activation type, each in a translation unit of its own
-// (lm_head_w4_bf16.hip, _f16.hip, _f32.hip): batch rows up to kW4Rows, kW4RowsF32 for f32.
-static constexpr int kW4Rows = 64, kW4RowsF32 = 32;
-int w4_pass_bf16(int mode, const W4Args& a, int group, hipStream_t s);
-int w4_pass_f16(int mode, const W4Args& a, int group, hipStream_t s);
-int w4_pass_f32(int mode, const W4Args& a, int group, hipStream_t s);
+template <int FMT, int TERMS, int MODE>
+static int w4_pass(const W4Args& a, int group, hipStream_t s) {
+  if (a.B <= 4) return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, s);
+  if (a.B <= 16) return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, s);
+  if (a.B <= 32) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, s);
+  return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, s);
+}
+
+// The passes by mode and activation type, each in a translation unit of its
+// own; up to kW4Rows batch rows.
+static constexpr int kW4Rows = 64;
+int w4_greedy_bf16(const W4Args& a, int group, hipStream_t s);
+int w4_greedy_f16(const W4Args& a, int group, hipStream_t s);
+int w4_greedy_f32(const W4Args& a, int group, hipStream_t s);
+int w4_logits_bf16(const W4Args& a, int group, hipStream_t s);
+int w4_logits_f16(const W4Args& a, int group, hipStream_t s);
+int w4_logits_f32(const W4Args& a, int group, hipStream_t s);
 
 }  // namespace nvjsel

@@ -4,8 +4,8 @@
 
 namespace nvjsel {
 
-// One thread per packed 32-bit word; thread 0 .. of a block's last words also
-// write the scales and zero points.
+// One thread per two packed 32-bit words of a block; the first ones also write
+// its scales and zero points.
 __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scales,
                                                       const uint8_t* __restrict__ zeros, int V, int H, int group,
                                                       uint8_t* __restrict__ packed) {
@@ -14,23 +14,26 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
   const int G = H / group;
   for (size_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     const int tile = (int)(blk / lay.kblocks), kb = (int)(blk % lay.kblocks);
-    const int t = (int)threadIdx.x, lane = t >> 2, j = t & 3;
-    const int v = tile * 16 + (lane & 15), k0 = kb * 128 + 32 * j + 8 * (lane >> 4);
-    uint32_t w = 0;
-    if (v < V && k0 < H) {  // H is a multiple of 32: the eight k are all there
-      const uint8_t* src = q + ((size_t)v * H + k0) / 2;
+    const int t = (int)threadIdx.x, lane = t >> 2, j = t & 3, k0 = kb * 128 + 32 * j + 8 * (lane >> 4);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const uint32_t b = src[p];
-        w |= (b & 15u) << (4 * p) | (b >> 4) << (16 + 4 * p);
+    for (int h = 0; h < 2; ++h) {
+      const int v = tile * 32 + 16 * h + (lane & 15);
+      uint32_t w = 0;
+      if (v < V && k0 < H) {  // H is a multiple of 32: the eight k are all there
+        const uint8_t* src = q + ((size_t)v * H + k0) / 2;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const uint32_t b = src[p];
+          w |= (b & 15u) << (4 * p) | (b >> 4) << (16 + 4 * p);
+        }
       }
+      ((uint32_t*)packed)[blk * 512 + h * 256 + t] = w;
     }
-    ((uint32_t*)packed)[blk * 256 + t] = w;
-    if (t < 16 * lay.ng) {
-      const int r = t / lay.ng, g = kb * lay.ng + t % lay.ng, vs = tile * 16 + r;
+    if (t < 32 * lay.ng) {
+      const int r = t / lay.ng, g = kb * lay.ng + t % lay.ng, vs = tile * 32 + 16 * (r & 1) + (r >> 1);
       const bool in = vs < V && g < G;
-      ((uint16_t*)(packed + lay.scales))[blk * 16 * lay.ng + t] = in ? scales[(size_t)vs * G + g] : (uint16_t)0;
-      if (zeros) (packed + lay.zeros)[blk * 16 * lay.ng + t] = in ? zeros[(size_t)vs * G + g] : (uint8_t)0;
+      ((uint16_t*)(packed + lay.scales))[blk * 32 * lay.ng + t] = in ? scales[(size_t)vs * G + g] : (uint16_t)0;
+      if (zeros) (packed + lay.zeros)[blk * 32 * lay.ng + t] = in ? zeros[(size_t)vs * G + g] : (uint8_t)0;
     }
   }
 }
@@ -135,7 +138,7 @@ static int w4_entry(int mode, const void* hidden, int hidden_dtype, const void* 
   a.out_dtype = out_dtype;
   a.out_stride = out_stride;
   a.counter = mode == MODE_GREEDY ? (unsigned int*)((char*)workspace + align_up((size_t)batch * 8, 256)) : nullptr;
-  const int most = hidden_dtype == DT_F32 ? kW4RowsF32 : kW4Rows;
+  const int most = kW4Rows;
   for (int b0 = 0; b0 < batch; b0 += most) {
     a.B = batch - b0 < most ? batch - b0 : most;
     a.hidden = (const char*)hidden + (size_t)b0 * H * dtype_size(hidden_dtype);
@@ -146,9 +149,13 @@ static int w4_entry(int mode, const void* hidden, int hidden_dtype, const void* 
     } else {
       a.out_logits = (char*)out_logits + (size_t)b0 * (size_t)out_stride * dtype_size(out_dtype);
     }
-    const int e = hidden_dtype == DT_F32    ? w4_pass_f32(mode, a, group, (hipStream_t)stream)
-                  : hidden_dtype == DT_BF16 ? w4_pass_bf16(mode, a, group, (hipStream_t)stream)
-                                            : w4_pass_f16(mode, a, group, (hipStream_t)stream);
+    const auto pass = mode == MODE_GREEDY ? (hidden_dtype == DT_F32    ? w4_greedy_f32
+                                             : hidden_dtype == DT_BF16 ? w4_greedy_bf16
+                                                                       : w4_greedy_f16)
+                                          : (hidden_dtype == DT_F32    ? w4_logits_f32
+                                             : hidden_dtype == DT_BF16 ? w4_logits_bf16
+                                                                       : w4_logits_f16);
+    const int e = pass(a, group, (hipStream_t)stream);
     if (e != NVJSEL_OK) return e;
   }
   return NVJSEL_OK;
