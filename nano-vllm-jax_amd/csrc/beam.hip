@@ -4,12 +4,14 @@
 //   candidate (w, v) of request b:  S[b,w] + (l[b,w,v] - m) - log sum_v' exp(l[b,w,v'] - m),  m = max_v' l[b,w,v']
 //
 // the K best over all w and v, by value, then by w V + v.  Within a row the order
-// is the logits' own, so one pass over them keeps each part's K largest logits
-// beside its maximum and its sum of exponentials (beam_scan_kernel), and a second
-// kernel, one block per request, joins the parts, turns the survivors into
-// scores in fp64 and ranks them (beam_select_kernel).  fp64 there because two
-// beams' candidates may lie closer than an fp32 score resolves; the sums of
-// exponentials are fp32 within a lane and fp64 across lanes and parts.
+// is the logits' own, so one pass over them takes each part's maximum, sum of
+// exponentials and the few logits that can be among the K best (beam_scan_kernel);
+// a second kernel, one block per request, joins the parts, turns those logits into
+// scores in fp64 and ranks them (beam_select_kernel).  fp64 there because two beams'
+// candidates may lie closer than an fp32 score resolves; the sums of exponentials
+// are fp32 within a lane and fp64 across lanes and parts.
+#include <float.h>
+
 #include "nvjsel_device.h"
 #include "nvjsel_host.h"
 
@@ -20,14 +22,21 @@ typedef bm_u32x4 bm_u32x4_any __attribute__((aligned(1)));  // 16 bytes from any
 typedef uint32_t bm_u32_any __attribute__((aligned(1)));
 
 static constexpr int kBeamMax = 64;        // beams and candidates per request: one lane each
-static constexpr int kBeamVecs = 8;        // 16-byte pieces per lane and chunk
+static constexpr int kBeamVecs = 4;        // 16-byte pieces per lane and chunk
+static constexpr int kBeamWaves = 16;      // per CU that a call is split into
+static constexpr int kBeamSlots = 8;       // lanes' maxima kept of a share, each over as many chunks as it takes
+static constexpr int kBeamHeld = 64;       // pieces of a lane and chunk that a wave can set aside
 static constexpr int kBeamScanThreads = 256;
-static constexpr int kBeamSelectWaves = 16;
+static constexpr int kBeamSelectThreads = 512, kBeamSelectWaves = kBeamSelectThreads / 64;
+static constexpr int kBeamRanked = 1024;   // candidates that the second kernel ranks by counting
+static constexpr int kBeamLists = 2048;    // parts of a request at most
+static constexpr int kBeamOneMax = 24;     // candidates that one maximum per lane bounds well enough, two above
+static constexpr int kBeamClasses = 128;   // two per lane of parts, for the second kernel's bound
 
 struct BeamPart {  // of one wave's share of a row
   double sum;      // sum of exp(l - max)
   float max;
-  float pad;
+  int count;       // candidates
 };
 
 struct BeamArgs {
@@ -39,7 +48,9 @@ struct BeamArgs {
   int end_token;
   int shares, share;  // parts of a row, and their length in elements (whole chunks)
   BeamPart* parts;    // [batch beams shares]
-  uint2* cand;        // [batch beams shares][k]: logit bits, token
+  uint2* cand;        // [batch beams shares][cap]: logit bits, token
+  int cap;            // candidates of a share at most
+  int group;          // chunks per kept maximum
   float* out_scores;
   int32_t* out_parents;
   int32_t* out_tokens;
@@ -70,150 +81,329 @@ struct BeamElems {
 __device__ __forceinline__ float readlane_f(float v, int l) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l));
 }
+// Maximum and sum over a wave without LDS: rotations in rows of 16, then the rows' and
+// halves' swaps.
+template <int N>
+__device__ __forceinline__ uint32_t row_ror(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, false);
+}
 __device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  return v;
+  v = fmaxf(v, __uint_as_float(row_ror<8>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(row_ror<4>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(row_ror<2>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(row_ror<1>(__float_as_uint(v))));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xor32_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
-
-// Sorts a wave's 64 values, the largest in lane 0 (bitonic).
-__device__ __forceinline__ float wave_sort_desc(float v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int d = size >> 1; d >= 1; d >>= 1) {
-      const float o = __shfl_xor(v, d, 64);
-      const bool up = (lane & size) == 0, low = (lane & d) == 0;  // up: the larger value to the lower lane
-      v = (up == low) ? fmaxf(v, o) : fminf(v, o);
-    }
-  return v;
+__device__ __forceinline__ double two_words(uint32_t lo, uint32_t hi) {
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
+template <int N>
+__device__ __forceinline__ double row_ror_add(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  return v + two_words(row_ror<N>((uint32_t)u), row_ror<N>((uint32_t)(u >> 32)));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v = row_ror_add<1>(row_ror_add<2>(row_ror_add<4>(row_ror_add<8>(v))));
+  uint64_t u = (uint64_t)__double_as_longlong(v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  v = two_words(lo[0], hi[0]) + two_words(lo[1], hi[1]);
+  u = (uint64_t)__double_as_longlong(v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  return two_words(lo[0], hi[0]) + two_words(lo[1], hi[1]);
+}
+// The largest t with its last `skip` bits clear that at least k of the wave's 2 x 64
+// numbers reach (0 if there are fewer than k): bit by bit, by counting lanes.
+__device__ __forceinline__ uint32_t wave_kth(uint32_t x, uint32_t y, int k, int skip) {
+  uint32_t t = 0;
+  for (int i = 31; i >= skip; --i) {
+    const uint32_t u = t | 1u << i;
+    if (__builtin_popcountll(__ballot(x >= u)) + __builtin_popcountll(__ballot(y >= u)) >= k) t = u;
+  }
+  return t;
+}
+// Exponentials are the hardware's exp2 (about 1 ulp) of fma(x, log2 e, -ref): one
+// rounding of the difference, and ref, a lane's maximum times log2 e, is a number that
+// the sum is relative to as it was rounded.  That holds for maxima up to this size;
+// the reference stays within it, and a share whose own maximum does not is summed
+// again (beam_sum_far).
+static constexpr float kLog2e = 1.44269504088896341f, kBeamFar = 16384.0f;
+__device__ __forceinline__ float beam_ref(float m) { return fminf(fmaxf(m, -kBeamFar), kBeamFar) * kLog2e; }
 
-// One share of a row per wave, in chunks of 64 lanes x kBeamVecs pieces that stay
-// in registers: their maximum, their exponentials, and every logit above the
-// K-th largest so far.  The K best so far lie in lanes 0 .. K - 1 in order; a
-// token enters by comparing all lanes at once.  The first chunk starts from the
-// K-th largest of the 64 lanes' maxima (at least K logits reach it), so that few
-// tokens enter.  Tokens are visited in order of index and enter only above the
-// K-th value, so among equal logits the lowest indices stay, and a row of equal
-// logits costs no more than another.
+// The piece at element o of a share that ends at e1; -inf past the end.
 template <int DT>
-__global__ void __launch_bounds__(kBeamScanThreads) beam_scan_kernel(BeamArgs a) {
+__device__ __forceinline__ bm_u32x4 beam_piece(const char* base, int o, int e1) {
   using E = BeamElems<DT>;
-  constexpr int N = E::N, CHUNK = 64 * kBeamVecs * N;
-  const int lane = (int)threadIdx.x & 63;
-  const int wid = (int)blockIdx.x * (kBeamScanThreads / 64) + ((int)threadIdx.x >> 6);
+  if (o + E::N <= e1) return *(const bm_u32x4_any*)(base + (size_t)o * (DT == DT_F32 ? 4 : 2));
+  bm_u32x4 t;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t x = E::none();
+    if constexpr (DT == DT_F32) {
+      if (o + q < e1) x = ((const uint32_t*)base)[o + q];
+    } else {
+      if (o + 2 * q < e1) x = (x & 0xFFFF0000u) | ((const uint16_t*)base)[o + 2 * q];
+      if (o + 2 * q + 1 < e1) x = (x & 0xFFFFu) | (uint32_t)((const uint16_t*)base)[o + 2 * q + 1] << 16;
+    }
+    t[q] = x;
+  }
+  return t;
+}
+
+// The sum of exp(l - m) of a share whose maximum m is known, a lane's part.
+template <int DT>
+__device__ __forceinline__ double beam_sum_far(const char* base, int e0, int e1, float m, int lane) {
+  using E = BeamElems<DT>;
+  double sum = 0.0;
+  for (int o = e0 + lane * E::N; o < e1; o += 64 * E::N) {
+    const bm_u32x4 w = beam_piece<DT>(base, o, e1);
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E::N; ++e) s += __builtin_amdgcn_exp2f((E::get(w, e) - m) * kLog2e);
+    sum += (double)s;
+  }
+  return sum;
+}
+
+// The K best logits of a share exactly, one lane each in order, where too many
+// logits reach the bound that the scan takes from its lanes' maxima: a row of equal
+// or masked values.  A token enters by comparing all lanes at once; tokens are
+// visited in order of index and enter only above the K-th value, so among equal
+// logits the lowest indices stay, and a row of equal logits costs K entries.
+template <int DT>
+__device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int k, int lane, float& val, uint32_t& idx) {
+  using E = BeamElems<DT>;
+  val = -INFINITY;
+  idx = 0xFFFFFFFFu;
+  float thr = -INFINITY;
+  for (int c0 = e0; c0 < e1; c0 += 64 * E::N) {
+    const bm_u32x4 w = beam_piece<DT>(base, c0 + lane * E::N, e1);
+    float gm = E::get(w, 0);
+#pragma unroll
+    for (int e = 1; e < E::N; ++e) gm = fmaxf(gm, E::get(w, e));
+    uint64_t hit = __ballot(gm > thr);
+    while (hit) {
+      const int l = __builtin_ctzll(hit);
+      bm_u32x4 t;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[q] = (uint32_t)__builtin_amdgcn_readlane((int)w[q], l);
+      const uint32_t i0 = (uint32_t)(c0 + l * E::N);
+#pragma unroll
+      for (int e = 0; e < E::N; ++e) {
+        const float x = E::get(t, e);
+        if (x > thr) {
+          const int pos = __builtin_popcountll(__ballot(val >= x));
+          if (pos < k) {
+            const float pv = __shfl_up(val, 1, 64);
+            const uint32_t pi = (uint32_t)__shfl_up((int)idx, 1, 64);
+            val = lane > pos ? pv : lane == pos ? x : val;
+            idx = lane > pos ? pi : lane == pos ? i0 + (uint32_t)e : idx;
+            thr = readlane_f(val, k - 1);  // -inf while fewer than K have entered
+          }
+        }
+      }
+      hit &= hit - 1;
+      hit &= __ballot(gm > thr);
+    }
+  }
+}
+
+// One share of a row per wave, in chunks of 64 lanes x kBeamVecs pieces, the next one
+// on its way in registers.  A lane keeps its own maximum and sum, so that the
+// stream's sums cross no lanes.  The K-th largest of the 64 lanes' maxima so far (of
+// 128, two per lane, for large K) is a bound that at least K logits reach and few
+// more: 64 ln(64 / (64 - K)) expected, 18 at K = 16, 128 ln(128 / (128 - K)), 89 at 64.
+// It is taken after 1, 2, 4, ... chunks, and a lane whose maximum of a chunk reaches it
+// sets the chunk's pieces aside in LDS; at the end the logits among them that reach
+// the last bound are the candidates.  Where more are set aside than there is room
+// for, the pieces are read again instead, by the lanes' maxima of every chunk in LDS
+// (V = 248,320, 256 rows, K = 16: 29 us so, 27 out of LDS).
+template <int DT>
+__global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs a) {
+  using E = BeamElems<DT>;
+  constexpr int N = E::N, CHUNK = 64 * kBeamVecs * N, DEPTH = 2;
+  __shared__ float lane_max[kBeamScanThreads / 64][kBeamSlots][64];
+  __shared__ bm_u32x4 aside[kBeamScanThreads / 64][kBeamHeld][kBeamVecs];  // or, read again: the (slot, lane) pairs
+  __shared__ int aside_at[kBeamScanThreads / 64][kBeamHeld];               // their first element
+  static_assert(sizeof(aside[0]) >= kBeamSlots * 64 * sizeof(uint16_t), "");
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wid = (int)blockIdx.x * (kBeamScanThreads / 64) + wave;
   const int row = wid / a.shares, part = wid % a.shares;
   if (row >= a.batch * a.beams) return;
   if (beam_state(a.scores[row], a.finished && a.finished[row]) != BEAM_LIVE) return;  // its logits are not looked at
   const size_t es = DT == DT_F32 ? 4 : 2;
   const char* base = (const char*)a.logits +
                      ((int64_t)(row / a.beams) * a.batch_stride + (int64_t)(row % a.beams) * a.beam_stride) * (int64_t)es;
-  const int e0 = part * a.share, e1 = min(a.vocab, e0 + a.share);
+  const int e0 = part * a.share, e1 = min(a.vocab, e0 + a.share), k = a.k;
+  const int full = (e1 - e0) / CHUNK;
+  float (*lm)[64] = lane_max[wave];
 
-  float val = -INFINITY;  // lane j: the j-th best so far
-  uint32_t idx = 0xFFFFFFFFu;
-  float thr = -INFINITY;  // logits above it enter
-  float m = -INFINITY, sum = 0.0f;
-  const int k = a.k;
-
-  for (int c0 = e0; c0 < e1; c0 += CHUNK) {
-    bm_u32x4 w[kBeamVecs];
-    if (c0 + CHUNK <= e1) {
+  float m = -INFINITY, ref = beam_ref(-INFINITY), sum = 0.0f, kept = -INFINITY;
+  float half[2] = {-INFINITY, -INFINITY};  // the maximum by pieces: the first and the last ones of every chunk
+  float bound = -FLT_MAX;                  // of the candidates: -inf is none
+  int taken = 0, held = 0;                 // chunks; pieces set aside
+  auto find_bound = [&]() NVJSEL_INLINE {  // in 16 bits of the order: bf16's own, and as good a bound for the others
+    const uint32_t t = k <= kBeamOneMax ? wave_kth(ord_f32(m), 0u, k, 16) : wave_kth(ord_f32(half[0]), ord_f32(half[1]), k, 16);
+    bound = t <= ord_f32(-INFINITY) ? -FLT_MAX : unord_f32(t);
+  };
+  int slot = 0, more = a.group;
+  auto take = [&](const bm_u32x4 (&w)[kBeamVecs]) NVJSEL_INLINE {  // chunk `taken` of the share
+    float x = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kBeamVecs; ++j)
-        w[j] = *(const bm_u32x4_any*)(base + ((size_t)c0 + (size_t)(j * 64 + lane) * N) * es);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+      float y = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kBeamVecs; ++j) {
-        const int o = c0 + (j * 64 + lane) * N;
-        if (o + N <= e1) w[j] = *(const bm_u32x4_any*)(base + (size_t)o * es);
-        else {
-          bm_u32x4 t;
+      for (int j = h * kBeamVecs / 2; j < (h + 1) * kBeamVecs / 2; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t x = E::none();
-            if constexpr (DT == DT_F32) {
-              if (o + q < e1) x = ((const uint32_t*)base)[o + q];
-            } else {
-              if (o + 2 * q < e1) x = (x & 0xFFFF0000u) | ((const uint16_t*)base)[o + 2 * q];
-              if (o + 2 * q + 1 < e1) x = (x & 0xFFFFu) | (uint32_t)((const uint16_t*)base)[o + 2 * q + 1] << 16;
-            }
-            t[q] = x;
-          }
-          w[j] = t;
-        }
-      }
+        for (int e = 0; e < N; ++e) y = __builtin_elementwise_maximum(y, E::get(w[j], e));
+      half[h] = __builtin_elementwise_maximum(half[h], y);
+      x = __builtin_elementwise_maximum(x, y);
     }
-    float gm[kBeamVecs], lm = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kBeamVecs; ++j) {
-      gm[j] = E::get(w[j], 0);
-#pragma unroll
-      for (int e = 1; e < N; ++e) gm[j] = fmaxf(gm[j], E::get(w[j], e));
-      lm = fmaxf(lm, gm[j]);
+    kept = __builtin_elementwise_maximum(kept, x);
+    lm[slot][lane] = kept;
+    if (--more == 0) {
+      more = a.group;
+      kept = -INFINITY;
+      ++slot;
     }
-    const float cm = wave_max_f32(lm);
-    if (cm > m) {
-      sum *= __expf(m - cm);  // 0 from -inf
-      m = cm;
-    }
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float s0 = 0.0f, s1 = 0.0f;
+    const float to = __builtin_elementwise_maximum(m, x), to_ref = beam_ref(to);
+    float s0 = sum * __builtin_amdgcn_exp2f(ref - to_ref), s1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < kBeamVecs; ++j)
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        s0 += __expf(E::get(w[j], e) - ref);
-        s1 += __expf(E::get(w[j], e + 1) - ref);
+        s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(E::get(w[j], e), kLog2e, -to_ref));
+        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(E::get(w[j], e + 1), kLog2e, -to_ref));
       }
-    sum += s0 + s1;
-
-    if (c0 == e0) {
-      const float f = readlane_f(wave_sort_desc(lm, lane), k - 1);
-      // the largest float below f: a logit equal to f (or the other zero) is above it
-      if (f > -INFINITY) thr = f == 0.0f ? -__uint_as_float(1u) : unord_f32(radix_key(f) - 1u);
+    m = to;
+    ref = to_ref;
+    sum = s0 + s1;
+    if ((taken & (taken + 1)) == 0) find_bound();
+    const uint64_t hit = __ballot(x >= bound);
+    if (hit) {
+      const int at = held + __builtin_popcountll(hit & ((1ull << lane) - 1));
+      if (x >= bound && at < kBeamHeld) {
+        aside_at[wave][at] = e0 + taken * CHUNK + lane * N;
+#pragma unroll
+        for (int j = 0; j < kBeamVecs; ++j) aside[wave][at][j] = w[j];
+      }
+      held += __builtin_popcountll(hit);
     }
+    ++taken;
+  };
+  if (full > 0) {
+    bm_u32x4 w[DEPTH][kBeamVecs];
+    int next = 0;
+    auto load = [&](auto D) NVJSEL_INLINE {  // always a load: the last full chunk again at the end
+      const char* p = base + ((size_t)e0 + (size_t)(next < full ? next : full - 1) * CHUNK + (size_t)lane * N) * es;
 #pragma unroll
-    for (int j = 0; j < kBeamVecs; ++j) {
-      uint64_t hit = __ballot(gm[j] > thr);
-      while (hit) {
-        const int l = __builtin_ctzll(hit);
-        bm_u32x4 t;
+      for (int j = 0; j < kBeamVecs; ++j) w[decltype(D)::value][j] = *(const bm_u32x4_any*)(p + j * 1024);
+      ++next;
+    };
+    static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE { load(D); });
+    int c = 0;
+    for (; c + DEPTH <= full; c += DEPTH)
+      static_for<DEPTH>([&](auto D) NVJSEL_INLINE {
+        load(std::integral_constant<int, (decltype(D)::value + DEPTH - 1) % DEPTH>{});
+        __builtin_amdgcn_sched_barrier(0);  // the loads first: else a round's are issued behind all its sums
+        take(w[decltype(D)::value]);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE {
+      if (c + decltype(D)::value < full) take(w[decltype(D)::value]);
+    });
+  }
+  if (e0 + full * CHUNK < e1) {  // the row's last elements
+    bm_u32x4 w[kBeamVecs];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) t[q] = (uint32_t)__builtin_amdgcn_readlane((int)w[j][q], l);
-        const uint32_t i0 = (uint32_t)(c0 + (j * 64 + l) * N);
+    for (int j = 0; j < kBeamVecs; ++j) w[j] = beam_piece<DT>(base, e0 + full * CHUNK + (j * 64 + lane) * N, e1);
+    take(w);
+  }
+
+  const float wm = wave_max_f32(m);
+  double total;
+  if (wm <= kBeamFar && (wm >= 100.0f - kBeamFar || wm == -INFINITY)) {
+    const float wref = beam_ref(wm);
+    total = wave_sum_f64((double)(sum * __builtin_amdgcn_exp2f(ref - wref)));  // a NaN's sum is NaN
+    // relative to exp(wm) now: 2^d, |d| < 2^-9 (the roundings of wref), by its series
+    const double d = wm == -INFINITY ? 0.0 : ((double)wref - (double)wm * (double)kLog2e) * 0.6931471805599453;
+    total *= 1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6.0)));
+  } else {
+    total = wave_sum_f64(beam_sum_far<DT>(base, e0, e1, wm, lane));
+  }
+
+  find_bound();
+  uint2* cand = a.cand + (size_t)wid * a.cap;
+  int count = 0;
+  auto collect = [&](const bm_u32x4& w, int o) NVJSEL_INLINE {  // the candidates of a piece per lane
+    uint32_t hits = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float x = E::get(t, e);
-          if (x > thr) {
-            const int pos = __builtin_popcountll(__ballot(val >= x));
-            if (pos < k) {
-              const float pv = __shfl_up(val, 1, 64);
-              const uint32_t pi = (uint32_t)__shfl_up((int)idx, 1, 64);
-              val = lane > pos ? pv : lane == pos ? x : val;
-              idx = lane > pos ? pi : lane == pos ? i0 + (uint32_t)e : idx;
-              const float last = readlane_f(val, k - 1);
-              if (last > -INFINITY) thr = last;
-            }
-          }
-        }
-        hit &= hit - 1;
-        hit &= __ballot(gm[j] > thr);
+    for (int e = 0; e < N; ++e) hits |= (uint32_t)(E::get(w, e) >= bound) << e;
+    uint64_t some = __ballot(hits != 0);
+    while (some) {  // a lane's first hit left, then its next
+      const int e = __builtin_ctz(hits | 1u << 31), at = count + __builtin_popcountll(some & ((1ull << lane) - 1));
+      if (hits && at < a.cap) {
+        const uint32_t v = DT == DT_F32 ? (e & 2 ? (e & 1 ? w[3] : w[2]) : (e & 1 ? w[1] : w[0]))
+                                        : (e & 4 ? (e & 2 ? w[3] : w[2]) : (e & 2 ? w[1] : w[0]));
+        const float x = DT == DT_F32    ? __uint_as_float(v)
+                        : DT == DT_BF16 ? bf16_to_f32((uint16_t)(e & 1 ? v >> 16 : v))
+                                        : f16_to_f32((uint16_t)(e & 1 ? v >> 16 : v));
+        cand[at] = make_uint2(__float_as_uint(x), (uint32_t)(o + e));
+      }
+      count += __builtin_popcountll(some);
+      hits &= hits - 1;
+      some = __ballot(hits != 0);
+    }
+  };
+  __builtin_amdgcn_wave_barrier();  // LDS operations of a wave are performed in order
+  if (held <= kBeamHeld) {
+    for (int i0 = 0; i0 < held * kBeamVecs; i0 += 64) {
+      const int i = i0 + lane;
+      bm_u32x4 w{E::none(), E::none(), E::none(), E::none()};
+      int o = 0;
+      if (i < held * kBeamVecs) {
+        w = aside[wave][i / kBeamVecs][i % kBeamVecs];
+        o = aside_at[wave][i / kBeamVecs] + (i % kBeamVecs) * 64 * N;
+      }
+      collect(w, o);
+    }
+  } else {
+    uint16_t* pairs = (uint16_t*)&aside[wave][0][0];
+    const int slots = slot + (more < a.group);
+    int np = 0;
+    for (int c = 0; c < slots; ++c) {
+      const bool hit = lm[c][lane] >= bound;
+      const uint64_t b = __ballot(hit);
+      if (hit) pairs[np + __builtin_popcountll(b & ((1ull << lane) - 1))] = (uint16_t)(c * 64 + lane);
+      np += __builtin_popcountll(b);
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int i0 = 0; i0 < np * kBeamVecs; i0 += 64) {  // a piece per lane
+      const int i = i0 + lane, pair = i < np * kBeamVecs ? pairs[i / kBeamVecs] : 0;
+      for (int g = 0; g < a.group; ++g) {
+        int o = e0 + ((pair >> 6) * a.group + g) * CHUNK + ((i % kBeamVecs) * 64 + (pair & 63)) * N;
+        o = i < np * kBeamVecs ? o : e1;
+        collect(beam_piece<DT>(base, o, e1), o);
       }
     }
   }
-  double total = (double)sum;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) total += __shfl_xor(total, x, 64);
+  if (count > a.cap) {
+    float val;
+    uint32_t idx;
+    beam_best<DT>(base, e0, e1, k, lane, val, idx);
+    const uint64_t b = __ballot(lane < k && val > -INFINITY);
+    if (b >> lane & 1) cand[lane] = make_uint2(__float_as_uint(val), idx);
+    count = __builtin_popcountll(b);
+  }
   if (lane == 0) {
     BeamPart p;
     p.sum = total;
-    p.max = m;
-    p.pad = 0.0f;
+    p.max = wm;
+    p.count = count;
     a.parts[wid] = p;
   }
-  if (lane < k) a.cand[(size_t)wid * k + lane] = make_uint2(__float_as_uint(val), idx);
 }
 
 // A candidate: its score, then beam (6 bits), logit (32, the largest first) and
@@ -259,61 +449,156 @@ __device__ __forceinline__ void beam_merge(BeamKey& x, const BeamKey& y, int lan
   for (int d = 32; d >= 1; d >>= 1) beam_step(x, d, true, lane);
 }
 
-__global__ void __launch_bounds__(64 * kBeamSelectWaves) beam_select_kernel(BeamArgs a) {
+// fp64 scores as unsigned numbers of the same order.
+__device__ __forceinline__ uint64_t beam_ord(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// One block per request.  The rows' normalisers from their parts; then a bound: the
+// parts fall into 128 classes, and the K-th best of the classes' best scores (by
+// their first 32 bits) is one that at least K candidates reach.  The candidates that reach it, seldom more than
+// twice K, are ranked by counting, each against all; where there are more than
+// kBeamRanked (many equal scores), every wave keeps the best 64 of its share of them
+// sorted and the waves' lists are merged.
+__global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArgs a) {
   __shared__ int state[kBeamMax];
   __shared__ float rmax[kBeamMax];
   __shared__ double rlog[kBeamMax], rscore[kBeamMax];
-  __shared__ double ls[kBeamSelectWaves][64];
-  __shared__ uint64_t lat[kBeamSelectWaves][64];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, req = (int)blockIdx.x;
-  const int W = a.beams, S = a.shares, k = a.k;
+  __shared__ uint32_t best_of[kBeamClasses];        // of the parts' classes: the scores' first 32 bits in order
+  __shared__ unsigned long long taken;              // parts that reach the bound, and above them their candidates
+  __shared__ int found;
+  __shared__ BeamPart part[kBeamLists];
+  __shared__ uint16_t list[kBeamLists];             // the parts that reach the bound,
+  __shared__ int start[kBeamLists];                 // and the number of their first candidate
+  __shared__ __attribute__((aligned(16))) BeamKey keys[kBeamRanked];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, req = (int)blockIdx.x;
+  const int W = a.beams, S = a.shares, k = a.k, lists = W * S;
 
+  if (tid < kBeamClasses) best_of[tid] = 0;
+  if (tid == 0) {
+    found = 0;
+    taken = 0;
+  }
+  for (int l = tid; l < lists; l += kBeamSelectThreads) part[l] = a.parts[(size_t)req * lists + l];
+  if (tid < W) {
+    const float sc = a.scores[(size_t)req * W + tid];
+    state[tid] = beam_state(sc, a.finished && a.finished[(size_t)req * W + tid]);
+    rscore[tid] = (double)sc;
+  }
+  __syncthreads();
   for (int w = wave; w < W; w += kBeamSelectWaves) {
-    const float sc = a.scores[(size_t)req * W + w];
-    int st = beam_state(sc, a.finished && a.finished[(size_t)req * W + w]);
+    int st = state[w];
+    if (st != BEAM_LIVE) continue;
+    const BeamPart* p = part + w * S;
     float m = -INFINITY;
     double t = 0.0;
-    if (st == BEAM_LIVE) {
-      const BeamPart* p = a.parts + ((size_t)req * W + w) * S;
-      for (int i = lane; i < S; i += 64) m = fmaxf(m, p[i].max);
-      m = wave_max_f32(m);
-      const double ref = m == -INFINITY ? 0.0 : (double)m;
-      for (int i = lane; i < S; i += 64) t += p[i].sum * exp((double)p[i].max - ref);
-#pragma unroll
-      for (int x = 32; x >= 1; x >>= 1) t += __shfl_xor(t, x, 64);
-      if (!(t < INFINITY)) st = BEAM_NAN;      // a NaN or an infinity among the logits
-      else if (m == -INFINITY) st = BEAM_DEAD;  // the mask leaves nothing
-    }
+    for (int i = lane; i < S; i += 64) m = fmaxf(m, p[i].max);
+    m = wave_max_f32(m);
+    const double ref = m == -INFINITY ? 0.0 : (double)m;
+    for (int i = lane; i < S; i += 64) t += p[i].sum * exp((double)p[i].max - ref);
+    t = wave_sum_f64(t);
+    if (!(t < INFINITY)) st = BEAM_NAN;      // a NaN or an infinity among the logits
+    else if (m == -INFINITY) st = BEAM_DEAD;  // the mask leaves nothing
     if (lane == 0) {
       state[w] = st;
       rmax[w] = m;
       rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
-      rscore[w] = (double)sc;
     }
   }
   __syncthreads();
+  auto score = [&](int w, float x) { return rscore[w] + (((double)x - (double)rmax[w]) - rlog[w]); };
 
-  BeamKey best{-INFINITY, kBeamNone};
-  int k2 = 1;
-  while (k2 < k) k2 *= 2;
-  const int per = 64 / k2, lists = W * S, j = lane % k2;
-  for (int l0 = wave * per; l0 < lists; l0 += kBeamSelectWaves * per) {
-    const int l = l0 + lane / k2;
-    BeamKey c{-INFINITY, kBeamNone};
-    if (l < lists && j < k) {
-      const int w = l / S;
-      if (state[w] == BEAM_LIVE) {
-        const uint2 e = a.cand[((size_t)req * lists + l) * k + j];
-        const float x = __uint_as_float(e.x);
-        if (x > -INFINITY) {
-          c.s = rscore[w] + (((double)x - (double)rmax[w]) - rlog[w]);
-          c.at = beam_at(w, x, e.y);
-        }
-      }
+  // the parts' best scores by class; an ended beam's score counts with them
+  auto put_best = [&](int l, double x) { atomicMax(&best_of[l % kBeamClasses], (uint32_t)(beam_ord(x) >> 32)); };
+  for (int l = tid; l < lists; l += kBeamSelectThreads) {
+    const int w = l / S;
+    if (state[w] == BEAM_LIVE) {
+      const float x = part[l].max;
+      if (x > -INFINITY) put_best(l, score(w, x));
+    } else if (state[w] == BEAM_ENDED && l % S == 0) {
+      put_best(l, rscore[w]);
     }
-    if (!__any(beam_before(c, beam_from(best, k - 1)))) continue;
-    beam_sort(c, lane);
-    beam_merge(best, c, lane);
+  }
+  __syncthreads();
+  const uint64_t low = (uint64_t)wave_kth(best_of[lane], best_of[64 + lane], k, 12) << 32;
+
+  auto candidate = [&](int l, int j) {  // candidate j of part l
+    const int w = l / S;
+    const uint2 e = a.cand[((size_t)req * lists + l) * a.cap + j];
+    const float x = __uint_as_float(e.x);
+    return BeamKey{score(w, x), beam_at(w, x, e.y)};
+  };
+  auto add = [&](const BeamKey& c) {
+    if (beam_ord(c.s) < low) return;
+    const int i = atomicAdd(&found, 1);
+    if (i < kBeamRanked) keys[i] = c;
+  };
+  for (int l = tid; l < lists; l += kBeamSelectThreads)
+    if (state[l / S] == BEAM_LIVE && part[l].count > 0 && beam_ord(score(l / S, part[l].max)) >= low) {
+      const unsigned long long at = atomicAdd(&taken, (unsigned long long)part[l].count << 32 | 1ull);
+      list[(uint32_t)at] = (uint16_t)l;
+      start[(uint32_t)at] = (int)(at >> 32);
+    }
+  __syncthreads();
+  const int nl = (int)(uint32_t)taken, nc = (int)(taken >> 32);
+  for (int i = tid; i < nc; i += kBeamSelectThreads) {
+    int lo = 0, hi = nl;  // the last list that starts at or before i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    add(candidate(list[lo], i - start[lo]));
+  }
+  if (tid < W && state[tid] == BEAM_ENDED) add(BeamKey{rscore[tid], beam_at(tid, 0.0f, (uint32_t)a.end_token)});
+  __syncthreads();
+
+  // NaN candidates come first, by place: every token of a NaN beam, the end token of an ended one
+  int nan = 0;
+  uint64_t nan_at = kBeamNone;
+  for (int w = 0; w < W && nan < k; ++w) {
+    const int st = state[w];
+    const int n = st == BEAM_NAN ? min(a.vocab, k - nan) : st == BEAM_ENDED_NAN ? 1 : 0;
+    if (tid >= nan && tid < nan + n) nan_at = beam_at(w, 0.0f, (uint32_t)(st == BEAM_NAN ? tid - nan : a.end_token));
+    nan += n;
+  }
+  auto put = [&](int j, const BeamKey& c) {
+    const size_t o = (size_t)req * k + j;
+    const bool none = c.at == kBeamNone;
+    a.out_scores[o] = (float)c.s;
+    a.out_parents[o] = none ? -1 : (int32_t)(c.at >> 58);
+    a.out_tokens[o] = none ? -1 : (int32_t)(c.at & ((1ull << kBeamVocabBits) - 1));
+  };
+  if (tid < nan) put(tid, BeamKey{NAN, nan_at});
+
+  const int n = found;
+  if (n <= kBeamRanked) {
+    int each = 1;  // threads of a candidate
+    while (each < 16 && 2 * each * n <= kBeamSelectThreads) each *= 2;
+    for (int i0 = 0; i0 < n; i0 += kBeamSelectThreads / each) {
+      const int i = i0 + tid / each;
+      const BeamKey c = keys[i < n ? i : 0];
+      int rank = 0;
+      for (int j = tid & (each - 1); j < n; j += each) rank += beam_before(keys[j], c);
+      for (int x = 1; x < each; x <<= 1) rank += __shfl_xor(rank, x, 64);
+      if (i < n && (tid & (each - 1)) == 0 && nan + rank < k) put(nan + rank, c);
+    }
+    if (tid >= nan + n && tid < k) put(tid, BeamKey{-INFINITY, kBeamNone});
+    return;
+  }
+  __syncthreads();
+  BeamKey best{-INFINITY, kBeamNone};
+  for (int l = wave; l < lists; l += kBeamSelectWaves) {
+    if (state[l / S] != BEAM_LIVE) continue;
+    const int n = part[l].count;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+      BeamKey c{-INFINITY, kBeamNone};
+      if (j0 + lane < n) c = candidate(l, j0 + lane);
+      if (!__any(beam_before(c, beam_from(best, k - 1)))) continue;
+      beam_sort(c, lane);
+      beam_merge(best, c, lane);
+    }
   }
   if (wave == 0) {  // ended beams: one candidate each
     BeamKey c{-INFINITY, kBeamNone};
@@ -321,63 +606,42 @@ __global__ void __launch_bounds__(64 * kBeamSelectWaves) beam_select_kernel(Beam
       c.s = rscore[lane];
       c.at = beam_at(lane, 0.0f, (uint32_t)a.end_token);
     }
-    if (__any(c.at != kBeamNone)) {
-      beam_sort(c, lane);
-      beam_merge(best, c, lane);
-    }
+    beam_sort(c, lane);
+    beam_merge(best, c, lane);
   }
-  ls[wave][lane] = best.s;
-  lat[wave][lane] = best.at;
+  keys[wave * 64 + lane] = best;
 #pragma unroll
   for (int h = kBeamSelectWaves / 2; h >= 1; h >>= 1) {
     __syncthreads();
     if (wave < h) {
-      const BeamKey o{ls[wave + h][lane], lat[wave + h][lane]};
+      const BeamKey o = keys[(wave + h) * 64 + lane];
       beam_merge(best, o, lane);
-      ls[wave][lane] = best.s;
-      lat[wave][lane] = best.at;
+      keys[wave * 64 + lane] = best;
     }
   }
-  if (wave != 0) return;
-  // NaN candidates come first, by place: every token of a NaN beam, the end token of an ended one
-  int nan = 0;
-  uint64_t at = kBeamNone;
-  for (int w = 0; w < W && nan < k; ++w) {
-    const int st = state[w];
-    const int n = st == BEAM_NAN ? min(a.vocab, k - nan) : st == BEAM_ENDED_NAN ? 1 : 0;
-    if (lane >= nan && lane < nan + n)
-      at = beam_at(w, 0.0f, (uint32_t)(st == BEAM_NAN ? lane - nan : a.end_token));
-    nan += n;
-  }
-  const int from = lane >= nan ? lane - nan : 0;
-  BeamKey out = beam_from(best, from);
-  if (lane < nan) out = BeamKey{NAN, at};
-  if (lane < k) {
-    const size_t o = (size_t)req * k + lane;
-    const bool none = out.at == kBeamNone;
-    a.out_scores[o] = (float)out.s;
-    a.out_parents[o] = none ? -1 : (int32_t)(out.at >> 58);
-    a.out_tokens[o] = none ? -1 : (int32_t)(out.at & ((1ull << kBeamVocabBits) - 1));
-  }
+  if (wave == 0 && nan + lane < k) put(nan + lane, best);
 }
 
 // Parts of a row: enough waves to fill the device, whole chunks each, and few
 // enough lists for the second kernel.
-static void beam_split(int rows, int beams, int vocab, int k, int dtype, int* shares, int* share) {
+static void beam_split(int rows, int beams, int vocab, int k, int dtype, int* shares, int* share, int* cap,
+                       int* group) {
   const int chunk = 64 * kBeamVecs * (dtype == DT_F32 ? 4 : 8);
   const int chunks = (vocab - 1) / chunk + 1;
-  int64_t s = (int64_t)device_cu_count() * 16 / rows;
-  const int64_t most = 16384 / ((int64_t)beams * k);
+  int64_t s = (int64_t)device_cu_count() * kBeamWaves / rows;
+  const int64_t most = kBeamLists / beams;
   if (s > most) s = most;
   if (s < 1) s = 1;
   if (s > chunks) s = chunks;
   const int per = (int)((chunks + s - 1) / s);
   *share = per * chunk;
+  *group = (per + kBeamSlots - 1) / kBeamSlots;
   *shares = (chunks + per - 1) / per;
+  *cap = k <= 32 ? 128 : 256;  // 30 expected at K = 24, 37 at 32, 89 at 64
 }
 
-static size_t beam_bytes(int rows, int shares, int k) {
-  return (size_t)rows * shares * sizeof(BeamPart) + (size_t)rows * shares * k * sizeof(uint2);
+static size_t beam_bytes(int rows, int shares, int cap) {
+  return (size_t)rows * shares * sizeof(BeamPart) + (size_t)rows * shares * cap * sizeof(uint2);
 }
 
 // ---------------------------------------------------------------- state reordering
@@ -500,9 +764,9 @@ static int beam_check(const char* who, int dtype, int batch, int beams, int voca
 
 extern "C" size_t nvjsel_beam_select_workspace_size(int dtype, int batch, int beams, int vocab, int k) {
   if (beam_check("beam_select", dtype, batch, beams, vocab, k) != NVJSEL_OK) return 0;
-  int shares, share;
-  beam_split(batch * beams, beams, vocab, k, dtype, &shares, &share);
-  return beam_bytes(batch * beams, shares, k);
+  int shares, share, cap, group;
+  beam_split(batch * beams, beams, vocab, k, dtype, &shares, &share, &cap, &group);
+  return beam_bytes(batch * beams, shares, cap);
 }
 
 extern "C" int nvjsel_beam_select(const void* logits, int dtype, int batch, int beams, int vocab, int64_t batch_stride,
@@ -529,8 +793,8 @@ extern "C" int nvjsel_beam_select(const void* logits, int dtype, int batch, int 
   a.scores = scores;
   a.finished = finished;
   a.end_token = end_token;
-  beam_split(batch * beams, beams, vocab, k, dtype, &a.shares, &a.share);
-  const size_t need = beam_bytes(batch * beams, a.shares, k);
+  beam_split(batch * beams, beams, vocab, k, dtype, &a.shares, &a.share, &a.cap, &a.group);
+  const size_t need = beam_bytes(batch * beams, a.shares, a.cap);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
     set_error("beam_select: workspace %zu bytes (16-byte aligned) < required %zu", workspace_bytes, need);
     return NVJSEL_EWORKSPACE;
@@ -547,7 +811,7 @@ extern "C" int nvjsel_beam_select(const void* logits, int dtype, int batch, int 
   else if (dtype == DT_BF16) hipLaunchKernelGGL(beam_scan_kernel<DT_BF16>, grid, dim3(kBeamScanThreads), 0, s, a);
   else hipLaunchKernelGGL(beam_scan_kernel<DT_F16>, grid, dim3(kBeamScanThreads), 0, s, a);
   NVJSEL_CHECK_LAUNCH("beam_scan_kernel");
-  hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)batch), dim3(64 * kBeamSelectWaves), 0, s, a);
+  hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)batch), dim3(kBeamSelectThreads), 0, s, a);
   NVJSEL_CHECK_LAUNCH("beam_select_kernel");
   return NVJSEL_OK;
 }
