@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs
     auto load = [&](auto D) NVJSEL_INLINE {  // always a load: the last full chunk again at the end
       const char* p = base + ((size_t)e0 + (size_t)(next < full ? next : full - 1) * CHUNK + (size_t)lane * N) * es;
 #pragma unroll
-      for (int j = 0; j < kBeamVecs; ++j) w[decltype(D)::value][j] = *(const bm_u32x4_any*)(p + j * 1024);
+      for (int j = 0; j < kBeamVecs; ++j) w[decltype(D)::value][j] = __builtin_nontemporal_load((const bm_u32x4_any*)(p + j * 1024));
       ++next;
     };
     static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE { load(D); });

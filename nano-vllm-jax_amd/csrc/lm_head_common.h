@@ -21,6 +21,8 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));  // a 16-byte load from any element address
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef u32x2_t u32x2_any_t __attribute__((aligned(2)));  // an 8-byte access at any element address
 
 // The eight 16-bit elements of w moved down by s places (0 <= s <= 7).
 __device__ __forceinline__ u32x4_t shift_down8(u32x4_t w, int s) {
@@ -260,6 +262,31 @@ __device__ __forceinline__ void score_run(const float (&raw)[N], int v0, int V, 
     for (int e = 0; e < N; ++e)
       if (v0 + e < V) best = max_u64(best, argmax_key(val[e], (uint32_t)(v0 + e)));
   }
+}
+
+// x[j]: this lane's value of row j, its column the lane's place in its quad.
+// Lane j of the quad gets row j's four columns as 16-bit values (bf16 or f16,
+// round to nearest even).
+__device__ __forceinline__ uint2 quad_transpose16(const float (&x)[4], int dtype, int lane) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  uint32_t r02, r13;  // rows 0 | 2 << 16 and 1 | 3 << 16 of this column
+  if (dtype == DT_BF16) {
+    r02 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[0], x[2]}), bf16x2_t));
+    r13 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[1], x[3]}), bf16x2_t));
+  } else {
+    r02 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[0], x[2]}), f16x2));
+    r13 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[1], x[3]}), f16x2));
+  }
+  const bool odd = lane & 1, high = lane & 2;
+  // with lane ^ 1: an even lane keeps rows 0 and 2, an odd one rows 1 and 3
+  const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(odd ? r02 : r13), 0xB1, 0xF, 0xF, false);
+  const uint32_t own = odd ? r13 : r02, lo = odd ? got : own, hi = odd ? own : got;
+  const uint32_t p = __builtin_amdgcn_perm(hi, lo, 0x05040100u);  // row (odd): this column pair
+  const uint32_t q = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // row 2 + (odd)
+  // with lane ^ 2: the low pair keeps rows 0 and 1, the high pair rows 2 and 3
+  const uint32_t g2 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(high ? p : q), 0x4E, 0xF, 0xF, false);
+  return high ? uint2{g2, q} : uint2{p, g2};
 }
 
 // Packs eight values into NS bf16 B-fragment words per term: NS = 1 rounds

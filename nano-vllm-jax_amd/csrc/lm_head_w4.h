@@ -109,20 +109,23 @@ __device__ __forceinline__ u32x4_t w4_unpack(uint32_t w, const W4Consts& c) {
 // k blocks kb0 .. of the hidden into LDS, as the matrix instructions' operands:
 // 16-byte slots [((4 kb + j) MB + mb) TERMS + t][k quarter][row of RT].  Three terms: x =
 // the bf16 values that its leading, next and last eight bits make (exact); a value
-// that is not finite keeps its first term only.  Then, by the matrix cores, the
+// that is not finite keeps its first term only.  No terms (0): f32 too, the three of
+// up to four batch rows as rows 4 t + b of one matrix tile, a third of the products; the
+// last four rows stay as LDS was and are left out of the results.  Then, by the matrix cores, the
 // groups' sums of activations times -1 (zero points) or -(16 + 8): xsum [group][16 MB].
 // first(): the loads that may be on their way while the weights' first ones are
 // requested; rest(): everything else.
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS>
 struct W4Stage {
   static constexpr int U = TERMS == 1 ? 8 : 4, EACH = kW4Threads / 16, LD = TERMS == 1 ? 1 : 2;
+  static constexpr int TM = TERMS ? TERMS : 1, ROWS = TERMS ? RT * MB : 4;  // terms of a slot, rows to load
   u32x4_t v[U][LD];
 
   __device__ __forceinline__ void load(const W4Args& a, int kb0, int items, int it0) {
     const int u = (int)threadIdx.x & 15;  // eight k of a k block
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int it = it0 + i * EACH, row = it % (RT * MB), k = (kb0 + it / (RT * MB)) * 128 + 8 * u;
+      const int it = it0 + i * EACH, row = it % (ROWS), k = (kb0 + it / (ROWS)) * 128 + 8 * u;
       const bool in = it < items && row < a.B && k < a.H;
       const size_t at = in ? (size_t)row * a.H + k : 0;  // always a load, of the first values where none is wanted
 #pragma unroll
@@ -136,10 +139,10 @@ struct W4Stage {
     const int u = (int)threadIdx.x & 15;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int it = it0 + i * EACH, row = it % (RT * MB), kb = it / (RT * MB), k = (kb0 + kb) * 128 + 8 * u;
+      const int it = it0 + i * EACH, row = it % (ROWS), kb = it / (ROWS), k = (kb0 + kb) * 128 + 8 * u;
       if (it >= items) break;
       const bool in = row < a.B && k < a.H;
-      u32x4_t* dst = frag + (((kb * 4 + (u >> 2)) * MB + row / RT) * TERMS * 4 + (u & 3)) * RT + row % RT;
+      u32x4_t* dst = frag + (((kb * 4 + (u >> 2)) * MB + row / RT) * TM * 4 + (u & 3)) * RT + row % RT;
       if constexpr (TERMS == 1) {
         *dst = in ? v[i][0] : u32x4_t{0u, 0u, 0u, 0u};
       } else {
@@ -157,16 +160,16 @@ struct W4Stage {
         }
 #pragma unroll
         for (int t = 0; t < 3; ++t)
-          dst[t * 4 * RT] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16,
+          dst[TERMS ? t * 4 * RT : 4 * t] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16,
                                     h[t][6] | h[t][7] << 16};
       }
     }
   }
   __device__ __forceinline__ void first(const W4Args& a, int kb0, int nkb) {
-    load(a, kb0, RT * MB * nkb, (int)threadIdx.x >> 4);
+    load(a, kb0, ROWS * nkb, (int)threadIdx.x >> 4);
   }
   __device__ __forceinline__ void rest(const W4Args& a, int kb0, int nkb, u32x4_t* frag, float* xsum) {
-    const int items = RT * MB * nkb;
+    const int items = ROWS * nkb;
     store(a, kb0, items, (int)threadIdx.x >> 4, frag);
     for (int it0 = ((int)threadIdx.x >> 4) + U * EACH; it0 < items; it0 += U * EACH) {
       load(a, kb0, items, it0);
@@ -185,8 +188,8 @@ struct W4Stage {
 #pragma unroll
         for (int j = 0; j < 4 / NG; ++j)
 #pragma unroll
-          for (int c = TERMS - 1; c >= 0; --c)
-            d = mfma16x16x32<FMT>(mine[(((g * (4 / NG) + j) * MB + m) * TERMS + c) * 4 * RT], ones, d);
+          for (int c = TM - 1; c >= 0; --c)
+            d = mfma16x16x32<FMT>(mine[(((g * (4 / NG) + j) * MB + m) * TM + c) * 4 * RT], ones, d);
         if ((lane & 15) == 0) *(f32x4_t*)(xsum + (g * MB + m) * 16 + 4 * (lane >> 4)) = d;
       }
     }
@@ -205,21 +208,24 @@ struct W4Stage {
 // dealt to the blocks, and a block splits its rest by k blocks over its waves, which
 // join their parts through LDS at the end (V = 151,936, H = 2560, 8 rows: 46 us with
 // whole tiles only, 2.3 rounds of them, 42 split).  STAGED waves walk the k blocks
-// together and repeat the last tile instead.
+// together, two tiles at a time (NB: half as many reads of the hidden, and stagings), and
+// repeat the last one instead.
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, bool STAGED, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int DEPTH = 4, NT = 2;
+  constexpr int TM = TERMS ? TERMS : 1;
+  constexpr int NB = STAGED ? 2 : 1, DEPTH = STAGED ? 2 : 4, NT = 2 * NB;
   const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int KB = lay.kblocks, kc = a.kc, col = lane & 15;
   u32x4_t* frag = (u32x4_t*)lds;
-  float* xsum = (float*)(lds + (size_t)kc * 256 * TERMS * RT * MB);
+  float* xsum = (float*)(lds + (size_t)kc * 256 * TM * RT * MB);
   const u32x4_t* mine = frag + (lane >> 4) * RT + (lane & (RT - 1));
   const float* xmine = xsum + 4 * (lane >> 4);
 
   const int step = (int)gridDim.x * kW4Waves, first = (int)blockIdx.x * kW4Waves + wave;
-  const int full = STAGED ? (lay.tiles - (int)blockIdx.x * kW4Waves + step - 1) / step : lay.tiles / step;  // whole rounds
+  const int supers = (lay.tiles + NB - 1) / NB;
+  const int full = STAGED ? (supers - (int)blockIdx.x * kW4Waves + step - 1) / step : lay.tiles / step;  // whole rounds
   // the block's rest: tiles from rest0, its k blocks dealt to the waves
   int rest0 = 0, nrest = 0;
   if (!STAGED) {
@@ -242,36 +248,39 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   // load's extension would be waited for a round of the ring early.
   struct Item {
     u32x4_t w[NT];
-    uint32_t s[NG];  // two 16-bit scales each: [t][g]
-    uint32_t z[(NG + 1) / 2];
+    uint32_t s[NB][NG];  // two 16-bit scales each: [t][g]
+    uint32_t z[NB][(NG + 1) / 2];
   };
   Item ring[DEPTH];
 
   int lkb = full ? 0 : tail_kb, ltile = full ? first : tail_tile, lfull = full;  // the item to be requested next
   auto load = [&](auto D) NVJSEL_INLINE {
     Item& it = ring[decltype(D)::value];
-    const int tile = ltile < lay.tiles ? ltile : lay.tiles - 1;
-    const size_t blk = (size_t)tile * KB + lkb;
-    const u32x4_t* wb = (const u32x4_t*)(a.packed + blk * 2048) + lane;
-    it.w[0] = __builtin_nontemporal_load(wb);
-    it.w[1] = __builtin_nontemporal_load(wb + 64);
-    const uint32_t* sb = (const uint32_t*)(a.packed + lay.scales + blk * (64 * NG)) + col * NG;
-    if constexpr (NG == 4) {
-      const u32x4_t v = *(const u32x4_t*)sb;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) it.s[g] = v[g];
-    } else if constexpr (NG == 2) {
-      const uint64_t v = *(const uint64_t*)sb;
-      it.s[0] = (uint32_t)v;
-      it.s[1] = (uint32_t)(v >> 32);
-    } else it.s[0] = *sb;
-    if constexpr (ZEROS) {
-      const uint8_t* zb = a.packed + lay.zeros + blk * (32 * NG) + zoff;
+    for (int n = 0; n < NB; ++n) {
+      const int at = ltile * NB + n, tile = at < lay.tiles ? at : lay.tiles - 1;
+      const size_t blk = (size_t)tile * KB + lkb;
+      const u32x4_t* wb = (const u32x4_t*)(a.packed + blk * 2048) + lane;
+      it.w[2 * n] = __builtin_nontemporal_load(wb);
+      it.w[2 * n + 1] = __builtin_nontemporal_load(wb + 64);
+      const uint32_t* sb = (const uint32_t*)(a.packed + lay.scales + blk * (64 * NG)) + col * NG;
       if constexpr (NG == 4) {
-        const uint64_t v = *(const uint64_t*)zb;
-        it.z[0] = (uint32_t)v;
-        it.z[1] = (uint32_t)(v >> 32);
-      } else it.z[0] = *(const uint32_t*)zb;
+        const u32x4_t v = *(const u32x4_t*)sb;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) it.s[n][g] = v[g];
+      } else if constexpr (NG == 2) {
+        const uint64_t v = *(const uint64_t*)sb;
+        it.s[n][0] = (uint32_t)v;
+        it.s[n][1] = (uint32_t)(v >> 32);
+      } else it.s[n][0] = *sb;
+      if constexpr (ZEROS) {
+        const uint8_t* zb = a.packed + lay.zeros + blk * (32 * NG) + zoff;
+        if constexpr (NG == 4) {
+          const uint64_t v = *(const uint64_t*)zb;
+          it.z[n][0] = (uint32_t)v;
+          it.z[n][1] = (uint32_t)(v >> 32);
+        } else it.z[n][0] = *(const uint32_t*)zb;
+      }
     }
     if (++lkb == KB) {
       --lfull;
@@ -281,7 +290,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   };
 
   // greedy: the best so far of each row among this lane's columns; no index yet: ~0, beside a NaN
-  float total[NT][MB][4], bval[MB][4], foreign[NT][MB][4];
+  float total[NT][MB][4], bval[MB][4], foreign[NT][MB][4];  // foreign: not STAGED
   uint32_t bidx[MB][4];
 #pragma unroll
   for (int m = 0; m < MB; ++m)
@@ -293,8 +302,27 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
       for (int t = 0; t < NT; ++t) total[t][m][i] = foreign[t][m][i] = 0.0f;
     }
 
+  char* orow[MB];  // logits: the rows that this lane stores (f32: the first of four)
+  if constexpr (MODE == MODE_LOGITS) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const bool f32 = a.out_dtype == DT_F32;
+      orow[m] = (char*)a.out_logits +
+                (size_t)(16 * m + 4 * (lane >> 4) + (f32 ? 0 : lane & 3)) * (size_t)a.out_stride * (f32 ? 4 : 2);
+    }
+  }
+
   // A tile's totals are whole: rounded, and scored or stored.
   auto finish_tile = [&](int tile) NVJSEL_INLINE {
+    if constexpr (TERMS == 0) {  // the terms of a row meet: lane quarters 0, 1 and 2
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = xpose_add16(lane < 48 ? total[t][0][i] : 0.0f, lane < 48 ? total[t][0][i] : 0.0f);
+          total[t][0][i] = xpose_add32(x, x);
+        }
+    }
     if (a.reduce_cast == 1) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -312,8 +340,8 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int v = tile * 32 + 16 * t + col;
-      const bool in = tile < lay.tiles && v < a.V;
+      const int v = (tile * NB + (t >> 1)) * 32 + 16 * (t & 1) + col;
+      const bool in = v < a.V;
       if constexpr (MODE == MODE_GREEDY) {
         bool up = false;  // seldom: a lane's best of so many tiles
 #pragma unroll
@@ -333,20 +361,34 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
             }
         }
       } else {
-        auto store = [&](auto* out) NVJSEL_INLINE {
-          typedef typename std::remove_reference<decltype(*out)>::type T;
-          T* p = out + v;
+        // 16-bit logits are transposed in quads of lanes (four rows x four columns) and
+        // stored 8 bytes per lane, at any element address; the vocabulary's last quad
+        // may be partial
+        const int v4 = v & ~3, left = a.V - v4;
 #pragma unroll
-          for (int m = 0; m < MB; ++m)
+        for (int m = 0; m < MB; ++m) {
+          const int b = 16 * m + 4 * (lane >> 4);
+          if (a.out_dtype != DT_F32) {
+            float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int b = 16 * m + 4 * (lane >> 4) + i;
-              if (in && b < a.B) p[(size_t)b * (size_t)a.out_stride] = (T)total[t][m][i];
+            for (int i = 0; i < 4; ++i) x[i] = total[t][m][i];
+            const uint2 q = quad_transpose16(x, a.out_dtype, lane);
+            if (left > 0 && b + (lane & 3) < a.B) {
+              uint16_t* out = (uint16_t*)orow[m] + v4;
+              if (left >= 4) {
+                *(u32x2_any_t*)out = u32x2_t{q.x, q.y};
+              } else {
+                out[0] = (uint16_t)q.x;
+                if (left > 1) out[1] = (uint16_t)(q.x >> 16);
+                if (left > 2) out[2] = (uint16_t)q.y;
+              }
             }
-        };
-        if (a.out_dtype == DT_F32) store((float*)a.out_logits);
-        else if (a.out_dtype == DT_BF16) store((__bf16*)a.out_logits);
-        else store((_Float16*)a.out_logits);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (in && b + i < a.B) ((float*)orow[m])[(size_t)i * (size_t)a.out_stride + v] = total[t][m][i];
+          }
+        }
       }
     }
   };
@@ -362,7 +404,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
     }
     const Item& it = ring[decltype(D)::value];
     const int kx = STAGED ? kl : kb;
-    const u32x4_t* fk = mine + kx * (4 * MB * TERMS * 4 * RT);
+    const u32x4_t* fk = mine + kx * (4 * MB * TM * 4 * RT);
     const float* xk = xmine + kx * (NG * MB * 16);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -373,8 +415,8 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           if constexpr (ZEROS) {
-            const int zi = t * NG + g;  // byte of the block's zero points of this row
-            const float z = 16.0f + (float)((it.z[zi >> 2] >> (zshift + 8 * (zi & 3))) & 0xFFu);
+            const int zi = (t & 1) * NG + g;  // byte of the block's zero points of this row
+            const float z = 16.0f + (float)((it.z[t >> 1][zi >> 2] >> (zshift + 8 * (zi & 3))) & 0xFFu);
             acc[t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
           } else acc[t][m] = xs;
         }
@@ -387,16 +429,16 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int c = TERMS - 1; c >= 0; --c) {
-            const u32x4_t xf = fk[((j * MB + m) * TERMS + c) * 4 * RT];
+          for (int c = TM - 1; c >= 0; --c) {
+            const u32x4_t xf = fk[((j * MB + m) * TM + c) * 4 * RT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t][m] = mfma16x16x32<FMT>(xf, wf[t], acc[t][m]);
           }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int si = t * NG + g;  // 16-bit scale of the block's scales of this row
-        const uint32_t sb = it.s[si >> 1] >> (16 * (si & 1));
+        const int si = (t & 1) * NG + g;  // 16-bit scale of the block's scales of this row
+        const uint32_t sb = it.s[t >> 1][si >> 1] >> (16 * (si & 1));
         const uint32_t fh = __float_as_uint(f16_to_f32((uint16_t)sb));
         const float s = __uint_as_float((sb << 16 & bf16_mask) | (fh & ~bf16_mask));
 #pragma unroll
@@ -500,7 +542,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, int MODE>
 static int launch_w4(W4Args a, hipStream_t stream) {
   const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
-  const size_t per_kb = (size_t)RT * MB * 256 * TERMS + (size_t)NG * 16 * MB * 4;
+  const size_t per_kb = (size_t)RT * MB * 256 * (TERMS ? TERMS : 1) + (size_t)NG * 16 * MB * 4;
   const size_t parts = (size_t)kW4Waves * MB * 2048;  // of the tiles that waves split; the rows' keys need less
   int chunks = 1;
   while ((size_t)((lay.kblocks + chunks - 1) / chunks) * per_kb > kW4Lds) ++chunks;
@@ -511,7 +553,7 @@ static int launch_w4(W4Args a, hipStream_t stream) {
                           : lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, true, MODE>;
   if (lds > 48 * 1024)
     NVJSEL_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  const int cus = device_cu_count(), need = chunks == 1 ? lay.tiles : (lay.tiles + kW4Waves - 1) / kW4Waves;
+  const int cus = device_cu_count(), need = chunks == 1 ? lay.tiles : (lay.tiles + 2 * kW4Waves - 1) / (2 * kW4Waves);
   hipLaunchKernelGGL(kern, dim3(need < cus ? need : cus), dim3(kW4Threads), lds, stream, a);
   NVJSEL_CHECK_LAUNCH("lm_head_w4_kernel");
   return NVJSEL_OK;
@@ -531,7 +573,7 @@ static int launch_w4_group(const W4Args& a, int group, hipStream_t s) {
 
 template <int FMT, int TERMS, int MODE>
 static int w4_pass(const W4Args& a, int group, hipStream_t s) {
-  if (a.B <= 4) return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, s);
+  if (a.B <= 4) return launch_w4_group<FMT, TERMS == 3 ? 0 : TERMS, 1, TERMS == 3 ? 16 : 4, MODE>(a, group, s);
   if (a.B <= 16) return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, s);
   if (a.B <= 32) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, s);
   return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, s);

@@ -52,11 +52,11 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     if logits.stride(2) != 1 and vocab > 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    out_scores = torch.empty((batch, k), dtype=torch.float32, device=dev)
-    parents, tokens = torch.empty((2, batch, k), dtype=torch.int32, device=dev).unbind(0)
+    out_scores = scores.new_empty((batch, k))
+    parents, tokens = scores.new_empty((2, batch, k), dtype=torch.int32).unbind(0)
     with _on_device(dev):
         nbytes = _lib.load().nvjsel_beam_select_workspace_size(dt, batch, beams, vocab, k)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        ws = scores.new_empty((nbytes,), dtype=torch.uint8)
         _lib.call("nvjsel_beam_select", logits.data_ptr(), dt, batch, beams, vocab, logits.stride(0), logits.stride(1),
                   scores.data_ptr(), None if finished is None else finished.data_ptr(), end_token or 0, k,
                   out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes,
