@@ -299,7 +299,7 @@ int nvjsel_lm_head_w4_logits(const void* hidden, int hidden_dtype, const void* p
  * ascending, give out_scores f32 [batch, k], out_parents int32 (w) and out_tokens
  * int32 (v).  logits [batch, beams, vocab] of dtype, batch_stride and
  * beam_stride elements apart; scores f32 [batch, beams].  1 <= beams, k <= 64,
- * vocab <= 2^26.
+ * vocab <= 2^26, batch <= 65536.
  *
  * A beam whose score is -inf is not live: it has no candidates and its logits
  * are not looked at.  A beam with finished[b,w] != 0 (nullable) has one
@@ -308,8 +308,9 @@ int nvjsel_lm_head_w4_logits(const void* hidden, int hidden_dtype, const void* p
  * fewer than k are left the rest is -inf, parent -1, token -1.  A NaN or +inf
  * among a live beam's logits, or as its score, makes its candidates NaN, and
  * NaN comes before every number, in order of place.
- * Workspace: nvjsel_beam_select_workspace_size() bytes of scratch, 16-byte
- * aligned, any contents on entry.
+ * Workspace: nvjsel_beam_select_workspace_size() bytes, 16-byte aligned; the first
+ * 256 KB (the requests' tickets, at the same offset for every shape) are zero at
+ * rest, every call leaves them so, and the rest is scratch.
  */
 size_t nvjsel_beam_select_workspace_size(int dtype, int batch, int beams, int vocab, int k);
 

@@ -5,12 +5,15 @@
 //
 // the K best over all w and v, by value, then by w V + v.  Within a row the order
 // is the logits' own, so one pass over them takes each part's maximum, sum of
-// exponentials and the few logits that can be among the K best (beam_scan_kernel);
-// a second kernel, one block per request, joins the parts, turns those logits into
-// scores in fp64 and ranks them (beam_select_kernel).  fp64 there because two beams'
+// exponentials and the few logits that can be among the K best (beam_scan), and one
+// block per request joins the parts, turns those logits into scores in fp64 and
+// ranks them (beam_join).  With few parts a request's last block to finish them joins
+// them in the same launch, with more a second kernel does (kBeamFew). fp64 there because two beams'
 // candidates may lie closer than an fp32 score resolves; the sums of exponentials
 // are fp32 within a lane and fp64 across lanes and parts.
 #include <float.h>
+
+#include <mutex>
 
 #include "nvjsel_device.h"
 #include "nvjsel_host.h"
@@ -22,16 +25,20 @@ typedef bm_u32x4 bm_u32x4_any __attribute__((aligned(1)));  // 16 bytes from any
 typedef uint32_t bm_u32_any __attribute__((aligned(1)));
 
 static constexpr int kBeamMax = 64;        // beams and candidates per request: one lane each
+static constexpr int kBeamRequests = 65536;  // of a call: a workspace's tickets are at the same place for every shape
 static constexpr int kBeamVecs = 4;        // 16-byte pieces per lane and chunk
 static constexpr int kBeamWaves = 16;      // per CU that a call is split into
 static constexpr int kBeamSlots = 8;       // lanes' maxima kept of a share, each over as many chunks as it takes
 static constexpr int kBeamHeld = 64;       // pieces of a lane and chunk that a wave can set aside
-static constexpr int kBeamScanThreads = 256;
-static constexpr int kBeamSelectThreads = 512, kBeamSelectWaves = kBeamSelectThreads / 64;
-static constexpr int kBeamRanked = 1024;   // candidates that the second kernel ranks by counting
-static constexpr int kBeamLists = 2048;    // parts of a request at most
+static constexpr int kBeamThreads = 256, kBeamBlockWaves = kBeamThreads / 64;
+// One launch scans and joins calls of up to kBeamOne parts, kBeamFew a request.  What
+// passes between its blocks goes by the device's coherence point: 64 / 392 / 512 / 1008 /
+// 2048 parts take 10.0 / 10.6 / 10.9 / 12.4 / 15.7 us so and 10.5 / 10.4 / 11.0 / 10.7 / 11.1
+// in two kernels, which cost the host 3 us more.  And the parts of a request at most.
+static constexpr int kBeamOne = 512, kBeamFew = 256, kBeamLists = 2048;
+static constexpr int kBeamJoinThreads = 512;             // of the second kernel
 static constexpr int kBeamOneMax = 24;     // candidates that one maximum per lane bounds well enough, two above
-static constexpr int kBeamClasses = 128;   // two per lane of parts, for the second kernel's bound
+static constexpr int kBeamClasses = 128;   // of parts, two per lane, for the join's bound
 
 struct BeamPart {  // of one wave's share of a row
   double sum;      // sum of exp(l - max)
@@ -47,14 +54,32 @@ struct BeamArgs {
   const uint8_t* finished;  // [batch, beams] or null
   int end_token;
   int shares, share;  // parts of a row, and their length in elements (whole chunks)
-  BeamPart* parts;    // [batch beams shares]
-  uint2* cand;        // [batch beams shares][cap]: logit bits, token
+  unsigned int* tickets;  // [batch], zero at rest: blocks that have finished their parts
+  int blocks;             // of a request
+  BeamPart* parts;        // [batch beams shares]
+  uint2* cand;            // [batch beams shares][cap]: logit bits, token
   int cap;            // candidates of a share at most
   int group;          // chunks per kept maximum
   float* out_scores;
   int32_t* out_parents;
   int32_t* out_tokens;
 };
+
+// Parts and candidates, 8 bytes at a time.  ONE: they pass between blocks of one launch,
+// on any XCDs, written and read at the device's coherence point (agent scope).
+template <bool ONE>
+__device__ __forceinline__ void beam_put(void* p, uint32_t lo, uint32_t hi) {
+  const unsigned long long v = (unsigned long long)hi << 32 | lo;
+  if constexpr (ONE) __hip_atomic_store((unsigned long long*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else *(unsigned long long*)p = v;
+}
+template <bool ONE>
+__device__ __forceinline__ uint2 beam_get(const void* p) {
+  unsigned long long v;
+  if constexpr (ONE) v = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else v = *(const unsigned long long*)p;
+  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+}
 
 // What a beam contributes: nothing, every token, one token, or NaN.
 enum { BEAM_DEAD = 0, BEAM_LIVE = 1, BEAM_ENDED = 2, BEAM_NAN = 3, BEAM_ENDED_NAN = 4 };
@@ -220,25 +245,26 @@ __device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int 
 // the last bound are the candidates.  Where more are set aside than there is room
 // for, the pieces are read again instead, by the lanes' maxima of every chunk in LDS
 // (V = 248,320, 256 rows, K = 16: 29 us so, 27 out of LDS).
-template <int DT>
-__global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs a) {
+struct BeamScanLds {
+  float lane_max[kBeamBlockWaves][kBeamSlots][64];
+  bm_u32x4 aside[kBeamBlockWaves][kBeamHeld][kBeamVecs];  // or, read again: the (slot, lane) pairs
+  int aside_at[kBeamBlockWaves][kBeamHeld];               // their first element
+};
+static_assert(sizeof(bm_u32x4) * kBeamHeld * kBeamVecs >= kBeamSlots * 64 * sizeof(uint16_t), "");
+
+template <int DT, bool ONE>
+__device__ __forceinline__ void beam_scan(const BeamArgs& a, BeamScanLds& lds, int row, int part, int wave, int lane) {
   using E = BeamElems<DT>;
   constexpr int N = E::N, CHUNK = 64 * kBeamVecs * N, DEPTH = 2;
-  __shared__ float lane_max[kBeamScanThreads / 64][kBeamSlots][64];
-  __shared__ bm_u32x4 aside[kBeamScanThreads / 64][kBeamHeld][kBeamVecs];  // or, read again: the (slot, lane) pairs
-  __shared__ int aside_at[kBeamScanThreads / 64][kBeamHeld];               // their first element
-  static_assert(sizeof(aside[0]) >= kBeamSlots * 64 * sizeof(uint16_t), "");
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int wid = (int)blockIdx.x * (kBeamScanThreads / 64) + wave;
-  const int row = wid / a.shares, part = wid % a.shares;
-  if (row >= a.batch * a.beams) return;
-  if (beam_state(a.scores[row], a.finished && a.finished[row]) != BEAM_LIVE) return;  // its logits are not looked at
+  const int wid = row * a.shares + part;
   const size_t es = DT == DT_F32 ? 4 : 2;
   const char* base = (const char*)a.logits +
                      ((int64_t)(row / a.beams) * a.batch_stride + (int64_t)(row % a.beams) * a.beam_stride) * (int64_t)es;
   const int e0 = part * a.share, e1 = min(a.vocab, e0 + a.share), k = a.k;
   const int full = (e1 - e0) / CHUNK;
-  float (*lm)[64] = lane_max[wave];
+  float (*lm)[64] = lds.lane_max[wave];
+  auto& aside = lds.aside[wave];
+  auto& aside_at = lds.aside_at[wave];
 
   float m = -INFINITY, ref = beam_ref(-INFINITY), sum = 0.0f, kept = -INFINITY;
   float half[2] = {-INFINITY, -INFINITY};  // the maximum by pieces: the first and the last ones of every chunk
@@ -285,9 +311,9 @@ __global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs
     if (hit) {
       const int at = held + __builtin_popcountll(hit & ((1ull << lane) - 1));
       if (x >= bound && at < kBeamHeld) {
-        aside_at[wave][at] = e0 + taken * CHUNK + lane * N;
+        aside_at[at] = e0 + taken * CHUNK + lane * N;
 #pragma unroll
-        for (int j = 0; j < kBeamVecs; ++j) aside[wave][at][j] = w[j];
+        for (int j = 0; j < kBeamVecs; ++j) aside[at][j] = w[j];
       }
       held += __builtin_popcountll(hit);
     }
@@ -350,7 +376,7 @@ __global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs
         const float x = DT == DT_F32    ? __uint_as_float(v)
                         : DT == DT_BF16 ? bf16_to_f32((uint16_t)(e & 1 ? v >> 16 : v))
                                         : f16_to_f32((uint16_t)(e & 1 ? v >> 16 : v));
-        cand[at] = make_uint2(__float_as_uint(x), (uint32_t)(o + e));
+        beam_put<ONE>(cand + at, __float_as_uint(x), (uint32_t)(o + e));
       }
       count += __builtin_popcountll(some);
       hits &= hits - 1;
@@ -364,13 +390,13 @@ __global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs
       bm_u32x4 w{E::none(), E::none(), E::none(), E::none()};
       int o = 0;
       if (i < held * kBeamVecs) {
-        w = aside[wave][i / kBeamVecs][i % kBeamVecs];
-        o = aside_at[wave][i / kBeamVecs] + (i % kBeamVecs) * 64 * N;
+        w = aside[i / kBeamVecs][i % kBeamVecs];
+        o = aside_at[i / kBeamVecs] + (i % kBeamVecs) * 64 * N;
       }
       collect(w, o);
     }
   } else {
-    uint16_t* pairs = (uint16_t*)&aside[wave][0][0];
+    uint16_t* pairs = (uint16_t*)&aside[0][0];
     const int slots = slot + (more < a.group);
     int np = 0;
     for (int c = 0; c < slots; ++c) {
@@ -394,15 +420,13 @@ __global__ void __launch_bounds__(kBeamScanThreads, 4) beam_scan_kernel(BeamArgs
     uint32_t idx;
     beam_best<DT>(base, e0, e1, k, lane, val, idx);
     const uint64_t b = __ballot(lane < k && val > -INFINITY);
-    if (b >> lane & 1) cand[lane] = make_uint2(__float_as_uint(val), idx);
+    if (b >> lane & 1) beam_put<ONE>(cand + lane, __float_as_uint(val), idx);
     count = __builtin_popcountll(b);
   }
   if (lane == 0) {
-    BeamPart p;
-    p.sum = total;
-    p.max = wm;
-    p.count = count;
-    a.parts[wid] = p;
+    const uint64_t u = (uint64_t)__double_as_longlong(total);
+    beam_put<ONE>(&a.parts[wid].sum, (uint32_t)u, (uint32_t)(u >> 32));
+    beam_put<ONE>(&a.parts[wid].max, __float_as_uint(wm), (uint32_t)count);
   }
 }
 
@@ -455,24 +479,42 @@ __device__ __forceinline__ uint64_t beam_ord(double x) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-// One block per request.  The rows' normalisers from their parts; then a bound: the
-// parts fall into 128 classes, and the K-th best of the classes' best scores (by
-// their first 32 bits) is one that at least K candidates reach.  The candidates that reach it, seldom more than
-// twice K, are ranked by counting, each against all; where there are more than
-// kBeamRanked (many equal scores), every wave keeps the best 64 of its share of them
-// sorted and the waves' lists are merged.
-__global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArgs a) {
-  __shared__ int state[kBeamMax];
-  __shared__ float rmax[kBeamMax];
-  __shared__ double rlog[kBeamMax], rscore[kBeamMax];
-  __shared__ uint32_t best_of[kBeamClasses];        // of the parts' classes: the scores' first 32 bits in order
-  __shared__ unsigned long long taken;              // parts that reach the bound, and above them their candidates
-  __shared__ int found;
-  __shared__ BeamPart part[kBeamLists];
-  __shared__ uint16_t list[kBeamLists];             // the parts that reach the bound,
-  __shared__ int start[kBeamLists];                 // and the number of their first candidate
-  __shared__ __attribute__((aligned(16))) BeamKey keys[kBeamRanked];
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, req = (int)blockIdx.x;
+// A request's parts joined by one block.  The rows' normalisers from their parts; then
+// a bound: the parts fall into 128 classes, and the K-th best of the classes' best
+// scores (by their first 32 bits) is one that at least K candidates reach.  The
+// candidates that reach it, seldom more than twice K, are ranked by counting, each
+// against all; where there are more than there is room for (many equal scores), every
+// wave keeps the best 64 of its share of them sorted and the waves' lists are merged.
+template <int LISTS>
+struct BeamJoinLds {
+  static constexpr int RANKED = LISTS == kBeamFew ? 512 : 1024;
+  BeamKey keys[RANKED];
+  BeamPart part[LISTS];
+  double rlog[kBeamMax], rscore[kBeamMax];
+  unsigned long long taken;        // parts that reach the bound, and above them their candidates
+  int state[kBeamMax];
+  float rmax[kBeamMax];
+  uint32_t best_of[kBeamClasses];  // of the parts' classes: the scores' first 32 bits in order
+  int start[LISTS];                // of the parts that reach the bound: the number of their first candidate
+  uint16_t list[LISTS];
+  int found;
+};
+
+template <int LISTS, int THREADS, bool ONE>
+__device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>& lds, int req, int tid) {
+  constexpr int RANKED = BeamJoinLds<LISTS>::RANKED;
+  auto& state = lds.state;
+  auto& rmax = lds.rmax;
+  auto& rlog = lds.rlog;
+  auto& rscore = lds.rscore;
+  auto& best_of = lds.best_of;
+  auto& taken = lds.taken;
+  auto& found = lds.found;
+  auto& part = lds.part;
+  auto& list = lds.list;
+  auto& start = lds.start;
+  auto& keys = lds.keys;
+  const int lane = tid & 63, wave = tid >> 6;
   const int W = a.beams, S = a.shares, k = a.k, lists = W * S;
 
   if (tid < kBeamClasses) best_of[tid] = 0;
@@ -480,14 +522,20 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
     found = 0;
     taken = 0;
   }
-  for (int l = tid; l < lists; l += kBeamSelectThreads) part[l] = a.parts[(size_t)req * lists + l];
+  for (int l = tid; l < lists; l += THREADS) {
+    const BeamPart* p = a.parts + (size_t)req * lists + l;
+    const uint2 u = beam_get<ONE>(&p->sum), v = beam_get<ONE>(&p->max);
+    part[l].sum = two_words(u.x, u.y);
+    part[l].max = __uint_as_float(v.x);
+    part[l].count = (int)v.y;
+  }
   if (tid < W) {
     const float sc = a.scores[(size_t)req * W + tid];
     state[tid] = beam_state(sc, a.finished && a.finished[(size_t)req * W + tid]);
     rscore[tid] = (double)sc;
   }
   __syncthreads();
-  for (int w = wave; w < W; w += kBeamSelectWaves) {
+  for (int w = wave; w < W; w += (THREADS / 64)) {
     int st = state[w];
     if (st != BEAM_LIVE) continue;
     const BeamPart* p = part + w * S;
@@ -511,7 +559,7 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
 
   // the parts' best scores by class; an ended beam's score counts with them
   auto put_best = [&](int l, double x) { atomicMax(&best_of[l % kBeamClasses], (uint32_t)(beam_ord(x) >> 32)); };
-  for (int l = tid; l < lists; l += kBeamSelectThreads) {
+  for (int l = tid; l < lists; l += THREADS) {
     const int w = l / S;
     if (state[w] == BEAM_LIVE) {
       const float x = part[l].max;
@@ -525,16 +573,16 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
 
   auto candidate = [&](int l, int j) {  // candidate j of part l
     const int w = l / S;
-    const uint2 e = a.cand[((size_t)req * lists + l) * a.cap + j];
+    const uint2 e = beam_get<ONE>(a.cand + ((size_t)req * lists + l) * a.cap + j);
     const float x = __uint_as_float(e.x);
     return BeamKey{score(w, x), beam_at(w, x, e.y)};
   };
   auto add = [&](const BeamKey& c) {
     if (beam_ord(c.s) < low) return;
     const int i = atomicAdd(&found, 1);
-    if (i < kBeamRanked) keys[i] = c;
+    if (i < RANKED) keys[i] = c;
   };
-  for (int l = tid; l < lists; l += kBeamSelectThreads)
+  for (int l = tid; l < lists; l += THREADS)
     if (state[l / S] == BEAM_LIVE && part[l].count > 0 && beam_ord(score(l / S, part[l].max)) >= low) {
       const unsigned long long at = atomicAdd(&taken, (unsigned long long)part[l].count << 32 | 1ull);
       list[(uint32_t)at] = (uint16_t)l;
@@ -542,7 +590,7 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
     }
   __syncthreads();
   const int nl = (int)(uint32_t)taken, nc = (int)(taken >> 32);
-  for (int i = tid; i < nc; i += kBeamSelectThreads) {
+  for (int i = tid; i < nc; i += THREADS) {
     int lo = 0, hi = nl;  // the last list that starts at or before i
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -573,10 +621,10 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
   if (tid < nan) put(tid, BeamKey{NAN, nan_at});
 
   const int n = found;
-  if (n <= kBeamRanked) {
+  if (n <= RANKED) {
     int each = 1;  // threads of a candidate
-    while (each < 16 && 2 * each * n <= kBeamSelectThreads) each *= 2;
-    for (int i0 = 0; i0 < n; i0 += kBeamSelectThreads / each) {
+    while (each < 16 && 2 * each * n <= THREADS) each *= 2;
+    for (int i0 = 0; i0 < n; i0 += THREADS / each) {
       const int i = i0 + tid / each;
       const BeamKey c = keys[i < n ? i : 0];
       int rank = 0;
@@ -589,7 +637,7 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
   }
   __syncthreads();
   BeamKey best{-INFINITY, kBeamNone};
-  for (int l = wave; l < lists; l += kBeamSelectWaves) {
+  for (int l = wave; l < lists; l += (THREADS / 64)) {
     if (state[l / S] != BEAM_LIVE) continue;
     const int n = part[l].count;
     for (int j0 = 0; j0 < n; j0 += 64) {
@@ -611,7 +659,7 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
   }
   keys[wave * 64 + lane] = best;
 #pragma unroll
-  for (int h = kBeamSelectWaves / 2; h >= 1; h >>= 1) {
+  for (int h = (THREADS / 64) / 2; h >= 1; h >>= 1) {
     __syncthreads();
     if (wave < h) {
       const BeamKey o = keys[(wave + h) * 64 + lane];
@@ -622,8 +670,48 @@ __global__ void __launch_bounds__(kBeamSelectThreads) beam_select_kernel(BeamArg
   if (wave == 0 && nan + lane < k) put(nan + lane, best);
 }
 
+// One launch: the last block of a request to finish its parts joins them.
+template <int DT>
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_select_kernel(BeamArgs a) {
+  using Join = BeamJoinLds<kBeamFew>;
+  constexpr size_t room = sizeof(BeamScanLds) > sizeof(Join) ? sizeof(BeamScanLds) : sizeof(Join);
+  __shared__ __attribute__((aligned(16))) char lds[room];
+  __shared__ int last;
+  const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int req = (int)blockIdx.x / a.blocks, l = (int)blockIdx.x % a.blocks * kBeamBlockWaves + wave;
+  if (l < a.beams * a.shares) {
+    const int row = req * a.beams + l / a.shares;
+    if (beam_state(a.scores[row], a.finished && a.finished[row]) == BEAM_LIVE)  // else its logits are not looked at
+      beam_scan<DT, true>(a, *(BeamScanLds*)lds, row, l % a.shares, wave, tid & 63);
+  }
+  // every wave's stores are performed before its block's ticket is drawn: the ticket is
+  // behind the barrier, the barrier behind the wait
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) last = ticket_add(a.tickets + req) == (unsigned int)a.blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0) __hip_atomic_store(a.tickets + req, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  beam_join<kBeamFew, kBeamThreads, true>(a, *(Join*)lds, req, tid);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(BeamArgs a) {
+  __shared__ __attribute__((aligned(16))) BeamScanLds lds;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l = (int)blockIdx.x * kBeamBlockWaves + wave, row = l / a.shares;
+  if (row >= a.batch * a.beams) return;
+  if (beam_state(a.scores[row], a.finished && a.finished[row]) != BEAM_LIVE) return;  // its logits are not looked at
+  beam_scan<DT, false>(a, lds, row, l % a.shares, wave, (int)threadIdx.x & 63);
+}
+
+__global__ void __launch_bounds__(kBeamJoinThreads) beam_join_kernel(BeamArgs a) {
+  __shared__ __attribute__((aligned(16))) BeamJoinLds<kBeamLists> lds;
+  beam_join<kBeamLists, kBeamJoinThreads, false>(a, lds, (int)blockIdx.x, (int)threadIdx.x);
+}
+
 // Parts of a row: enough waves to fill the device, whole chunks each, and few
-// enough lists for the second kernel.
+// enough lists for the join.
 static void beam_split(int rows, int beams, int vocab, int k, int dtype, int* shares, int* share, int* cap,
                        int* group) {
   const int chunk = 64 * kBeamVecs * (dtype == DT_F32 ? 4 : 8);
@@ -640,8 +728,29 @@ static void beam_split(int rows, int beams, int vocab, int k, int dtype, int* sh
   *cap = k <= 32 ? 128 : 256;  // 30 expected at K = 24, 37 at 32, 89 at 64
 }
 
-static size_t beam_bytes(int rows, int shares, int cap) {
-  return (size_t)rows * shares * sizeof(BeamPart) + (size_t)rows * shares * cap * sizeof(uint2);
+static size_t beam_bytes(int batch, int beams, int shares, int cap) {
+  return kBeamRequests * 4 + (size_t)batch * beams * shares * (sizeof(BeamPart) + cap * sizeof(uint2));
+}
+
+// The two launches of a call stay together on their stream: calls of several threads on
+// one stream may share a workspace.
+static std::mutex g_beam_mu;
+
+template <int DT>
+static int launch_beam(const BeamArgs& a, hipStream_t s) {
+  const int64_t waves = (int64_t)a.batch * a.beams * a.shares;
+  if (waves <= kBeamOne && a.beams * a.shares <= kBeamFew) {
+    hipLaunchKernelGGL(beam_select_kernel<DT>, dim3((unsigned)(a.batch * a.blocks)), dim3(kBeamThreads), 0, s, a);
+    NVJSEL_CHECK_LAUNCH("beam_select_kernel");
+    return NVJSEL_OK;
+  }
+  std::lock_guard<std::mutex> lock(g_beam_mu);
+  hipLaunchKernelGGL(beam_scan_kernel<DT>, dim3((unsigned)((waves + kBeamBlockWaves - 1) / kBeamBlockWaves)),
+                     dim3(kBeamThreads), 0, s, a);
+  NVJSEL_CHECK_LAUNCH("beam_scan_kernel");
+  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a.batch), dim3(kBeamJoinThreads), 0, s, a);
+  NVJSEL_CHECK_LAUNCH("beam_join_kernel");
+  return NVJSEL_OK;
 }
 
 // ---------------------------------------------------------------- state reordering
@@ -755,8 +864,8 @@ static int beam_check(const char* who, int dtype, int batch, int beams, int voca
     set_error("%s: beams (%d) and candidates (%d) must be in 1..%d", who, beams, k, kBeamMax);
     return NVJSEL_EINVAL;
   }
-  if (vocab > (1 << kBeamVocabBits) || (int64_t)batch * beams > (1 << 24)) {
-    set_error("%s: vocab (%d) or batch x beams too large", who, vocab);
+  if (vocab > (1 << kBeamVocabBits) || batch > kBeamRequests) {
+    set_error("%s: vocab (%d) must be at most 2^26, batch (%d) at most 65536", who, vocab, batch);
     return NVJSEL_EINVAL;
   }
   return NVJSEL_OK;
@@ -766,7 +875,7 @@ extern "C" size_t nvjsel_beam_select_workspace_size(int dtype, int batch, int be
   if (beam_check("beam_select", dtype, batch, beams, vocab, k) != NVJSEL_OK) return 0;
   int shares, share, cap, group;
   beam_split(batch * beams, beams, vocab, k, dtype, &shares, &share, &cap, &group);
-  return beam_bytes(batch * beams, shares, cap);
+  return beam_bytes(batch, beams, shares, cap);
 }
 
 extern "C" int nvjsel_beam_select(const void* logits, int dtype, int batch, int beams, int vocab, int64_t batch_stride,
@@ -794,26 +903,22 @@ extern "C" int nvjsel_beam_select(const void* logits, int dtype, int batch, int 
   a.finished = finished;
   a.end_token = end_token;
   beam_split(batch * beams, beams, vocab, k, dtype, &a.shares, &a.share, &a.cap, &a.group);
-  const size_t need = beam_bytes(batch * beams, a.shares, a.cap);
+  const size_t need = beam_bytes(batch, beams, a.shares, a.cap);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
     set_error("beam_select: workspace %zu bytes (16-byte aligned) < required %zu", workspace_bytes, need);
     return NVJSEL_EWORKSPACE;
   }
-  a.parts = (BeamPart*)workspace;
+  a.tickets = (unsigned int*)workspace;
+  a.blocks = (beams * a.shares + kBeamBlockWaves - 1) / kBeamBlockWaves;
+  a.parts = (BeamPart*)((char*)workspace + kBeamRequests * 4);
   a.cand = (uint2*)(a.parts + (size_t)batch * beams * a.shares);
   a.out_scores = out_scores;
   a.out_parents = out_parents;
   a.out_tokens = out_tokens;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t waves = (int64_t)batch * beams * a.shares;
-  const dim3 grid((unsigned)((waves + kBeamScanThreads / 64 - 1) / (kBeamScanThreads / 64)));
-  if (dtype == DT_F32) hipLaunchKernelGGL(beam_scan_kernel<DT_F32>, grid, dim3(kBeamScanThreads), 0, s, a);
-  else if (dtype == DT_BF16) hipLaunchKernelGGL(beam_scan_kernel<DT_BF16>, grid, dim3(kBeamScanThreads), 0, s, a);
-  else hipLaunchKernelGGL(beam_scan_kernel<DT_F16>, grid, dim3(kBeamScanThreads), 0, s, a);
-  NVJSEL_CHECK_LAUNCH("beam_scan_kernel");
-  hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)batch), dim3(kBeamSelectThreads), 0, s, a);
-  NVJSEL_CHECK_LAUNCH("beam_select_kernel");
-  return NVJSEL_OK;
+  if (dtype == DT_F32) return launch_beam<DT_F32>(a, s);
+  if (dtype == DT_BF16) return launch_beam<DT_BF16>(a, s);
+  return launch_beam<DT_F16>(a, s);
 }
 
 extern "C" int nvjsel_reorder_states(const nvjsel_state* states, int count, const int32_t* parents, int64_t parent_stride,

@@ -19,8 +19,8 @@
 // instructions: piece t (1 KB), lane l, word j hold row 16 t + (l & 15) and the
 // eight k at 32 j + 8 (l >> 4), the nibble of the even k = 2 p at bits 4 p, of 2 p + 1
 // at 16 + 4 p.  All k blocks of 32 rows lie together, then the next 32 rows.  The
-// scales follow, per block [row of 16][t][128 / group], and the zero points in the
-// same order.  Rows past V and k past H are zero with scale zero.
+// scales follow, per block [row of 16][t][128 / group], and the zero points, 16 added,
+// in the same order.  Rows past V and k past H are zero with scale zero.
 //
 // What bounds it: the weights' stream (7 TB/s), and beside it the sum of vector
 // and matrix instructions, which overlap little on a SIMD: measured with two
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
         for (int t = 0; t < NT; ++t) {
           if constexpr (ZEROS) {
             const int zi = (t & 1) * NG + g;  // byte of the block's zero points of this row
-            const float z = 16.0f + (float)((it.z[t >> 1][zi >> 2] >> (zshift + 8 * (zi & 3))) & 0xFFu);
+            const float z = (float)(((it.z[t >> 1][zi >> 2] >> zshift) >> (8 * (zi & 3))) & 0xFFu);  // packed as 16 + z
             acc[t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
           } else acc[t][m] = xs;
         }

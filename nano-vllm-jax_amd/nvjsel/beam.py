@@ -7,10 +7,11 @@ import math
 import torch
 
 from . import _lib
-from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle
+from ._tensors import _WS, _dtype_code, _on_device, _require_cuda, _stream_handle
 from .selection import lm_head_logits_hip, rms_norm_hip
 
 MAX_BEAMS = 64  # beams and candidates of a request
+MAX_REQUESTS, MAX_VOCAB = 65536, 1 << 26  # of a selection
 _MAX_STATES = 4096  # descriptions of one call
 
 
@@ -39,6 +40,8 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     k = beams if num_candidates is None else int(num_candidates)
     if beams > MAX_BEAMS or not 1 <= k <= MAX_BEAMS:
         raise ValueError(f"beams and num_candidates must be in 1..{MAX_BEAMS} (got {beams} and {k})")
+    if batch > MAX_REQUESTS or vocab > MAX_VOCAB:
+        raise ValueError(f"at most {MAX_REQUESTS} requests and {MAX_VOCAB} tokens (got {batch} and {vocab})")
     dt = _dtype_code(logits, "logits")
     if scores.shape != (batch, beams) or scores.dtype != torch.float32:
         raise ValueError("scores must be float32 [B, W]")
@@ -52,15 +55,22 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     if logits.stride(2) != 1 and vocab > 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    out_scores = scores.new_empty((batch, k))
-    parents, tokens = scores.new_empty((2, batch, k), dtype=torch.int32).unbind(0)
+    out, parents, tokens = scores.new_empty((3, batch, k), dtype=torch.int32).unbind(0)
+    out_scores = out.view(torch.float32)
     with _on_device(dev):
         nbytes = _lib.load().nvjsel_beam_select_workspace_size(dt, batch, beams, vocab, k)
-        ws = scores.new_empty((nbytes,), dtype=torch.uint8)
+        stream = _stream_handle(dev)
+        if torch.cuda.is_current_stream_capturing():
+            # a graph keeps a workspace of its own: graphs captured on one stream may be
+            # replayed at the same time
+            ws = scores.new_empty((nbytes,), dtype=torch.uint8)
+            ws[:4 * batch].zero_()  # the requests' tickets
+        else:
+            ws = _WS.get(dev, stream, "beam", nbytes)
         _lib.call("nvjsel_beam_select", logits.data_ptr(), dt, batch, beams, vocab, logits.stride(0), logits.stride(1),
                   scores.data_ptr(), None if finished is None else finished.data_ptr(), end_token or 0, k,
                   out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes,
-                  _stream_handle(dev))
+                  stream)
     return out_scores, parents, tokens
 
 
