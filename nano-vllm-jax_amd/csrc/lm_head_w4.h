@@ -60,6 +60,7 @@ struct W4Args {
   int zeros;   // zero points are there
   int V, H;
   int B;       // batch rows of this pass
+  int blocks;  // of each group of rows that a block holds; the groups follow each other in the grid
   int kc;      // k blocks of the hidden in LDS at a time
   int reduce_cast;
   unsigned long long* row_keys;
@@ -119,6 +120,7 @@ template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS>
 struct W4Stage {
   static constexpr int U = TERMS == 1 ? 8 : 4, EACH = kW4Threads / 16, LD = TERMS == 1 ? 1 : 2;
   static constexpr int TM = TERMS ? TERMS : 1, ROWS = TERMS ? RT * MB : 4;  // terms of a slot, rows to load
+  static constexpr int XS = TERMS == 3 ? 2 : 1;                              // sums of a group
   u32x4_t v[U][LD];
 
   __device__ __forceinline__ void load(const W4Args& a, int kb0, int items, int it0) {
@@ -184,13 +186,18 @@ struct W4Stage {
     for (int g = (int)threadIdx.x >> 6; g < nkb * NG; g += kW4Waves) {
 #pragma unroll
       for (int m = 0; m < MB; ++m) {
-        f32x4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4_t d[XS];
+#pragma unroll
+        for (int h = 0; h < XS; ++h) d[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < 4 / NG; ++j)
 #pragma unroll
           for (int c = TM - 1; c >= 0; --c)
-            d = mfma16x16x32<FMT>(mine[(((g * (4 / NG) + j) * MB + m) * TM + c) * 4 * RT], ones, d);
-        if ((lane & 15) == 0) *(f32x4_t*)(xsum + (g * MB + m) * 16 + 4 * (lane >> 4)) = d;
+            d[c ? XS - 1 : 0] =
+                mfma16x16x32<FMT>(mine[(((g * (4 / NG) + j) * MB + m) * TM + c) * 4 * RT], ones, d[c ? XS - 1 : 0]);
+#pragma unroll
+        for (int h = 0; h < XS; ++h)
+          if ((lane & 15) == 0) *(f32x4_t*)(xsum + ((g * MB + m) * XS + h) * 16 + 4 * (lane >> 4)) = d[h];
       }
     }
     __syncthreads();
@@ -213,25 +220,30 @@ struct W4Stage {
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, bool STAGED, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int TM = TERMS ? TERMS : 1;
+  constexpr int TM = TERMS ? TERMS : 1, XS = TERMS == 3 ? 2 : 1, ROWS = TERMS ? RT * MB : 4;
   constexpr int NB = STAGED ? 2 : 1, DEPTH = STAGED ? 2 : 4, NT = 2 * NB;
   const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // the block's group of batch rows
+  const int batch = a.B, blocks = a.blocks, row0 = (int)((unsigned)blockIdx.x / (unsigned)blocks) * ROWS;
+  const int block = (int)blockIdx.x - row0 / ROWS * blocks;
+  a.B = batch - row0 < ROWS ? batch - row0 : ROWS;
+  a.hidden = (const char*)a.hidden + (size_t)row0 * a.H * (TERMS == 1 ? 2 : 4);
   const int KB = lay.kblocks, kc = a.kc, col = lane & 15;
   u32x4_t* frag = (u32x4_t*)lds;
   float* xsum = (float*)(lds + (size_t)kc * 256 * TM * RT * MB);
   const u32x4_t* mine = frag + (lane >> 4) * RT + (lane & (RT - 1));
   const float* xmine = xsum + 4 * (lane >> 4);
 
-  const int step = (int)gridDim.x * kW4Waves, first = (int)blockIdx.x * kW4Waves + wave;
+  const int step = blocks * kW4Waves, first = block * kW4Waves + wave;
   const int supers = (lay.tiles + NB - 1) / NB;
-  const int full = STAGED ? (supers - (int)blockIdx.x * kW4Waves + step - 1) / step : lay.tiles / step;  // whole rounds
+  const int full = STAGED ? (supers - block * kW4Waves + step - 1) / step : lay.tiles / step;  // whole rounds
   // the block's rest: tiles from rest0, its k blocks dealt to the waves
   int rest0 = 0, nrest = 0;
   if (!STAGED) {
     const int rest = lay.tiles - full * step;
-    const int each = (int)((unsigned)rest / gridDim.x), more = rest - each * (int)gridDim.x, b = (int)blockIdx.x;
-    const int r0 = each * b + (b < more ? b : more), r1 = r0 + each + (b < more);
+    const int each = (int)((unsigned)rest / (unsigned)blocks), more = rest - each * blocks;
+    const int r0 = each * block + (block < more ? block : more), r1 = r0 + each + (block < more);
     rest0 = full * step + r0;
     nrest = (r1 - r0) * KB;
   }
@@ -308,7 +320,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
     for (int m = 0; m < MB; ++m) {
       const bool f32 = a.out_dtype == DT_F32;
       orow[m] = (char*)a.out_logits +
-                (size_t)(16 * m + 4 * (lane >> 4) + (f32 ? 0 : lane & 3)) * (size_t)a.out_stride * (f32 ? 4 : 2);
+                (size_t)(row0 + 16 * m + 4 * (lane >> 4) + (f32 ? 0 : lane & 3)) * (size_t)a.out_stride * (f32 ? 4 : 2);
     }
   }
 
@@ -405,22 +417,24 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
     const Item& it = ring[decltype(D)::value];
     const int kx = STAGED ? kl : kb;
     const u32x4_t* fk = mine + kx * (4 * MB * TM * 4 * RT);
-    const float* xk = xmine + kx * (NG * MB * 16);
+    const float* xk = xmine + kx * (NG * MB * XS * 16);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      f32x4_t acc[NT][MB];
+      f32x4_t acc[XS][NT][MB];
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const f32x4_t xs = *(const f32x4_t*)(xk + (g * MB + m) * 16);
+      for (int h = 0; h < XS; ++h)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (ZEROS) {
-            const int zi = (t & 1) * NG + g;  // byte of the block's zero points of this row
-            const float z = (float)(((it.z[t >> 1][zi >> 2] >> zshift) >> (8 * (zi & 3))) & 0xFFu);  // packed as 16 + z
-            acc[t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
-          } else acc[t][m] = xs;
+        for (int m = 0; m < MB; ++m) {
+          const f32x4_t xs = *(const f32x4_t*)(xk + ((g * MB + m) * XS + h) * 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (ZEROS) {
+              const int zi = (t & 1) * NG + g;  // byte of the block's zero points of this row
+              const float z = (float)(((it.z[t >> 1][zi >> 2] >> zshift) >> (8 * (zi & 3))) & 0xFFu);  // packed as 16 + z
+              acc[h][t][m] = f32x4_t{xs.x * z, xs.y * z, xs.z * z, xs.w * z};
+            } else acc[h][t][m] = xs;
+          }
         }
-      }
 #pragma unroll
       for (int j = g * 4 / NG; j < (g + 1) * 4 / NG; ++j) {
         u32x4_t wf[NT];
@@ -432,7 +446,8 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
           for (int c = TM - 1; c >= 0; --c) {
             const u32x4_t xf = fk[((j * MB + m) * TM + c) * 4 * RT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t][m] = mfma16x16x32<FMT>(xf, wf[t], acc[t][m]);
+            for (int t = 0; t < NT; ++t)
+              acc[c ? XS - 1 : 0][t][m] = mfma16x16x32<FMT>(xf, wf[t], acc[c ? XS - 1 : 0][t][m]);
           }
       }
 #pragma unroll
@@ -444,7 +459,10 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) total[t][m][i] = __builtin_fmaf(s, acc[t][m][i], total[t][m][i]);
+          for (int i = 0; i < 4; ++i) {
+            const float sum = XS == 2 ? acc[XS - 1][t][m][i] + acc[0][t][m][i] : acc[0][t][m][i];
+            total[t][m][i] = __builtin_fmaf(s, sum, total[t][m][i]);
+          }
       }
     }
     ++kl;
@@ -534,49 +552,114 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
         for (int x = 8; x >= 1; x >>= 1) k = max_u64(k, shfl_xor_u64(k, x));
         if (col == 0) red[wave * 16 * MB + 16 * m + 4 * (lane >> 4) + i] = k;
       }
-    block_commit<kW4Waves, 16 * MB>(red, a.B, a.row_keys);
-    finish_rows(a.row_keys, a.counter, a.B, a.out_ids, a.out_best);
+    block_commit<kW4Waves, 16 * MB>(red, a.B, a.row_keys + row0);
+    finish_rows(a.row_keys, a.counter, batch, a.out_ids, a.out_best);
   }
 }
 
-template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, int MODE>
-static int launch_w4(W4Args a, hipStream_t stream) {
-  const W4Layout lay = w4_layout(a.V, a.H, 128 / NG, ZEROS);
-  const size_t per_kb = (size_t)RT * MB * 256 * (TERMS ? TERMS : 1) + (size_t)NG * 16 * MB * 4;
-  const size_t parts = (size_t)kW4Waves * MB * 2048;  // of the tiles that waves split; the rows' keys need less
+// How a pass is laid over the device by one shape of tiles.
+struct W4Plan {
+  int groups, blocks;  // of batch rows; blocks of each
+  int kc;              // k blocks of the hidden in LDS at a time
+  bool staged;
+  size_t lds;
+  float us;  // estimated
+};
+
+// Rows beyond a tile's go to groups of blocks of their own, which read the same weights;
+// blocks with the same tiles share an XCD's L2 (blocks are dealt to the 8 XCDs in turn).
+static inline W4Plan w4_plan(const W4Args& a, int group, int terms, int mb, int rt) {
+  const W4Layout lay = w4_layout(a.V, a.H, group, a.zeros);
+  const size_t per_kb = (size_t)rt * mb * 256 * (terms ? terms : 1) + (size_t)lay.ng * 16 * mb * (terms == 3 ? 8 : 4);
+  const int rows = terms ? rt * mb : 4, cus = device_cu_count();
+  W4Plan p;
+  p.groups = (a.B + rows - 1) / rows;
   int chunks = 1;
   while ((size_t)((lay.kblocks + chunks - 1) / chunks) * per_kb > kW4Lds) ++chunks;
-  a.kc = (lay.kblocks + chunks - 1) / chunks;
-  size_t lds = a.kc * per_kb;
-  if (lds < parts) lds = parts;
-  auto kern = chunks == 1 ? lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, false, MODE>
-                          : lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, true, MODE>;
-  if (lds > 48 * 1024)
-    NVJSEL_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  const int cus = device_cu_count(), need = chunks == 1 ? lay.tiles : (lay.tiles + 2 * kW4Waves - 1) / (2 * kW4Waves);
-  hipLaunchKernelGGL(kern, dim3(need < cus ? need : cus), dim3(kW4Threads), lds, stream, a);
+  p.kc = (lay.kblocks + chunks - 1) / chunks;
+  p.staged = chunks > 1;
+  p.lds = p.kc * per_kb;
+  const size_t parts = (size_t)kW4Waves * mb * 2048;  // of the tiles that waves split; the rows' keys need less
+  if (p.lds < parts) p.lds = parts;
+  const int waves = p.staged ? (lay.tiles + 1) / 2 : lay.tiles, need = p.staged ? (waves + kW4Waves - 1) / kW4Waves : waves;
+  int most = cus / p.groups;
+  if (p.groups > 1 && most > 8) most &= ~7;
+  if (most < 1) most = 1;
+  p.blocks = need < most ? need : most;
+
+  // us: a call (between logits' and greedy's, so that both add up in the same order), and
+  // per k block the hidden's staging and a round of all waves: a fit to 1,276 timings
+  // (5..64 rows, V 2,000..248,320, H 512..8192; 5-12% rms).  The shape that it picks took
+  // 1% longer than the fastest on average, the widest one 48%.
+  struct Fit {
+    float call, stage, round, staged;
+  };
+  static constexpr Fit fits[4] = {
+      {6.3f, 0.12f, 0.55f, 1.04f},   // one tile of 16 rows
+      {7.3f, 0.22f, 0.73f, 1.48f},   // two
+      {9.2f, 0.55f, 1.21f, 2.36f},   // four
+      {6.4f, 0.34f, 0.85f, 1.94f}};  // one, three terms apart
+  const Fit& f = fits[terms == 3 ? 3 : mb == 4 ? 2 : mb - 1];
+  const int slots = p.blocks * kW4Waves;
+  const float each = p.staged ? f.staged * ((waves + slots - 1) / slots)
+                              : f.stage + f.round * fmaxf((float)waves / slots, 1.0f / kW4Waves);
+  p.us = f.call + lay.kblocks * each;
+  return p;
+}
+
+template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, int MODE>
+static int launch_w4(W4Args a, const W4Plan& p, hipStream_t stream) {
+  a.kc = p.kc;
+  a.blocks = p.blocks;
+  auto kern = p.staged ? lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, true, MODE>
+                       : lm_head_w4_kernel<FMT, TERMS, MB, RT, NG, ZEROS, false, MODE>;
+  if (p.lds > 48 * 1024)
+    NVJSEL_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
+  hipLaunchKernelGGL(kern, dim3(p.blocks * p.groups), dim3(kW4Threads), p.lds, stream, a);
   NVJSEL_CHECK_LAUNCH("lm_head_w4_kernel");
   return NVJSEL_OK;
 }
 
 template <int FMT, int TERMS, int MB, int RT, int MODE>
-static int launch_w4_group(const W4Args& a, int group, hipStream_t s) {
+static int launch_w4_group(const W4Args& a, int group, const W4Plan& p, hipStream_t s) {
   if (a.zeros) {
-    if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, true, MODE>(a, s);
-    if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, true, MODE>(a, s);
-    return launch_w4<FMT, TERMS, MB, RT, 4, true, MODE>(a, s);
+    if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, true, MODE>(a, p, s);
+    if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, true, MODE>(a, p, s);
+    return launch_w4<FMT, TERMS, MB, RT, 4, true, MODE>(a, p, s);
   }
-  if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, false, MODE>(a, s);
-  if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, false, MODE>(a, s);
-  return launch_w4<FMT, TERMS, MB, RT, 4, false, MODE>(a, s);
+  if (group == 128) return launch_w4<FMT, TERMS, MB, RT, 1, false, MODE>(a, p, s);
+  if (group == 64) return launch_w4<FMT, TERMS, MB, RT, 2, false, MODE>(a, p, s);
+  return launch_w4<FMT, TERMS, MB, RT, 4, false, MODE>(a, p, s);
 }
 
+// The widest tile reads and unpacks the weights the fewest times; narrower ones leave more
+// of the hidden in LDS (64 rows, V = 32,000, H = 4096: 38 us with 16 rows a tile, 76 with
+// 64, staged) and give a small vocabulary's tiles to more blocks (32 rows, V = 8000, H = 1024: 5.7 us
+// with 16 rows, 7.5 with 32), but a large one costs more with them (64 rows, V = 248,320, H =
+// 1024: 70 us with 16, 49 with 64).  f32: the terms apart where the hidden stays in LDS so
+// (16 rows, V = 248,320, H = 1024: 36 us, 67 in fours), rows in fours where not (V = 8000, H =
+// 4096: 16 us, 63 staged); two tiles of three terms were no faster than two groups of one.
 template <int FMT, int TERMS, int MODE>
 static int w4_pass(const W4Args& a, int group, hipStream_t s) {
-  if (a.B <= 4) return launch_w4_group<FMT, TERMS == 3 ? 0 : TERMS, 1, TERMS == 3 ? 16 : 4, MODE>(a, group, s);
-  if (a.B <= 16) return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, s);
-  if (a.B <= 32) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, s);
-  return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, s);
+  if constexpr (TERMS == 3) {
+    const W4Plan fours = w4_plan(a, group, 0, 1, 16), one = w4_plan(a, group, 3, 1, 16);
+    if (a.B <= 4 || fours.us < one.us) return launch_w4_group<FMT, 0, 1, 16, MODE>(a, group, fours, s);
+    return launch_w4_group<FMT, 3, 1, 16, MODE>(a, group, one, s);
+  } else {
+    if (a.B <= 4) return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, w4_plan(a, group, TERMS, 1, 4), s);
+    W4Plan best = w4_plan(a, group, TERMS, 1, 16);
+    int mb = 1;
+    for (int m = 2; 8 * m < a.B && m <= 4; m *= 2) {
+      const W4Plan p = w4_plan(a, group, TERMS, m, 16);
+      if (p.us < best.us) {
+        best = p;
+        mb = m;
+      }
+    }
+    if (mb == 4) return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, best, s);
+    if (mb == 2) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, best, s);
+    return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, best, s);
+  }
 }
 
 // The passes by mode and activation type, each in a translation unit of its

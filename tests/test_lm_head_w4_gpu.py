@@ -94,6 +94,56 @@ def test_logits_and_greedy(rows, vocab, hidden, group, act, scale, zeros):
         assert np.array_equal(best.cpu().numpy(), l.max(1))
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(3, 300), (16, 1000), (5, 40000), (16, 40000), (33, 40000)])
+def test_f32_terms_do_not_round_each_other(rows, vocab, zeros):
+    """Activations hi + lo, hi an integer of 8 bits and lo a multiple of 2^-11 below one:
+    over 128 of them, each part's sum with codes below 32 fits 24 bits (255 x 31 x 128 <
+    2^20; 2^11 x 31 x 128 < 2^23), both together need 31.  Kept apart they meet in at
+    most two roundings, each of at most the result and lo's part (31 x 128 x 2^-8 < 16
+    of the last term); the scale is a power of two."""
+    rng = np.random.default_rng(rows + vocab)
+    hi = rng.integers(128, 256, (rows, 128)) * rng.choice([-1, 1], (rows, 128))
+    x = hi + np.sign(hi) * rng.integers(0, 2048, (rows, 128)) / 2048.0
+    x = torch.from_numpy(x.astype(np.float32))
+    codes, q, scales, z = make(vocab, 128, 128, torch.float16, zeros, 3)
+    scales.fill_(0.125)
+    head = nvjsel.pack_lm_head_w4(q.cuda(), scales.cuda(), None if z is None else z.cuda())
+    want, _ = exact(codes, scales, z, 128, x)
+    got = nvjsel.lm_head_logits_hip(x.cuda(), head).double().cpu()
+    assert bool(((got - want).abs() <= 2.0 ** -24 * (2 * want.abs() + 2)).all())
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,group,act,zeros", [
+    (16, 40000, 1024, 128, "f32", True),    # terms apart, hidden in LDS
+    (16, 9000, 1664, 64, "f32", False),     # rows in fours: four groups of blocks
+    (31, 70000, 2048, 128, "f32", False),   # terms apart, hidden in parts
+    (64, 9000, 2048, 32, "bf16", True),     # four groups of 16 rows
+    (40, 33000, 1024, 128, "f16", False),   # two groups of 32, the second with 8
+    (48, 9000, 1024, 128, "bf16", False),   # three groups: blocks not a power of two
+    (64, 70000, 1024, 64, "f16", True),     # one tile of 64
+    (64, 70000, 8192, 128, "bf16", False),  # in parts
+])
+def test_tile_shapes(rows, vocab, hidden, group, act, zeros):
+    """Sizes at which each shape of tiles is taken; a sample of the vocabulary is compared."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    q = torch.randint(0, 256, (vocab, hidden // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.002 + 0.01 * torch.rand(vocab, hidden // group, generator=g, device="cuda")).to(DT["f16"])
+    z = torch.randint(0, 16, (vocab, hidden // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    x = hidden_rows(rows, hidden, DT[act], 4)
+    head = nvjsel.pack_lm_head_w4(q, scales, z)
+    logits = nvjsel.lm_head_logits_hip(x.cuda(), head, reduce_cast=0)
+    pick = torch.cat([torch.arange(0, vocab, 37), torch.arange(vocab - 70, vocab)])
+    qp = q[pick.cuda()].cpu()
+    codes = torch.stack([qp & 15, qp >> 4], 2).reshape(len(pick), hidden)
+    want, mag = exact(codes, scales[pick.cuda()].cpu(), None if z is None else z[pick.cuda()].cpu(), group, x)
+    assert bool(((logits[:, pick.cuda()].double().cpu() - want).abs() <= tolerance(want, mag, torch.float32)).all())
+    ids, best = nvjsel.lm_head_greedy_top1_hip(x.cuda().reshape(rows, 1, hidden), head, reduce_cast=0, return_best=True)
+    l = logits.cpu().numpy()
+    assert np.array_equal(ids.cpu().numpy()[:, 0], l.argmax(1))
+    assert np.array_equal(best.cpu().numpy(), l.max(1))
+
+
 def test_other_routes_take_the_weight():
     """Sampling, top-k, the prenorm input and the MTP route are those of the dense logits."""
     codes, q, scales, z = make(3001, 512, 64, torch.bfloat16, True, 5)
