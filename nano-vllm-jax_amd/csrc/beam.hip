@@ -38,7 +38,9 @@ static constexpr int kBeamThreads = 256, kBeamBlockWaves = kBeamThreads / 64;
 static constexpr int kBeamOne = 512, kBeamFew = 256, kBeamLists = 2048;
 static constexpr int kBeamJoinThreads = 512;             // of the second kernel
 static constexpr int kBeamOneMax = 24;     // candidates that one maximum per lane bounds well enough, two above
-static constexpr int kBeamClasses = 128;   // of parts, two per lane, for the join's bound
+static constexpr int kBeamClasses = 128;   // of parts or candidates, two per lane, for the join's bounds
+static constexpr int kBeamFewShares = 4;   // of a row, whose sums a lane joins, not a wave (64 beams of one share: 14 us by waves, 1.2 so)
+static constexpr int kBeamRefine = 128;    // candidates that are ranked without a second bound
 
 struct BeamPart {  // of one wave's share of a row
   double sum;      // sum of exp(l - max)
@@ -535,23 +537,33 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     rscore[tid] = (double)sc;
   }
   __syncthreads();
-  for (int w = wave; w < W; w += (THREADS / 64)) {
-    int st = state[w];
-    if (st != BEAM_LIVE) continue;
-    const BeamPart* p = part + w * S;
-    float m = -INFINITY;
-    double t = 0.0;
-    for (int i = lane; i < S; i += 64) m = fmaxf(m, p[i].max);
-    m = wave_max_f32(m);
-    const double ref = m == -INFINITY ? 0.0 : (double)m;
-    for (int i = lane; i < S; i += 64) t += p[i].sum * exp((double)p[i].max - ref);
-    t = wave_sum_f64(t);
-    if (!(t < INFINITY)) st = BEAM_NAN;      // a NaN or an infinity among the logits
-    else if (m == -INFINITY) st = BEAM_DEAD;  // the mask leaves nothing
-    if (lane == 0) {
-      state[w] = st;
-      rmax[w] = m;
-      rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
+  auto norm = [&](int w, float m, double t) NVJSEL_INLINE {  // a beam's maximum, and the sum relative to it
+    const int st = !(t < INFINITY) ? BEAM_NAN : m == -INFINITY ? BEAM_DEAD : BEAM_LIVE;  // NaN: or an infinity; the mask leaves nothing
+    state[w] = st;
+    rmax[w] = m;
+    rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
+  };
+  auto part_sum = [&](const BeamPart& p, float m) { return p.sum * exp((double)p.max - (m == -INFINITY ? 0.0 : (double)m)); };
+  if (S <= kBeamFewShares) {  // a lane each
+    if (tid < W && state[tid] == BEAM_LIVE) {
+      const BeamPart* p = part + tid * S;
+      float m = -INFINITY;
+      double t = 0.0;
+      for (int i = 0; i < S; ++i) m = fmaxf(m, p[i].max);
+      for (int i = 0; i < S; ++i) t += part_sum(p[i], m);
+      norm(tid, m, t);
+    }
+  } else {  // a wave each
+    for (int w = wave; w < W; w += (THREADS / 64)) {
+      if (state[w] != BEAM_LIVE) continue;
+      const BeamPart* p = part + w * S;
+      float m = -INFINITY;
+      double t = 0.0;
+      for (int i = lane; i < S; i += 64) m = fmaxf(m, p[i].max);
+      m = wave_max_f32(m);
+      for (int i = lane; i < S; i += 64) t += part_sum(p[i], m);
+      t = wave_sum_f64(t);
+      if (lane == 0) norm(w, m, t);
     }
   }
   __syncthreads();
@@ -569,11 +581,11 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     }
   }
   __syncthreads();
-  const uint64_t low = (uint64_t)wave_kth(best_of[lane], best_of[64 + lane], k, 12) << 32;
+  // to 12 bits of the score's mantissa
+  uint64_t low = (uint64_t)wave_kth(best_of[lane], best_of[64 + lane], k, 8) << 32;
 
-  auto candidate = [&](int l, int j) {  // candidate j of part l
+  auto scored = [&](int l, uint2 e) {  // a candidate of part l
     const int w = l / S;
-    const uint2 e = beam_get<ONE>(a.cand + ((size_t)req * lists + l) * a.cap + j);
     const float x = __uint_as_float(e.x);
     return BeamKey{score(w, x), beam_at(w, x, e.y)};
   };
@@ -590,23 +602,65 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     }
   __syncthreads();
   const int nl = (int)(uint32_t)taken, nc = (int)(taken >> 32);
-  for (int i = tid; i < nc; i += THREADS) {
-    int lo = 0, hi = nl;  // the last list that starts at or before i
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid] <= i) lo = mid;
-      else hi = mid;
+  auto gather = [&](bool all) NVJSEL_INLINE {  // or until there are too many to rank
+    constexpr int AHEAD = 4;  // loads of a thread on their way together
+    for (int i0 = tid; i0 < nc; i0 += AHEAD * THREADS) {
+      if (!all && *(volatile int*)&found > RANKED) break;
+      int of[AHEAD];
+      uint2 e[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = min(i0 + u * THREADS, nc - 1);
+        int lo = 0, hi = nl;  // the last list that starts at or before i
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (start[mid] <= i) lo = mid;
+          else hi = mid;
+        }
+        of[u] = list[lo];
+        e[u] = beam_get<ONE>(a.cand + ((size_t)req * lists + of[u]) * a.cap + (i - start[lo]));
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (i0 + u * THREADS < nc) add(scored(of[u], e[u]));
     }
-    add(candidate(list[lo], i - start[lo]));
+    if (tid < W && state[tid] == BEAM_ENDED) add(BeamKey{rscore[tid], beam_at(tid, 0.0f, (uint32_t)a.end_token)});
+    __syncthreads();
+  };
+  gather(false);
+
+  // Few parts bound badly, fewer than K not at all: the bound again, by the candidates' own
+  // classes (18 requests, 8 beams, V = 2332, K = 16: 54 us with the 300 candidates ranked, 17 so)
+  if (found > max(kBeamRefine, 3 * k)) {  // block-uniform
+    static_assert(RANKED == 2 * THREADS, "");
+    const int n = found;
+    BeamKey mine[2] = {keys[tid], keys[tid + THREADS]};
+    __syncthreads();
+    if (tid < kBeamClasses) best_of[tid] = 0;
+    if (tid == 0) found = 0;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (tid + h * THREADS < n) atomicMax(&best_of[tid % kBeamClasses], (uint32_t)(beam_ord(mine[h].s) >> 32));
+    __syncthreads();
+    const uint64_t t = (uint64_t)wave_kth(best_of[lane], best_of[64 + lane], k, 4) << 32;
+    low = t > low ? t : low;
+    if (n <= RANKED) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (tid + h * THREADS < n) add(mine[h]);
+      __syncthreads();
+    } else {
+      gather(true);
+    }
   }
-  if (tid < W && state[tid] == BEAM_ENDED) add(BeamKey{rscore[tid], beam_at(tid, 0.0f, (uint32_t)a.end_token)});
-  __syncthreads();
 
   // NaN candidates come first, by place: every token of a NaN beam, the end token of an ended one
   int nan = 0;
   uint64_t nan_at = kBeamNone;
-  for (int w = 0; w < W && nan < k; ++w) {
-    const int st = state[w];
+  const int own = lane < W ? state[lane] : BEAM_DEAD;
+  for (uint64_t b = __ballot(own == BEAM_NAN || own == BEAM_ENDED_NAN); b && nan < k; b &= b - 1) {
+    const int w = __builtin_ctzll(b), st = state[w];
     const int n = st == BEAM_NAN ? min(a.vocab, k - nan) : st == BEAM_ENDED_NAN ? 1 : 0;
     if (tid >= nan && tid < nan + n) nan_at = beam_at(w, 0.0f, (uint32_t)(st == BEAM_NAN ? tid - nan : a.end_token));
     nan += n;
@@ -642,7 +696,7 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     const int n = part[l].count;
     for (int j0 = 0; j0 < n; j0 += 64) {
       BeamKey c{-INFINITY, kBeamNone};
-      if (j0 + lane < n) c = candidate(l, j0 + lane);
+      if (j0 + lane < n) c = scored(l, beam_get<ONE>(a.cand + ((size_t)req * lists + l) * a.cap + j0 + lane));
       if (!__any(beam_before(c, beam_from(best, k - 1)))) continue;
       beam_sort(c, lane);
       beam_merge(best, c, lane);

@@ -94,6 +94,21 @@ def test_select(b, w, v, k, dtype):
     check(logits, scores, k)
 
 
+@pytest.mark.parametrize("b,w,v,k,dtype", [(18, 8, 2332, 16, "f16"), (16, 16, 2000, 16, "bf16"), (2, 16, 2000, 32, "f32"),
+                                           (2, 64, 2000, 64, "f16"), (40, 64, 2100, 64, "bf16"), (5, 3, 5000, 64, "f32")])
+def test_few_parts_many_candidates(b, w, v, k, dtype):
+    """Fewer parts than candidates, or not many more: one bound from the parts is not enough."""
+    logits, scores = make(b, w, v, dtype, 77 + v + w)
+    check(logits, scores, k)
+    finished = torch.zeros(b, w, dtype=torch.bool)
+    finished[:, w // 2:] = True
+    check(logits, scores, k, finished, 7)
+    scores[:, ::2] = NINF
+    check(logits, scores, k)
+    if w <= 16:  # equal logits: more than are ranked
+        check(logits.to(DT["bf16"]).round().to(DT[dtype]), torch.zeros_like(scores), k)
+
+
 def test_first_step_and_ended_beams():
     logits, scores = make(4, 4, 5003, "bf16", 3)
     scores[:, 1:] = NINF
