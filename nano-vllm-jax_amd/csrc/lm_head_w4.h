@@ -34,6 +34,7 @@ namespace nvjsel {
 
 static constexpr int kW4Waves = 8, kW4Threads = 64 * kW4Waves;
 static constexpr size_t kW4Lds = 150 * 1024;  // for the hidden and its groups' sums
+static constexpr int kW4Turn = 8;             // k blocks between barriers at most, where not all of it fits
 
 struct W4Layout {
   int tiles, kblocks, ng;  // 32-row tiles, 128-wide k blocks, groups per k block
@@ -61,7 +62,7 @@ struct W4Args {
   int V, H;
   int B;       // batch rows of this pass
   int blocks;  // of each group of rows that a block holds; the groups follow each other in the grid
-  int kc;      // k blocks of the hidden in LDS at a time
+  int kc;      // k blocks of the hidden that LDS holds
   int reduce_cast;
   unsigned long long* row_keys;
   unsigned int* counter;
@@ -107,13 +108,21 @@ __device__ __forceinline__ u32x4_t w4_unpack(uint32_t w, const W4Consts& c) {
   return r;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+
 // k blocks kb0 .. of the hidden into LDS, as the matrix instructions' operands:
 // 16-byte slots [((4 kb + j) MB + mb) TERMS + t][k quarter][row of RT].  Three terms: x =
 // the bf16 values that its leading, next and last eight bits make (exact); a value
 // that is not finite keeps its first term only.  No terms (0): f32 too, the three of
 // up to four batch rows as rows 4 t + b of one matrix tile, a third of the products; the
 // last four rows stay as LDS was and are left out of the results.  Then, by the matrix cores, the
-// groups' sums of activations times -1 (zero points) or -(16 + 8): xsum [group][16 MB].
+// groups' sums of activations times -1 (zero points) or -(16 + 8): xsum [group][MB][16],
+// with three terms the leading one's sums, then the other two's.  Each has accumulators of
+// its own: at the leading term's offset the others would lose half of their bits (16
+// rows, H = 1024: relative error 1.5e-6 with one sum, 2e-7 with two).
 // first(): the loads that may be on their way while the weights' first ones are
 // requested; rest(): everything else.
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS>
@@ -123,10 +132,11 @@ struct W4Stage {
   static constexpr int XS = TERMS == 3 ? 2 : 1;                              // sums of a group
   u32x4_t v[U][LD];
 
+  template <int N = U>
   __device__ __forceinline__ void load(const W4Args& a, int kb0, int items, int it0) {
     const int u = (int)threadIdx.x & 15;  // eight k of a k block
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int it = it0 + i * EACH, row = it % (ROWS), k = (kb0 + it / (ROWS)) * 128 + 8 * u;
       const bool in = it < items && row < a.B && k < a.H;
       const size_t at = in ? (size_t)row * a.H + k : 0;  // always a load, of the first values where none is wanted
@@ -137,35 +147,82 @@ struct W4Stage {
       }
     }
   }
-  __device__ __forceinline__ void store(const W4Args& a, int kb0, int items, int it0, u32x4_t* frag) {
+  // Item i's eight values in their slots, kb the k block's place in LDS; put: its terms as
+  // they go there, zero where the item lies outside.
+  static constexpr int PUT = TERMS == 1 ? 1 : 3;
+  __device__ __forceinline__ void put(int i, bool in, int kb, int row, u32x4_t* frag, u32x4_t (&out)[PUT]) {
     const int u = (int)threadIdx.x & 15;
+    u32x4_t* dst = frag + (((kb * 4 + (u >> 2)) * MB + row / RT) * TM * 4 + (u & 3)) * RT + row % RT;
+    if constexpr (TERMS == 1) {
+      out[0] = in ? v[i][0] : u32x4_t{0u, 0u, 0u, 0u};
+      *dst = out[0];
+    } else {
+      uint32_t h[3][8];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int it = it0 + i * EACH, row = it % (ROWS), kb = it / (ROWS), k = (kb0 + kb) * 128 + 8 * u;
-      if (it >= items) break;
-      const bool in = row < a.B && k < a.H;
-      u32x4_t* dst = frag + (((kb * 4 + (u >> 2)) * MB + row / RT) * TM * 4 + (u & 3)) * RT + row % RT;
-      if constexpr (TERMS == 1) {
-        *dst = in ? v[i][0] : u32x4_t{0u, 0u, 0u, 0u};
-      } else {
-        uint32_t h[3][8];
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = in ? v[i][e >> 2][e & 3] : 0u;
+        const float x = __uint_as_float(b);
+        const bool fin = (b & 0x7F800000u) != 0x7F800000u;
+        h[0][e] = fin ? b >> 16 : bf16_bits_rne(x);
+        const float r1 = x - __uint_as_float(b & 0xFFFF0000u);
+        h[1][e] = fin ? __float_as_uint(r1) >> 16 : 0u;
+        const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xFFFF0000u);
+        h[2][e] = fin ? __float_as_uint(r2) >> 16 : 0u;
+      }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t b = in ? v[i][e >> 2][e & 3] : 0u;
-          const float x = __uint_as_float(b);
-          const bool fin = (b & 0x7F800000u) != 0x7F800000u;
-          h[0][e] = fin ? b >> 16 : bf16_bits_rne(x);
-          const float r1 = x - __uint_as_float(b & 0xFFFF0000u);
-          h[1][e] = fin ? __float_as_uint(r1) >> 16 : 0u;
-          const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xFFFF0000u);
-          h[2][e] = fin ? __float_as_uint(r2) >> 16 : 0u;
-        }
-#pragma unroll
-        for (int t = 0; t < 3; ++t)
-          dst[TERMS ? t * 4 * RT : 4 * t] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16,
-                                    h[t][6] | h[t][7] << 16};
+      for (int t = 0; t < 3; ++t) {
+        out[t] = u32x4_t{h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16, h[t][4] | h[t][5] << 16, h[t][6] | h[t][7] << 16};
+        dst[TERMS ? t * 4 * RT : 4 * t] = out[t];
       }
     }
+  }
+  __device__ __forceinline__ void store(const W4Args& a, int kb0, int items, int it0, u32x4_t* frag) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int it = it0 + i * EACH, row = it % (ROWS), kb = it / (ROWS), k = (kb0 + kb) * 128 + 8 * ((int)threadIdx.x & 15);
+      if (it >= items) break;
+      u32x4_t out[PUT];
+      put(i, row < a.B && k < a.H, kb, row, frag, out);
+    }
+  }
+  // One k block at a time, on its way while others are in work (STAGED): load() with
+  // one k block's items, then this, its groups' sums by the lanes that hold them.
+  static_assert(ROWS <= EACH * U, "");
+  __device__ __forceinline__ void store_one(const W4Args& a, int kb0, int at, u32x4_t* frag, float* xsum) {
+    const int u = (int)threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < (ROWS + EACH - 1) / EACH; ++i) {
+      const int row = ((int)threadIdx.x >> 4) + i * EACH;
+      if (ROWS % EACH && row >= ROWS) break;
+      u32x4_t out[PUT];
+      put(i, row < a.B && kb0 * 128 + 8 * u < a.H, at, row, frag, out);
+      float sum[PUT];
+#pragma unroll
+      for (int t = 0; t < PUT; ++t) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t w = out[t][e >> 1];
+          s += FMT == DT_BF16 ? __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16) : f16_to_f32((uint16_t)(e & 1 ? w >> 16 : w));
+        }
+        sum[t] = s;
+      }
+      if constexpr (TERMS == 3) sum[1] += sum[2];
+      const float f = ZEROS ? -1.0f : -24.0f;
+#pragma unroll
+      for (int t = 0; t < (TERMS == 0 ? 3 : XS); ++t) {
+        float s = sum[t];  // over the 16 / NG lanes of a group
+        s += dpp_f32<0xB1>(s);
+        s += dpp_f32<0x4E>(s);
+        if (NG <= 2) s += dpp_f32<0x141>(s);
+        if (NG == 1) s += dpp_f32<0x140>(s);
+        if (u % (16 / NG) == 0)
+          xsum[((at * NG + u / (16 / NG)) * MB + row / 16) * XS * 16 + (TERMS == 0 ? 4 * t + row : 16 * t + row % 16)] = s * f;
+      }
+    }
+  }
+  __device__ __forceinline__ void load_one(const W4Args& a, int kb) {
+    load<(ROWS + EACH - 1) / EACH>(a, kb, ROWS, (int)threadIdx.x >> 4);
   }
   __device__ __forceinline__ void first(const W4Args& a, int kb0, int nkb) {
     load(a, kb0, ROWS * nkb, (int)threadIdx.x >> 4);
@@ -206,8 +263,8 @@ struct W4Stage {
 
 // One block per CU, eight waves.  A wave takes a block of 32 vocabulary rows at a
 // time and runs over all of H, its next k blocks' pieces on the way in registers
-// (DEPTH); the waves share the hidden in LDS, all of it where it fits, kc k blocks at
-// a time where not (STAGED).  Matrix tile: M = batch rows (MB tiles of 16), N =
+// (DEPTH); the waves share the hidden in LDS, all of it where it fits, kc k blocks in
+// a ring where not (STAGED).  Matrix tile: M = batch rows (MB tiles of 16), N =
 // vocabulary rows, so that a lane's results share their scale.  RT: batch rows that
 // have slots in LDS (4: the others repeat them).
 //
@@ -215,8 +272,11 @@ struct W4Stage {
 // dealt to the blocks, and a block splits its rest by k blocks over its waves, which
 // join their parts through LDS at the end (V = 151,936, H = 2560, 8 rows: 46 us with
 // whole tiles only, 2.3 rounds of them, 42 split).  STAGED waves walk the k blocks
-// together, two tiles at a time (NB: half as many reads of the hidden, and stagings), and
-// repeat the last one instead.
+// together, two tiles at a time (NB: half as many reads of the hidden), and repeat the
+// last tile instead; with every k block the block stores one of the hidden, requested
+// with the last one, for half a ring later, and a barrier every half ring keeps both
+// ends apart (64 rows, V = 128,256, H = 2048: 58 us where all waves stopped to fill the
+// LDS, 50 so).
 template <int FMT, int TERMS, int MB, int RT, int NG, bool ZEROS, bool STAGED, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -406,16 +466,23 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   };
 
   int kb = full ? 0 : tail_kb, tile = full ? first : tail_tile, left = full;  // the item in work
-  int kl = 0;  // its k block in LDS (STAGED)
+  // STAGED: the item's place in LDS, the items to the next barrier; the k block on its way and its place
+  int at = 0, turn = 0, skb = kc / 2 % KB, sat = kc / 2;
+  W4Stage<FMT, TERMS, MB, RT, NG, ZEROS> st;
   auto body = [&](auto D) NVJSEL_INLINE {
-    if (STAGED && kl == 0) {
-      __syncthreads();
-      W4Stage<FMT, TERMS, MB, RT, NG, ZEROS> st;
-      st.first(a, kb, KB - kb < kc ? KB - kb : kc);
-      st.rest(a, kb, KB - kb < kc ? KB - kb : kc, frag, xsum);
+    if constexpr (STAGED) {
+      if (turn == 0) {
+        __syncthreads();
+        turn = kc / 2;
+      }
+      --turn;
+      st.store_one(a, skb, sat, frag, xsum);
+      if (++skb == KB) skb = 0;
+      if (++sat == kc) sat = 0;
+      st.load_one(a, skb);
     }
     const Item& it = ring[decltype(D)::value];
-    const int kx = STAGED ? kl : kb;
+    const int kx = STAGED ? at : kb;
     const u32x4_t* fk = mine + kx * (4 * MB * TM * 4 * RT);
     const float* xk = xmine + kx * (NG * MB * XS * 16);
 #pragma unroll
@@ -465,8 +532,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
           }
       }
     }
-    ++kl;
-    if (STAGED && kl == kc) kl = 0;
+    if (STAGED && ++at == kc) at = 0;
     if (++kb < KB) return;
     if (!STAGED && left == 0 && tile == tail_tile && tail_kb != 0) {  // the end of another wave's tile
 #pragma unroll
@@ -484,7 +550,6 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
       for (int m = 0; m < MB; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) total[t][m][i] = 0.0f;
-    kl = 0;
     if (left > 0) --left;  // as the loads go
     const bool to_tail = left == 0 && (tile < rest0 || STAGED);
     kb = to_tail ? tail_kb : 0;
@@ -494,11 +559,17 @@ __global__ void __launch_bounds__(kW4Threads, 2) lm_head_w4_kernel(W4Args a) {
   // Every load is unconditional (tiles past the end repeat the last one), so that the
   // waits count the same requests on every path to a body: with bounds tests before
   // the first loads each round of the ring waited for all of it.
-  {
-    W4Stage<FMT, TERMS, MB, RT, NG, ZEROS> st;
-    if (!STAGED) st.first(a, 0, KB);
+  if constexpr (STAGED) {
     static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE { load(D); });
-    if (!STAGED) st.rest(a, 0, KB, frag, xsum);
+    for (int i = 0; i < kc / 2; ++i) {
+      st.load_one(a, i % KB);
+      st.store_one(a, i % KB, i, frag, xsum);
+    }
+    st.load_one(a, skb);
+  } else {
+    st.first(a, 0, KB);
+    static_for<DEPTH - 1>([&](auto D) NVJSEL_INLINE { load(D); });
+    st.rest(a, 0, KB, frag, xsum);
   }
   int i = 0;
   for (; i + DEPTH <= n; i += DEPTH)
@@ -574,10 +645,9 @@ static inline W4Plan w4_plan(const W4Args& a, int group, int terms, int mb, int 
   const int rows = terms ? rt * mb : 4, cus = device_cu_count();
   W4Plan p;
   p.groups = (a.B + rows - 1) / rows;
-  int chunks = 1;
-  while ((size_t)((lay.kblocks + chunks - 1) / chunks) * per_kb > kW4Lds) ++chunks;
-  p.kc = (lay.kblocks + chunks - 1) / chunks;
-  p.staged = chunks > 1;
+  const int fit = (int)(kW4Lds / per_kb);
+  p.staged = lay.kblocks > fit;
+  p.kc = p.staged ? 2 * (fit / 2 < kW4Turn ? fit / 2 : kW4Turn) : lay.kblocks;
   p.lds = p.kc * per_kb;
   const size_t parts = (size_t)kW4Waves * mb * 2048;  // of the tiles that waves split; the rows' keys need less
   if (p.lds < parts) p.lds = parts;
@@ -588,18 +658,20 @@ static inline W4Plan w4_plan(const W4Args& a, int group, int terms, int mb, int 
   p.blocks = need < most ? need : most;
 
   // us: a call (between logits' and greedy's, so that both add up in the same order), and
-  // per k block the hidden's staging and a round of all waves: a fit to 1,276 timings
-  // (5..64 rows, V 2,000..248,320, H 512..8192; 5-12% rms).  The shape that it picks took
-  // 1% longer than the fastest on average, the widest one 48%.
+  // per k block the hidden's staging and a round of all waves: a fit to 754 timings
+  // (5..64 rows, V 2,000..248,320, H 512..8192; 4-9% rms).  The shape that it picks took
+  // 0.3% longer than the fastest on average, the widest one 53%.
   struct Fit {
     float call, stage, round, staged;
   };
-  static constexpr Fit fits[4] = {
-      {6.3f, 0.12f, 0.55f, 1.04f},   // one tile of 16 rows
-      {7.3f, 0.22f, 0.73f, 1.48f},   // two
-      {9.2f, 0.55f, 1.21f, 2.36f},   // four
-      {6.4f, 0.34f, 0.85f, 1.94f}};  // one, three terms apart
-  const Fit& f = fits[terms == 3 ? 3 : mb == 4 ? 2 : mb - 1];
+  static constexpr Fit fits[6] = {
+      {6.5f, 0.03f, 0.45f, 1.00f},   // four rows
+      {6.4f, 0.10f, 0.53f, 0.98f},   // one tile of 16
+      {7.4f, 0.22f, 0.70f, 1.42f},   // two
+      {9.6f, 0.55f, 1.21f, 2.20f},   // four
+      {6.6f, 0.09f, 0.50f, 1.20f},   // four rows of three terms
+      {6.5f, 0.34f, 0.85f, 1.90f}};  // one tile, three terms apart
+  const Fit& f = fits[terms == 3 ? 5 : terms == 0 ? 4 : rt == 4 ? 0 : mb == 4 ? 3 : mb];
   const int slots = p.blocks * kW4Waves;
   const float each = p.staged ? f.staged * ((waves + slots - 1) / slots)
                               : f.stage + f.round * fmaxf((float)waves / slots, 1.0f / kW4Waves);
@@ -646,10 +718,9 @@ static int w4_pass(const W4Args& a, int group, hipStream_t s) {
     if (a.B <= 4 || fours.us < one.us) return launch_w4_group<FMT, 0, 1, 16, MODE>(a, group, fours, s);
     return launch_w4_group<FMT, 3, 1, 16, MODE>(a, group, one, s);
   } else {
-    if (a.B <= 4) return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, w4_plan(a, group, TERMS, 1, 4), s);
-    W4Plan best = w4_plan(a, group, TERMS, 1, 16);
-    int mb = 1;
-    for (int m = 2; 8 * m < a.B && m <= 4; m *= 2) {
+    W4Plan best = w4_plan(a, group, TERMS, 1, 4);
+    int mb = 0;
+    for (int m = 1; a.B > (m == 1 ? 4 : 8 * m) && m <= 4; m *= 2) {  // more than 4, 16, 32 rows
       const W4Plan p = w4_plan(a, group, TERMS, m, 16);
       if (p.us < best.us) {
         best = p;
@@ -658,7 +729,8 @@ static int w4_pass(const W4Args& a, int group, hipStream_t s) {
     }
     if (mb == 4) return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, best, s);
     if (mb == 2) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, best, s);
-    return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, best, s);
+    if (mb == 1) return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, best, s);
+    return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, best, s);
   }
 }
 
