@@ -295,8 +295,8 @@ int nvjsel_lm_head_w4_logits(const void* hidden, int hidden_dtype, const void* p
  * Beam search's selection (no counterpart in the reference).  Request b's
  * candidates are
  *   scores[b,w] + log_softmax(logits[b,w,:])[v]   for every beam w and token v;
- * the k best of them, by value descending and, among equal values, by w * vocab + v
- * ascending, give out_scores f32 [batch, k], out_parents int32 (w) and out_tokens
+ * the k best of them, by value descending and, among equal values, by w ascending,
+ * then the larger logit, then v ascending, give out_scores f32 [batch, k], out_parents int32 (w) and out_tokens
  * int32 (v).  logits [batch, beams, vocab] of dtype, batch_stride and
  * beam_stride elements apart; scores f32 [batch, beams].  1 <= beams, k <= 64,
  * vocab <= 2^26, batch <= 65536.
@@ -328,8 +328,9 @@ int nvjsel_beam_select(const void* logits, int dtype, int batch, int beams, int 
  * stays as it is.  slots (nullable: row b * beams + w) int32 [batch, beams], the
  * slots of a call distinct; parents rows are parent_stride apart.  A beam
  * whose parent is itself or outside 0..beams-1, or whose own or parent's slot is
- * outside 0..rows-1, stays as it is.  beams <= 64, batch <= 65535.  The descriptions
- * are read before the call returns.
+ * outside 0..rows-1, stays as it is.  No two tensors share memory.  beams <= 64,
+ * batch <= 65535, rows of at most 64 GB (16 GB above 16 beams).  The descriptions are read
+ * before the call returns.
  */
 typedef struct {
   void* data;

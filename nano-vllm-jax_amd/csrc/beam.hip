@@ -818,6 +818,7 @@ struct ReorderTensor {
   int64_t token;       // bytes of one position, 0 without lengths
   int outer;
   int rows;
+  int chunks;          // blocks of each span
 };
 
 struct ReorderArgs {
@@ -827,7 +828,6 @@ struct ReorderArgs {
   const int32_t* slots;    // [batch, beams] or null
   const int32_t* lengths;  // [batch] or null
   int beams;
-  int chunks;  // per outer index, of the largest tensor
 };
 
 // state[slot(b, w)] = old state[slot(b, parent(b, w))] in place.  A thread owns the
@@ -842,14 +842,14 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   typedef typename std::conditional<VEC == 16, bm_u32x4_any, bm_u32_any>::type Any;
   const ReorderTensor& t = a.t[blockIdx.z];
   const int req = (int)blockIdx.y, W = a.beams;
-  const int o = (int)blockIdx.x / a.chunks;
+  const int o = (int)blockIdx.x / t.chunks;
   if (o >= t.outer) return;
   int64_t valid = t.span;
   if (t.token) {
     const int64_t n = (int64_t)a.lengths[req] * t.token;
     valid = n < valid ? n : valid;
   }
-  const int64_t at = ((int64_t)((int)blockIdx.x % a.chunks) * 256 + threadIdx.x) * VEC;
+  const int64_t at = ((int64_t)((int)blockIdx.x - o * t.chunks) * 256 + threadIdx.x) * VEC;
   if (at >= valid) return;
   char* base = t.data + (int64_t)o * t.span + at;
 
@@ -998,8 +998,7 @@ extern "C" int nvjsel_reorder_states(const nvjsel_state* states, int count, cons
   for (int i0 = 0; i0 < count; i0 += kReorderTensors) {
     const int n = count - i0 < kReorderTensors ? count - i0 : kReorderTensors;
     ReorderArgs a{};
-    int64_t chunks = 1;
-    int outer = 1;
+    int64_t blocks = 1;
     for (int i = 0; i < n; ++i) {
       const nvjsel_state& t = states[i0 + i];
       ReorderTensor& r = a.t[i];
@@ -1010,21 +1009,20 @@ extern "C" int nvjsel_reorder_states(const nvjsel_state* states, int count, cons
       r.outer = lengths ? t.outer : 1;
       r.span = t.length * t.token_bytes * (lengths ? 1 : t.outer);
       const int64_t c = (r.span + 256 * vec - 1) / (256 * vec);
-      if (c > chunks) chunks = c;
-      if (r.outer > outer) outer = r.outer;
+      if (c * (__int128)r.outer > 0xFFFFFF) return fail(NVJSEL_EINVAL, "reorder_states: state too large");  // 2^32 threads
+      r.chunks = (int)c;
+      if (c * r.outer > blocks) blocks = c * r.outer;
     }
-    if (chunks * outer > 0x7FFFFFFF) return fail(NVJSEL_EINVAL, "reorder_states: state too large");
     a.parents = parents;
     a.parent_stride = parent_stride;
     a.slots = slots;
     a.lengths = lengths;
     a.beams = beams;
-    a.chunks = (int)chunks;
     hipStream_t s = (hipStream_t)stream;
-    const int rc = beams <= 4    ? launch_reorder<16, 4>(a, n, batch, chunks * outer, s)
-                   : beams <= 8  ? launch_reorder<16, 8>(a, n, batch, chunks * outer, s)
-                   : beams <= 16 ? launch_reorder<16, 16>(a, n, batch, chunks * outer, s)
-                                 : launch_reorder<4, 64>(a, n, batch, chunks * outer, s);
+    const int rc = beams <= 4    ? launch_reorder<16, 4>(a, n, batch, blocks, s)
+                   : beams <= 8  ? launch_reorder<16, 8>(a, n, batch, blocks, s)
+                   : beams <= 16 ? launch_reorder<16, 16>(a, n, batch, blocks, s)
+                                 : launch_reorder<4, 64>(a, n, batch, blocks, s);
     if (rc != NVJSEL_OK) return rc;
   }
   return NVJSEL_OK;

@@ -9,6 +9,7 @@ non-native path.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -55,11 +56,12 @@ SIGNATURES = {
 }
 
 
-class State(ctypes.Structure):
-    """nvjsel_state: one tensor of nvjsel_reorder_states."""
+_STATE = "Pqqqii"  # nvjsel_state: data, row_bytes, length, token_bytes, outer, rows
 
-    _fields_ = [("data", _vp), ("row_bytes", _i64), ("length", _i64), ("token_bytes", _i64),
-                ("outer", ctypes.c_int32), ("rows", ctypes.c_int32)]
+
+def states(fields: list) -> bytes:
+    """An array of nvjsel_state from all their fields in turn."""
+    return struct.pack(_STATE * (len(fields) // len(_STATE)), *fields)
 
 
 class NvjselError(RuntimeError):

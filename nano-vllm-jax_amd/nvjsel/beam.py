@@ -23,8 +23,8 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     ``scores`` f32 ``[B, W]`` the beams' cumulative log-probabilities.  The
     candidates of request ``b`` are ``scores[b, w] + log_softmax(logits[b, w])[v]``;
     the ``num_candidates`` (default W, at most 64) best ones come back as
-    ``(scores f32[B, K], parents int32[B, K], tokens int32[B, K])``, the best first,
-    equal ones by ``w * V + v`` ascending.
+    ``(scores f32[B, K], parents int32[B, K], tokens int32[B, K])``, the best first, equal
+    ones by beam; within a beam the larger logit first, equal ones by token.
 
     A beam whose score is ``-inf`` is not live (the first step has one live beam): it
     has no candidates and its logits are not looked at.  A beam with ``finished`` set (bool
@@ -74,13 +74,34 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     return out_scores, parents, tokens
 
 
+def _describe_state(t: torch.Tensor, rows: int | None, length_dim: int | None) -> tuple:
+    """A nvjsel_state without its pointer."""
+    shape = t.shape
+    if t.ndim == 0 or (rows is not None and shape[0] < rows):
+        raise ValueError("a state needs one row per beam along its first dimension")
+    n = t.numel()
+    if n == 0:
+        raise ValueError("states must not be empty")
+    row = n // shape[0]
+    if not t.is_contiguous() and (not t[0].is_contiguous() or (shape[0] > 1 and t.stride(0) < row)):
+        raise ValueError("a state's rows must be contiguous and must not overlap")
+    size = t.element_size()
+    outer, length = 1, 1
+    if length_dim is not None:
+        at = length_dim + t.ndim if length_dim < 0 else length_dim
+        if not 1 <= at < t.ndim:
+            raise ValueError(f"length_dim {length_dim} is not a dimension of a row of {tuple(shape)}")
+        outer, length = math.prod(shape[1:at]), shape[at]
+    return (t.stride(0) if shape[0] > 1 else row) * size, length, row // (outer * length) * size, outer, shape[0]
+
+
 def reorder_beam_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None = None,
                         lengths: torch.Tensor | None = None, length_dim: int | None = None) -> None:
     """Give every beam its parent's state, in place, in one launch per 24 tensors.
 
     ``states``: a tensor or a sequence of tensors (caches, recurrent states, token
     histories; any types), one row per beam along the first dimension, each row
-    contiguous.  Row ``b * W + w``, or ``slots[b, w]`` (int32 ``[B, W]``, distinct) of a
+    contiguous, no two of them sharing memory.  Row ``b * W + w``, or ``slots[b, w]`` (int32 ``[B, W]``, distinct) of a
     state table, receives what the row of beam ``parents[b, w]`` held.  With ``lengths``
     (int32 ``[B]``) only the first ``lengths[b]`` positions along ``length_dim`` move and
     the rest stays as it is.  ``parents`` is int32 ``[B, W]``, e.g. the first W columns of
@@ -110,28 +131,17 @@ def reorder_beam_states(states, parents: torch.Tensor, *, slots: torch.Tensor | 
     if not 1 <= count <= _MAX_STATES:
         raise ValueError(f"reorder_beam_states takes 1..{_MAX_STATES} states")
     dev = _require_cuda(parents, slots, lengths, *states)
-    table = (_lib.State * count)()
-    for t, d in zip(states, table):
-        shape = t.shape
-        if t.ndim == 0 or (slots is None and shape[0] < batch * beams):
-            raise ValueError("a state needs one row per beam along its first dimension")
-        n = t.numel()
-        if n == 0:
-            raise ValueError("states must not be empty")
-        row = n // shape[0]
-        if not t.is_contiguous() and (not t[0].is_contiguous() or (shape[0] > 1 and t.stride(0) < row)):
-            raise ValueError("a state's rows must be contiguous and must not overlap")
-        size = t.element_size()
-        outer, length = 1, 1
-        if lengths is not None:
-            at = length_dim + t.ndim if length_dim < 0 else length_dim
-            if not 1 <= at < t.ndim:
-                raise ValueError(f"length_dim {length_dim} is not a dimension of a row of {tuple(shape)}")
-            outer, length = math.prod(shape[1:at]), shape[at]
-        d.data, d.row_bytes, d.length = t.data_ptr(), (t.stride(0) if shape[0] > 1 else row) * size, length
-        d.token_bytes, d.outer, d.rows = row // (outer * length) * size, outer, shape[0]
+    table, last = [], None
+    for t in states:
+        form = (t.shape, t.stride(), t.dtype)
+        if form != last:  # the layers of a cache are alike
+            described, last = _describe_state(t, None if slots is not None else batch * beams, length_dim), form
+        table.append(t.data_ptr())
+        table += described
+    if len(set(table[::6])) != count:
+        raise ValueError("a state is given twice")
     with _on_device(dev):
-        _lib.call("nvjsel_reorder_states", table, count, parents.data_ptr(), parents.stride(0),
+        _lib.call("nvjsel_reorder_states", _lib.states(table), count, parents.data_ptr(), parents.stride(0),
                   None if slots is None else slots.data_ptr(), None if lengths is None else lengths.data_ptr(), batch,
                   beams, _stream_handle(dev))
 

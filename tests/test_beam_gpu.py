@@ -281,6 +281,19 @@ def test_reorder(b, w, row, dtype):
     assert torch.equal(got.cpu(), want[0])
 
 
+def test_reorder_long_and_many_pieces_together():
+    """One state in a few long pieces beside one in many short ones."""
+    lengths = torch.tensor([5, 70001], dtype=torch.int32)
+    parents = torch.tensor([[1, 0, 0], [2, 2, 1]], dtype=torch.int32)
+    states = [state((6, 1, 70001), torch.float32, 1), state((6, 3001, 9), torch.float16, 2), state((7, 2, 40), torch.uint8, 3)]
+    got = [s.cuda() for s in states]
+    nvjsel.reorder_beam_states(got, parents.cuda(), lengths=lengths.cuda(), length_dim=2)
+    for a, b in zip(got, moved(states, parents, None, lengths, 2)):
+        assert torch.equal(a.cpu(), b)
+    with pytest.raises(ValueError, match="twice"):
+        nvjsel.reorder_beam_states([got[0], got[1], got[0]], parents.cuda())
+
+
 @pytest.mark.parametrize("w", [3, 16, 30])
 def test_reorder_cycles_and_copies(w):
     """Every beam from the next one, all from one, and pairs that change places."""

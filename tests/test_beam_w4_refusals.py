@@ -165,10 +165,11 @@ def test_c_entries():
         assert select(**kw) == code, kw
 
     def reorder(count=1, parents=DUMMY, stride=4, batch=2, beams=4, slots=None, **kw):
-        t = _lib.State(**{"data": DUMMY, "row_bytes": 64, "length": 4, "token_bytes": 8, "outer": 2, "rows": 8, **kw})
-        return lib.nvjsel_reorder_states((_lib.State * 1)(t), count, parents, stride, slots, None, batch, beams, None)
+        t = {"data": DUMMY, "row_bytes": 64, "length": 4, "token_bytes": 8, "outer": 2, "rows": 8, **kw}
+        table = _lib.states([x or 0 for x in t.values()])
+        return lib.nvjsel_reorder_states(table, count, parents, stride, slots, None, batch, beams, None)
 
     for kw in ({"count": 0}, {"parents": None}, {"stride": -1}, {"batch": 0}, {"batch": 65536}, {"beams": 65},
                {"data": None}, {"row_bytes": 63}, {"length": 0}, {"outer": 0}, {"token_bytes": 0}, {"rows": 7},
-               {"length": 1 << 62}):
+               {"length": 1 << 62}, {"length": 1 << 36, "row_bytes": 1 << 40}):  # more than 64 GB a row
         assert reorder(**kw) == -1, kw
