@@ -7,6 +7,7 @@ of 2^-24 are independent: 16 of them, and a few for the exponentials).  Two
 candidates of one beam keep their logits' order exactly; two beams' candidates
 may change places where they are closer than the two sums' errors."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -404,3 +405,62 @@ def test_step(packed):
             finished[0, 1] = True  # an end by length
         d_finished, d_scores = finished.cuda(), new
         assert torch.equal(d_cache.cpu(), cache) and torch.equal(d_tokens.cpu(), tokens)
+
+
+def test_captured_step():
+    """A whole step as a graph, replayed with new inputs and eager calls between."""
+    g = torch.Generator().manual_seed(5)
+    b, w, h, v = 3, 4, 256, 5003
+    weight = (torch.randn(v, h, generator=g) * 0.05).to(torch.bfloat16).cuda()
+    head = nvjsel.pack_lm_head_w4(*nvjsel.quantize_lm_head_w4(weight.T))
+    inputs = [(torch.randn(b, w, h, generator=g).to(torch.bfloat16).cuda(), torch.randn(b, w, generator=g).cuda(),
+               torch.randn(b * w, 6, 33, generator=g).cuda()) for _ in range(3)]
+
+    def step(hidden, scores, cache):
+        return nvjsel.lm_head_beam_search_step(hidden, head, scores, states=[cache])
+
+    want = []
+    for hidden, scores, cache in inputs:
+        moved_cache = cache.clone()
+        want.append((*(x.clone() for x in step(hidden, scores, moved_cache)), moved_cache))
+    fixed = tuple(x.clone() for x in inputs[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*fixed)
+    for rep in range(5):
+        for to, x in zip(fixed, inputs[rep % 3]):
+            to.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip((*out, fixed[2]), want[rep % 3]):
+            assert torch.equal(x, y)
+        assert torch.equal(step(*(x.clone() for x in inputs[1]))[2], want[1][2])
+
+
+def test_threads_share_a_stream():
+    """Two threads on one stream: selections in one launch and in two, and ids beside them."""
+    small, large = [make(2, 4, 9001, "bf16", 60)], [make(24, 8, 20011, "f16", 61)]
+    data = [(l.cuda(), s.cuda()) for l, s in small + large]
+    want = [nvjsel.beam_search_select(l, s, num_candidates=8) for l, s in data]
+    weight = (torch.randn(3001, 128, generator=torch.Generator().manual_seed(1)) * 0.1).to(torch.bfloat16).cuda()
+    head = nvjsel.pack_lm_head_w4(*nvjsel.quantize_lm_head_w4(weight.T))
+    x = torch.randn(5, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    ids = nvjsel.lm_head_greedy_top1_hip(x, head)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(first):
+        for i in range(40):
+            at = (first + i) % 2
+            got = nvjsel.beam_search_select(*data[at], num_candidates=8)
+            same = torch.equal(nvjsel.lm_head_greedy_top1_hip(x, head), ids)
+            if not same or not all(torch.equal(a, b) for a, b in zip(got, want[at])):
+                wrong.append((first, i))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
