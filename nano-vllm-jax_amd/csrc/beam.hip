@@ -40,6 +40,7 @@ static constexpr int kBeamJoinThreads = 512;             // of the second kernel
 static constexpr int kBeamOneMax = 24;     // candidates that one maximum per lane bounds well enough, two above
 static constexpr int kBeamClasses = 128;   // of parts or candidates, two per lane, for the join's bounds
 static constexpr int kBeamFewShares = 4;   // of a row, whose sums a lane joins, not a wave (64 beams of one share: 14 us by waves, 1.2 so)
+static constexpr int kBeamEarly = 1024;    // candidates that one launch's join loads with the parts
 static constexpr int kBeamRefine = 128;    // candidates that are ranked without a second bound
 
 struct BeamPart {  // of one wave's share of a row
@@ -362,7 +363,7 @@ __device__ __forceinline__ void beam_scan(const BeamArgs& a, BeamScanLds& lds, i
     total = wave_sum_f64(beam_sum_far<DT>(base, e0, e1, wm, lane));
   }
 
-  find_bound();
+  if (taken & (taken - 1)) find_bound();  // else it is of all chunks already
   uint2* cand = a.cand + (size_t)wid * a.cap;
   int count = 0;
   auto collect = [&](const bm_u32x4& w, int o) NVJSEL_INLINE {  // the candidates of a piece per lane
@@ -497,6 +498,7 @@ struct BeamJoinLds {
   int state[kBeamMax];
   float rmax[kBeamMax];
   uint32_t best_of[kBeamClasses];  // of the parts' classes: the scores' first 32 bits in order
+  uint2 early[LISTS == kBeamFew ? kBeamEarly : 1];  // every part's first candidates
   int start[LISTS];                // of the parts that reach the bound: the number of their first candidate
   uint16_t list[LISTS];
   int found;
@@ -524,12 +526,29 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     found = 0;
     taken = 0;
   }
+  // One launch: the parts' first candidates on their way with the parts, whatever of them
+  // are there, so that the ones that reach the bound need no round trip of their own
+  int firsts = 0;
+  uint2 e[ONE ? kBeamEarly / THREADS : 1];
+  if constexpr (ONE) {
+    firsts = min(kBeamEarly / lists, a.cap);
+#pragma unroll
+    for (int u = 0; u < kBeamEarly / THREADS; ++u) {
+      const int i = min(tid + u * THREADS, lists * firsts - 1);
+      e[u] = beam_get<ONE>(a.cand + ((size_t)req * lists + i / firsts) * a.cap + i % firsts);
+    }
+  }
   for (int l = tid; l < lists; l += THREADS) {
     const BeamPart* p = a.parts + (size_t)req * lists + l;
     const uint2 u = beam_get<ONE>(&p->sum), v = beam_get<ONE>(&p->max);
     part[l].sum = two_words(u.x, u.y);
     part[l].max = __uint_as_float(v.x);
     part[l].count = (int)v.y;
+  }
+  if constexpr (ONE) {
+#pragma unroll
+    for (int u = 0; u < kBeamEarly / THREADS; ++u)
+      if (tid + u * THREADS < lists * firsts) lds.early[tid + u * THREADS] = e[u];
   }
   if (tid < W) {
     const float sc = a.scores[(size_t)req * W + tid];
@@ -602,14 +621,14 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     }
   __syncthreads();
   const int nl = (int)(uint32_t)taken, nc = (int)(taken >> 32);
-  auto gather = [&](bool all) NVJSEL_INLINE {  // or until there are too many to rank
-    constexpr int AHEAD = 4;  // loads of a thread on their way together
-    for (int i0 = tid; i0 < nc; i0 += AHEAD * THREADS) {
+  auto gather_by = [&](auto AHEAD, bool all) NVJSEL_INLINE {  // loads of a thread on their way together
+    constexpr int N = decltype(AHEAD)::value;
+    for (int i0 = tid; i0 < nc; i0 += N * THREADS) {
       if (!all && *(volatile int*)&found > RANKED) break;
-      int of[AHEAD];
-      uint2 e[AHEAD];
+      int of[N];
+      uint2 c[N];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
+      for (int u = 0; u < N; ++u) {
         const int i = min(i0 + u * THREADS, nc - 1);
         int lo = 0, hi = nl;  // the last list that starts at or before i
         while (hi - lo > 1) {
@@ -618,12 +637,18 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
           else hi = mid;
         }
         of[u] = list[lo];
-        e[u] = beam_get<ONE>(a.cand + ((size_t)req * lists + of[u]) * a.cap + (i - start[lo]));
+        const int j = i - start[lo];
+        if (N == 1 && ONE && j < firsts) c[u] = lds.early[of[u] * firsts + j];
+        else c[u] = beam_get<ONE>(a.cand + ((size_t)req * lists + of[u]) * a.cap + j);
       }
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (i0 + u * THREADS < nc) add(scored(of[u], e[u]));
+      for (int u = 0; u < N; ++u)
+        if (i0 + u * THREADS < nc) add(scored(of[u], c[u]));
     }
+  };
+  auto gather = [&](bool all) NVJSEL_INLINE {  // or until there are too many to rank
+    if (nc > 2 * THREADS) gather_by(std::integral_constant<int, 4>{}, all);
+    else gather_by(std::integral_constant<int, 1>{}, all);
     if (tid < W && state[tid] == BEAM_ENDED) add(BeamKey{rscore[tid], beam_at(tid, 0.0f, (uint32_t)a.end_token)});
     __syncthreads();
   };

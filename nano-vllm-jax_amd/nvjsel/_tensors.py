@@ -21,12 +21,12 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
 
 def _require_cuda(*ts: torch.Tensor) -> torch.device:
     dev = ts[0].device
+    if dev.type != "cuda":
+        raise ValueError("nvjsel kernels take device tensors (got a CPU tensor)")
     for t in ts:
-        if t is None:
-            continue
-        if t.device.type != "cuda":
-            raise ValueError("nvjsel kernels take device tensors (got a CPU tensor)")
-        if t.device != dev:
+        if t is not None and t.device != dev:
+            if t.device.type != "cuda":
+                raise ValueError("nvjsel kernels take device tensors (got a CPU tensor)")
             raise ValueError("all tensors must live on one device")
     return dev
 
@@ -54,6 +54,9 @@ class _WorkspacePool:
 
     def get(self, device: torch.device, stream: int, kind: str, nbytes: int) -> torch.Tensor:
         key = (device.index, stream, kind)
+        buf = self._bufs.get(key)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
         with self._lock:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
@@ -66,8 +69,9 @@ _WS = _WorkspacePool()
 
 
 _HERE = nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _on_device(device: torch.device):
     """Makes ``device`` the current one for a launch, where it is not already."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)

@@ -3,6 +3,7 @@ states, and the decode step that joins them with the LM head."""
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 
@@ -13,6 +14,11 @@ from .selection import lm_head_logits_hip, rms_norm_hip
 MAX_BEAMS = 64  # beams and candidates of a request
 MAX_REQUESTS, MAX_VOCAB = 65536, 1 << 26  # of a selection
 _MAX_STATES = 4096  # descriptions of one call
+
+
+@lru_cache(maxsize=1024)
+def _select_bytes(device: int, *shape: int) -> int:  # by device: its compute units count
+    return _lib.load().nvjsel_beam_select_workspace_size(*shape)
 
 
 def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: int | None = None,
@@ -58,7 +64,7 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     out, parents, tokens = scores.new_empty((3, batch, k), dtype=torch.int32).unbind(0)
     out_scores = out.view(torch.float32)
     with _on_device(dev):
-        nbytes = _lib.load().nvjsel_beam_select_workspace_size(dt, batch, beams, vocab, k)
+        nbytes = _select_bytes(dev.index, dt, batch, beams, vocab, k)
         stream = _stream_handle(dev)
         if torch.cuda.is_current_stream_capturing():
             # a graph keeps a workspace of its own: graphs captured on one stream may be
