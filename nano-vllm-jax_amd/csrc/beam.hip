@@ -32,9 +32,10 @@ static constexpr int kBeamSlots = 8;       // lanes' maxima kept of a share, eac
 static constexpr int kBeamHeld = 64;       // pieces of a lane and chunk that a wave can set aside
 static constexpr int kBeamThreads = 256, kBeamBlockWaves = kBeamThreads / 64;
 // One launch scans and joins calls of up to kBeamOne parts, kBeamFew a request.  What
-// passes between its blocks goes by the device's coherence point: 64 / 392 / 512 / 1008 /
-// 2048 parts take 10.0 / 10.6 / 10.9 / 12.4 / 15.7 us so and 10.5 / 10.4 / 11.0 / 10.7 / 11.1
-// in two kernels, which cost the host 3 us more.  And the parts of a request at most.
+// passes between its blocks goes by the device's coherence point: calls of 64 / 400 / 512 /
+// 625 / 1024 / 2048 parts take 9.9 / 11.6 / 11.0 / 12.2 / 12.7 / 18.5 us so and 12.4 / 12.1 /
+// 12.3 / 11.6 / 11.5 / 12.7 in two kernels, one after the other from Python.  And the
+// parts of a request at most.
 static constexpr int kBeamOne = 512, kBeamFew = 256, kBeamLists = 2048;
 static constexpr int kBeamJoinThreads = 512;             // of the second kernel
 static constexpr int kBeamOneMax = 24;     // candidates that one maximum per lane bounds well enough, two above
@@ -248,6 +249,9 @@ __device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int 
 // the last bound are the candidates.  Where more are set aside than there is room
 // for, the pieces are read again instead, by the lanes' maxima of every chunk in LDS
 // (V = 248,320, 256 rows, K = 16: 29 us so, 27 out of LDS).
+//
+// Bound: vector instructions (an exponential and a maximum per logit) at 70% of the
+// streaming rate: 256 rows of 248,320 bf16 logits, 127 MB, take 25 us, 5.1 TB/s.
 struct BeamScanLds {
   float lane_max[kBeamBlockWaves][kBeamSlots][64];
   bm_u32x4 aside[kBeamBlockWaves][kBeamHeld][kBeamVecs];  // or, read again: the (slot, lane) pairs
@@ -488,6 +492,9 @@ __device__ __forceinline__ uint64_t beam_ord(double x) {
 // candidates that reach it, seldom more than twice K, are ranked by counting, each
 // against all; where there are more than there is room for (many equal scores), every
 // wave keeps the best 64 of its share of them sorted and the waves' lists are merged.
+// Bound: the chain of memory round trips (parts, candidates) and barriers, 6-7 us
+// whatever the size (8 requests of 4 beams, 488 parts each: normalisers 2.0 us, bounds 1.6,
+// candidates 1.0, ranks 0.7).
 template <int LISTS>
 struct BeamJoinLds {
   static constexpr int RANKED = LISTS == kBeamFew ? 512 : 1024;
@@ -860,7 +867,10 @@ struct ReorderArgs {
 // then stores them, so no order of the moves matters and nothing waits for
 // another thread.  Beams that keep their place are not touched.  Memory bound:
 // each moved beam is written once; a source that several beams take comes from
-// the cache after its first read.
+// the cache after its first read.  The loads of W beams are in flight together, 16
+// bytes a lane up to 16 beams and 4 above, so that they fit the registers.  12 bf16 states
+// of 64 rows x 1 MB with ragged lengths, 535 MB read and written: 111 us, 4.8 TB/s; whole
+// f32 rows, 1.07 GB: 202 us, 5.3 TB/s; a large copy runs at 5.1.
 template <int VEC, int WREG>
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   typedef typename std::conditional<VEC == 16, bm_u32x4, uint32_t>::type Vec;
