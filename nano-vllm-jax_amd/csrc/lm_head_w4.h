@@ -269,7 +269,7 @@ struct W4Stage {
 // (DEPTH); the waves share the hidden in LDS, all of it where it fits, kc k blocks in
 // a ring where not (STAGED).  Matrix tile: M = batch rows (MB tiles of 16), N =
 // vocabulary rows, so that a lane's results share their scale.  RT: batch rows that
-// have slots in LDS (4: the others repeat them).
+// have slots in LDS (8: the others repeat them).
 //
 // Rows go round all waves of the device while every wave gets some; what is left is
 // dealt to the blocks, and a block splits its rest by k blocks over its waves, which
@@ -668,13 +668,13 @@ static inline W4Plan w4_plan(const W4Args& a, int group, int terms, int mb, int 
     float call, stage, round, staged;
   };
   static constexpr Fit fits[6] = {
-      {6.5f, 0.03f, 0.45f, 1.00f},   // four rows
+      {6.4f, 0.06f, 0.48f, 1.00f},   // eight rows
       {6.4f, 0.10f, 0.53f, 0.98f},   // one tile of 16
       {7.4f, 0.22f, 0.70f, 1.42f},   // two
       {9.6f, 0.55f, 1.21f, 2.20f},   // four
       {6.6f, 0.09f, 0.50f, 1.20f},   // four rows of three terms
       {6.5f, 0.34f, 0.85f, 1.90f}};  // one tile, three terms apart
-  const Fit& f = fits[terms == 3 ? 5 : terms == 0 ? 4 : rt == 4 ? 0 : mb == 4 ? 3 : mb];
+  const Fit& f = fits[terms == 3 ? 5 : terms == 0 ? 4 : rt == 8 ? 0 : mb == 4 ? 3 : mb];
   const int slots = p.blocks * kW4Waves;
   const float each = p.staged ? f.staged * ((waves + slots - 1) / slots)
                               : f.stage + f.round * fmaxf((float)waves / slots, 1.0f / kW4Waves);
@@ -708,7 +708,8 @@ static int launch_w4_group(const W4Args& a, int group, const W4Plan& p, hipStrea
 }
 
 // The widest tile reads and unpacks the weights the fewest times; narrower ones leave more
-// of the hidden in LDS (64 rows, V = 32,000, H = 4096: 38 us with 16 rows a tile, 76 with
+// of the hidden in LDS, and stage it sooner (up to 8 rows of H = 8192, V = 50,000: 43 us with
+// 8 rows' slots, 65 with 16; 64 rows, V = 32,000, H = 4096: 38 us with 16 rows a tile, 76 with
 // 64, staged) and give a small vocabulary's tiles to more blocks (32 rows, V = 8000, H = 1024: 5.7 us
 // with 16 rows, 7.5 with 32), but a large one costs more with them (64 rows, V = 248,320, H =
 // 1024: 70 us with 16, 49 with 64).  f32: the terms apart where the hidden stays in LDS so
@@ -721,9 +722,9 @@ static int w4_pass(const W4Args& a, int group, hipStream_t s) {
     if (a.B <= 4 || fours.us < one.us) return launch_w4_group<FMT, 0, 1, 16, MODE>(a, group, fours, s);
     return launch_w4_group<FMT, 3, 1, 16, MODE>(a, group, one, s);
   } else {
-    W4Plan best = w4_plan(a, group, TERMS, 1, 4);
+    W4Plan best = w4_plan(a, group, TERMS, 1, 8);
     int mb = 0;
-    for (int m = 1; a.B > (m == 1 ? 4 : 8 * m) && m <= 4; m *= 2) {  // more than 4, 16, 32 rows
+    for (int m = 1; a.B > 8 * m && m <= 4; m *= 2) {
       const W4Plan p = w4_plan(a, group, TERMS, m, 16);
       if (p.us < best.us) {
         best = p;
@@ -733,7 +734,7 @@ static int w4_pass(const W4Args& a, int group, hipStream_t s) {
     if (mb == 4) return launch_w4_group<FMT, TERMS, 4, 16, MODE>(a, group, best, s);
     if (mb == 2) return launch_w4_group<FMT, TERMS, 2, 16, MODE>(a, group, best, s);
     if (mb == 1) return launch_w4_group<FMT, TERMS, 1, 16, MODE>(a, group, best, s);
-    return launch_w4_group<FMT, TERMS, 1, 4, MODE>(a, group, best, s);
+    return launch_w4_group<FMT, TERMS, 1, 8, MODE>(a, group, best, s);
   }
 }
 

@@ -125,10 +125,10 @@ def test_f32_terms_do_not_round_each_other(rows, vocab, zeros):
     (64, 70000, 8192, 128, "bf16", False),  # in parts
     (32, 66000, 5120, 64, "bf16", True),    # one tile of 32, in parts
     (16, 40000, 8192, 32, "f16", True),     # one of 16, in parts
-    (4, 3001, 20480, 32, "bf16", True),     # rows in fours, in parts
+    (4, 3001, 20480, 32, "bf16", True),     # rows in eights, in parts
     (4, 3001, 5120, 64, "f32", True),
     (7, 3001, 5120, 32, "f32", False),
-    (9, 2000, 1024, 128, "f16", False),     # three groups of four
+    (9, 2000, 1024, 128, "f16", False),     # two groups of eight
 ])
 def test_tile_shapes(rows, vocab, hidden, group, act, zeros):
     """Sizes at which each shape of tiles is taken; a sample of the vocabulary is compared."""
