@@ -250,8 +250,10 @@ __device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int 
 // for, the pieces are read again instead, by the lanes' maxima of every chunk in LDS
 // (V = 248,320, 256 rows, K = 16: 29 us so, 27 out of LDS).
 //
-// Bound: vector instructions (an exponential and a maximum per logit) at 70% of the
-// streaming rate: 256 rows of 248,320 bf16 logits, 127 MB, take 25 us, 5.1 TB/s.
+// Bound: the stream, and in part beside it an exponential and a maximum per logit and
+// the pieces set aside: 256 rows of 248,320 bf16 logits (127 MB) take 25 us, 5.1 TB/s, 20 with sums of
+// the logits themselves, 18 with nothing set aside either.  The bound by halving between the least and
+// the greatest lane instead of bit by bit took 2 us more.
 struct BeamScanLds {
   float lane_max[kBeamBlockWaves][kBeamSlots][64];
   bm_u32x4 aside[kBeamBlockWaves][kBeamHeld][kBeamVecs];  // or, read again: the (slot, lane) pairs
