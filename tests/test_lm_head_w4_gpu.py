@@ -129,6 +129,9 @@ def test_f32_terms_do_not_round_each_other(rows, vocab, zeros):
     (4, 3001, 5120, 64, "f32", True),
     (7, 3001, 5120, 32, "f32", False),
     (9, 2000, 1024, 128, "f16", False),     # two groups of eight
+    (256, 9000, 1024, 64, "bf16", True),    # sixteen groups
+    (200, 40000, 2048, 128, "f16", False),
+    (300, 2000, 640, 128, "f32", False),    # several launches
 ])
 def test_tile_shapes(rows, vocab, hidden, group, act, zeros):
     """Sizes at which each shape of tiles is taken; a sample of the vocabulary is compared."""
