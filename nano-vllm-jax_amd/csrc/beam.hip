@@ -29,7 +29,9 @@ static constexpr int kBeamRequests = 65536;  // of a call: a workspace's tickets
 static constexpr int kBeamVecs = 4;        // 16-byte pieces per lane and chunk
 static constexpr int kBeamWaves = 16;      // per CU that a call is split into
 static constexpr int kBeamSlots = 8;       // lanes' maxima kept of a share, each over as many chunks as it takes
-static constexpr int kBeamHeld = 64;       // pieces of a lane and chunk that a wave can set aside
+// Pieces of a lane and chunk that a wave can set aside: 50 expected over 8 chunks at K = 16,
+// 90 at 32 (256 rows of 248,320, K = 32: 42.8 us with 64, read again, 39.1 so); four blocks fit a CU.
+static constexpr int kBeamHeld = 112;
 static constexpr int kBeamThreads = 256, kBeamBlockWaves = kBeamThreads / 64;
 // One launch scans and joins calls of up to kBeamOne parts, kBeamFew a request.  What
 // passes between its blocks goes by the device's coherence point: calls of 64 / 400 / 512 /
@@ -248,7 +250,7 @@ __device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int 
 // sets the chunk's pieces aside in LDS; at the end the logits among them that reach
 // the last bound are the candidates.  Where more are set aside than there is room
 // for, the pieces are read again instead, by the lanes' maxima of every chunk in LDS
-// (V = 248,320, 256 rows, K = 16: 29 us so, 27 out of LDS).
+// (V = 248,320, 256 rows, K = 16: 2 us more).
 //
 // Bound: the stream, and in part beside it an exponential and a maximum per logit and
 // the pieces set aside: 256 rows of 248,320 bf16 logits (127 MB) take 25 us, 5.1 TB/s, 20 with sums of
