@@ -28,7 +28,7 @@
 // the 16x16x32 product and 33 for the 32x32x16 one, so the smaller tile costs
 // half where up to 16 batch rows are there and nothing where there are more.  V =
 // 248,320, H = 1024, groups of 128: one row 26.6 us (131 MB, 4.9 TB/s), 16 rows 26.4; V = 151,936, H =
-// 2560, groups of 64 with zero points, 8 f16 rows 42.6 us (5.0 TB/s); V = 128,256, H = 2048, 64
+// 2560, groups of 64 with zero points, 8 f16 rows 40.3 us (5.3 TB/s); V = 128,256, H = 2048, 64
 // rows 51 us (660 TFLOP/s).
 #pragma once
 #include "lm_head_common.h"
