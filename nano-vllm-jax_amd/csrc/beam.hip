@@ -554,7 +554,7 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     const uint2 u = beam_get<ONE>(&p->sum), v = beam_get<ONE>(&p->max);
     part[l].sum = two_words(u.x, u.y);
     part[l].max = __uint_as_float(v.x);
-    part[l].count = (int)v.y;
+    part[l].count = (int)min(v.y, (uint32_t)a.cap);  // whatever is there, no candidate is read outside the workspace
   }
   if constexpr (ONE) {
 #pragma unroll
@@ -822,19 +822,19 @@ static size_t beam_bytes(int batch, int beams, int shares, int cap) {
   return kBeamRequests * 4 + (size_t)batch * beams * shares * (sizeof(BeamPart) + cap * sizeof(uint2));
 }
 
-// The two launches of a call stay together on their stream: calls of several threads on
-// one stream may share a workspace.
+// Calls of several threads on one stream may share a workspace: no other call's launch,
+// of one kernel or of two, comes between a call's scan and the join that reads what it wrote.
 static std::mutex g_beam_mu;
 
 template <int DT>
 static int launch_beam(const BeamArgs& a, hipStream_t s) {
   const int64_t waves = (int64_t)a.batch * a.beams * a.shares;
+  std::lock_guard<std::mutex> lock(g_beam_mu);
   if (waves <= kBeamOne && a.beams * a.shares <= kBeamFew) {
     hipLaunchKernelGGL(beam_select_kernel<DT>, dim3((unsigned)(a.batch * a.blocks)), dim3(kBeamThreads), 0, s, a);
     NVJSEL_CHECK_LAUNCH("beam_select_kernel");
     return NVJSEL_OK;
   }
-  std::lock_guard<std::mutex> lock(g_beam_mu);
   hipLaunchKernelGGL(beam_scan_kernel<DT>, dim3((unsigned)((waves + kBeamBlockWaves - 1) / kBeamBlockWaves)),
                      dim3(kBeamThreads), 0, s, a);
   NVJSEL_CHECK_LAUNCH("beam_scan_kernel");
