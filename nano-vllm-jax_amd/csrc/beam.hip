@@ -10,7 +10,7 @@
 // ranks them (beam_join).  With few parts a request's last block to finish them joins
 // them in the same launch, with more a second kernel does (kBeamFew). fp64 there because two beams'
 // candidates may lie closer than an fp32 score resolves; the sums of exponentials
-// are fp32 within a lane and fp64 across lanes and parts.
+// are fp32 within a lane's 16 or 32 logits of a chunk and fp64 across chunks, lanes and parts.
 #include <float.h>
 
 #include <mutex>
@@ -156,12 +156,28 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t x, uint32_t y, int k, int 
   return t;
 }
 // Exponentials are the hardware's exp2 (about 1 ulp) of fma(x, log2 e, -ref): one
-// rounding of the difference, and ref, a lane's maximum times log2 e, is a number that
-// the sum is relative to as it was rounded.  That holds for maxima up to this size;
-// the reference stays within it, and a share whose own maximum does not is summed
-// again (beam_sum_far).
+// rounding of the difference.  ref is a whole number next to a lane's maximum times log2 e,
+// so that a sum moves from one reference to another by its exponent alone, exactly, however
+// often its maximum rises.  That holds for maxima up to this size; the reference stays
+// within it, and a share whose own maximum does not is summed again (beam_sum_far).
 static constexpr float kLog2e = 1.44269504088896341f, kBeamFar = 16384.0f;
-__device__ __forceinline__ float beam_ref(float m) { return fminf(fmaxf(m, -kBeamFar), kBeamFar) * kLog2e; }
+__device__ __forceinline__ float beam_ref(float m) { return rintf(fminf(fmaxf(m, -kBeamFar), kBeamFar) * kLog2e); }
+// sum, relative to 2^from, relative to 2^to.
+__device__ __forceinline__ double beam_move(double sum, float from, float to) {
+  return __builtin_amdgcn_ldexp(sum, (int)(from - to));
+}
+// The sum of N numbers, a power of two, in log2 N roundings.
+template <int N>
+__device__ __forceinline__ float sum_tree(const float (&t)[N]) {
+  if constexpr (N == 1) {
+    return t[0];
+  } else {
+    float u[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) u[i] = t[2 * i] + t[2 * i + 1];
+    return sum_tree(u);
+  }
+}
 
 // The piece at element o of a share that ends at e1; -inf past the end.
 template <int DT>
@@ -277,7 +293,8 @@ __device__ __forceinline__ void beam_scan(const BeamArgs& a, BeamScanLds& lds, i
   auto& aside = lds.aside[wave];
   auto& aside_at = lds.aside_at[wave];
 
-  float m = -INFINITY, ref = beam_ref(-INFINITY), sum = 0.0f, kept = -INFINITY;
+  float m = -INFINITY, ref = beam_ref(-INFINITY), kept = -INFINITY;
+  double sum = 0.0;                        // relative to 2^ref
   float half[2] = {-INFINITY, -INFINITY};  // the maximum by pieces: the first and the last ones of every chunk
   float bound = -FLT_MAX;                  // of the candidates: -inf is none
   int taken = 0, held = 0;                 // chunks; pieces set aside
@@ -306,17 +323,20 @@ __device__ __forceinline__ void beam_scan(const BeamArgs& a, BeamScanLds& lds, i
       ++slot;
     }
     const float to = __builtin_elementwise_maximum(m, x), to_ref = beam_ref(to);
-    float s0 = sum * __builtin_amdgcn_exp2f(ref - to_ref), s1 = 0.0f;
+    // a chunk's terms in five roundings at most, from zero: added to the sum of the chunks
+    // before, the small ones of a long share would be lost (one large logit and 122 chunks
+    // of small ones: scores off by 9e-5 so)
+    float s[kBeamVecs];
 #pragma unroll
-    for (int j = 0; j < kBeamVecs; ++j)
+    for (int j = 0; j < kBeamVecs; ++j) {
+      float t[N];
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(E::get(w[j], e), kLog2e, -to_ref));
-        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(E::get(w[j], e + 1), kLog2e, -to_ref));
-      }
+      for (int e = 0; e < N; ++e) t[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(E::get(w[j], e), kLog2e, -to_ref));
+      s[j] = sum_tree(t);
+    }
+    sum = beam_move(sum, ref, to_ref) + (double)sum_tree(s);
     m = to;
     ref = to_ref;
-    sum = s0 + s1;
     if ((taken & (taken + 1)) == 0) find_bound();
     const uint64_t hit = __ballot(x >= bound);
     if (hit) {
@@ -363,10 +383,13 @@ __device__ __forceinline__ void beam_scan(const BeamArgs& a, BeamScanLds& lds, i
   double total;
   if (wm <= kBeamFar && (wm >= 100.0f - kBeamFar || wm == -INFINITY)) {
     const float wref = beam_ref(wm);
-    total = wave_sum_f64((double)(sum * __builtin_amdgcn_exp2f(ref - wref)));  // a NaN's sum is NaN
-    // relative to exp(wm) now: 2^d, |d| < 2^-9 (the roundings of wref), by its series
+    total = wave_sum_f64(beam_move(sum, ref, wref));  // a NaN's sum is NaN
+    // relative to exp(wm) now: exp(d), |d| < 0.35, by its series (to 2^-32)
     const double d = wm == -INFINITY ? 0.0 : ((double)wref - (double)wm * (double)kLog2e) * 0.6931471805599453;
-    total *= 1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6.0)));
+    double f = 1.0;
+#pragma unroll
+    for (int i = 8; i >= 1; --i) f = __builtin_fma(f, d * (1.0 / i), 1.0);
+    total *= f;
   } else {
     total = wave_sum_f64(beam_sum_far<DT>(base, e0, e1, wm, lane));
   }
