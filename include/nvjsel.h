@@ -263,7 +263,8 @@ int nvjsel_derive_keys_table(const int32_t* slots, int batch, int32_t* counter_t
  * uint8 [vocab, hidden_dim / 2] with k even in the low nibble, scales
  * [vocab, hidden_dim / group] of scale_dtype, zeros uint8 of the same shape
  * (0..15), or null for codes around 8.  A group with a NaN or an infinity gets a NaN
- * scale: its row's logits are NaN.  nvjsel_w4_pack lays a plain form out
+ * scale: its row's logits are NaN; a scale beyond its type becomes the type's
+ * largest.  nvjsel_w4_pack lays a plain form out
  * for the kernels, once: packed, nvjsel_w4_packed_size() bytes (0 for a shape
  * that is not served), 16-byte aligned.
  */

@@ -42,7 +42,8 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
 // element strides sv and sk.  Without zero points s = max|w| / 7 and q - 8 =
 // rint(w / s) in -8..7; with them s = (max - min) / 15 over the values and 0,
 // z = rint(-min / s).  The codes are taken against the scale as it is stored.  A group
-// that holds a NaN or an infinity gets a NaN scale, which makes its row's logits NaN.
+// that holds a NaN or an infinity gets a NaN scale, which makes its row's logits NaN; a
+// finite one whose scale is beyond its type the type's largest, and its codes end at 0 and 15.
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict__ weight, int wdt, int64_t sv, int64_t sk,
                                                           int V, int H, int group, int sdt, uint8_t* __restrict__ q,
                                                           uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros) {
@@ -60,9 +61,11 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict
       lo = fminf(lo, __shfl_xor(lo, m, 64));
       hi = fmaxf(hi, __shfl_xor(hi, m, 64));
     }
-    const float raw = zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
+    float raw = zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
+    if (!__builtin_isfinite(raw)) raw = hi / 15.0f - lo / 15.0f;  // hi - lo is beyond f32
     const bool finite = !__any(!__builtin_isfinite(a) || !__builtin_isfinite(b));  // of the wave's group
-    const float s = finite ? round_to_dtype(raw, sdt) : NAN;
+    const float most = sdt == DT_BF16 ? 0x1.FEp127f : 65504.0f;
+    const float s = finite ? fminf(round_to_dtype(raw, sdt), most) : NAN;
     float z = 8.0f;
     if (zeros) z = s > 0.0f ? fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f) : 0.0f;
     const float ca = s > 0.0f ? fminf(fmaxf(rintf(a / s) + z, 0.0f), 15.0f) : z;

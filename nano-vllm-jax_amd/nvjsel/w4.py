@@ -59,7 +59,8 @@ def quantize_lm_head_w4(weight: torch.Tensor, *, group_size: int = 128, symmetri
     None; else ``scale = (max - min) / 15`` over the values and 0, and zero points.
     Scales are of ``scale_dtype`` (the weight's own 16-bit type, bf16 for f32), and
     the codes are rounded against them as stored.  A group that holds a NaN or an
-    infinity gets a NaN scale: its row's logits are NaN.  Returns the plain form
+    infinity gets a NaN scale: its row's logits are NaN.  A scale beyond its type is the
+    type's largest, and weights that its codes do not reach end at the last one.  Returns the plain form
     ``(qweight, scales, zeros)``."""
     if weight.ndim != 2:
         raise ValueError("the LM-head weight must be [H, V] (or [V, H] with weight_layout='vh')")

@@ -44,3 +44,36 @@ def test_weights_that_are_not_finite(dtype, group, scale, symmetric):
     want = nvjsel.lm_head_logits_hip(x, nvjsel.pack_lm_head_w4(q0, s0, z0), reduce_cast=0).cpu()
     rows = at.any(1)
     assert bool(logits[:, rows].isnan().all()) and torch.equal(logits[:, ~rows], want[:, ~rows])
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype,scale,size", [("f32", "f16", 1e6), ("bf16", "f16", 3e7), ("f32", "f16", 3e38),
+                                              ("f32", "bf16", 3.3e38), ("bf16", "bf16", 3.3e38)])
+def test_scales_beyond_their_type(dtype, scale, size, symmetric):
+    """Finite weights whose scale does not fit its type: the largest scale, codes that end at
+    0 and 15, and finite logits.  A code is the nearest one that there is: the value it
+    stands for is off by half a scale at most, or ends at the codes' end."""
+    w = torch.randn(17, 128, generator=torch.Generator().manual_seed(3)).clamp(-1, 1)
+    w[5] *= 1e-3
+    w[9] = 1.0
+    w[10, ::2], w[10, 1::2] = 1.0, -1.0
+    w = (w * size).to(DT[dtype])
+    q, s, z = nvjsel.quantize_lm_head_w4(w.cuda(), group_size=32, symmetric=symmetric, scale_dtype=DT[scale],
+                                         weight_layout="vh")
+    assert bool(s.isfinite().all()) and bool((s > 0).all())
+    wide = w.double().reshape(17, 4, 32)
+    lo, hi = wide.amin(2).clamp(max=0), wide.amax(2).clamp(min=0)
+    want = torch.maximum(hi, -lo) / 7 if symmetric else (hi - lo) / 15
+    most = torch.finfo(DT[scale]).max
+    step = torch.finfo(DT[scale]).eps / 2 + 2.0 ** -22  # the scale's rounding, and those of the f32 steps to it
+    assert bool(((s.double().cpu() - want.clamp(max=most)).abs() <= step * want).all())
+    assert bool((s.double().cpu()[want > most] == most).all())
+    zero = torch.full((17, 4), 8.0, dtype=torch.float64) if symmetric else z.cpu().double()
+    sd = s.cpu().double()
+    bottom, top = -zero * sd, (15 - zero) * sd  # what the codes reach
+    back = dequantized(q, s, z, 32).reshape(17, 4, 32)
+    near = torch.minimum(torch.maximum(wide, bottom[:, :, None]), top[:, :, None])
+    assert bool(((back - near).abs() <= sd[:, :, None] * (0.5 + 2.0 ** -18)).all())
+    x = torch.randn(2, 128, generator=torch.Generator().manual_seed(2)) * 1e-6
+    logits = nvjsel.lm_head_logits_hip(x.cuda(), nvjsel.pack_lm_head_w4(q, s, z))
+    assert bool(logits.isfinite().all())
