@@ -266,7 +266,7 @@ int nvjsel_derive_keys_table(const int32_t* slots, int batch, int32_t* counter_t
  * scale: its row's logits are NaN; a scale beyond its type becomes the type's
  * largest.  nvjsel_w4_pack lays a plain form out
  * for the kernels, once: packed, nvjsel_w4_packed_size() bytes (0 for a shape
- * that is not served), 16-byte aligned.
+ * that is not served), 16-byte aligned; of a zero point the low four bits count.
  */
 size_t nvjsel_w4_packed_size(int vocab, int hidden_dim, int group, int has_zeros);
 

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
       const int r = t / lay.ng, g = kb * lay.ng + t % lay.ng, vs = tile * 32 + 16 * (r & 1) + (r >> 1);
       const bool in = vs < V && g < G;
       ((uint16_t*)(packed + lay.scales))[blk * 32 * lay.ng + t] = in ? scales[(size_t)vs * G + g] : (uint16_t)0;
-      if (zeros) (packed + lay.zeros)[blk * 32 * lay.ng + t] = in ? (uint8_t)(16 + zeros[(size_t)vs * G + g]) : (uint8_t)16;
+      if (zeros) (packed + lay.zeros)[blk * 32 * lay.ng + t] = in ? (uint8_t)(16 + (zeros[(size_t)vs * G + g] & 15)) : (uint8_t)16;
     }
   }
 }

@@ -91,7 +91,9 @@ def quantize_lm_head_w4(weight: torch.Tensor, *, group_size: int = 128, symmetri
 def pack_lm_head_w4(qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> W4Weight:
     """Lay the plain form out for the kernels (a copy; the plain form may go).
 
-    The group size is ``H / scales.shape[1]``: 32, 64 or 128.  ``zeros`` hold 0..15."""
+    The group size is ``H / scales.shape[1]``: 32, 64 or 128.  ``zeros`` hold 0..15:
+    larger ones are refused, which waits for the device once (under graph capture, where
+    nothing can be waited for, their low four bits count)."""
     if qweight.ndim != 2 or qweight.dtype != torch.uint8:
         raise ValueError("qweight must be uint8 [V, H / 2]")
     vocab, hidden = int(qweight.shape[0]), 2 * int(qweight.shape[1])
@@ -112,6 +114,8 @@ def pack_lm_head_w4(qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Te
     packed = torch.empty((lib.nvjsel_w4_packed_size(vocab, hidden, group, zeros is not None),), dtype=torch.uint8,
                          device=dev)
     with _on_device(dev):
+        if zeros is not None and not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > 15:
+            raise ValueError("zeros must be 0..15")
         _lib.call("nvjsel_w4_pack", qweight.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                   vocab, hidden, group, packed.data_ptr(), packed.numel(), _stream_handle(dev))
     return W4Weight(packed, vocab, hidden, group, scales.dtype, zeros is not None)

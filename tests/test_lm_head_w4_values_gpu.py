@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import nvjsel
+from nvjsel import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,22 @@ def test_scales_beyond_their_type(dtype, scale, size, symmetric):
     x = torch.randn(2, 128, generator=torch.Generator().manual_seed(2)) * 1e-6
     logits = nvjsel.lm_head_logits_hip(x.cuda(), nvjsel.pack_lm_head_w4(q, s, z))
     assert bool(logits.isfinite().all())
+
+
+def test_zero_points_are_0_to_15():
+    q = torch.randint(0, 256, (33, 64), dtype=torch.uint8, device="cuda")
+    s = torch.full((33, 4), 0.01, dtype=torch.float16, device="cuda")
+    z = torch.randint(0, 16, (33, 4), dtype=torch.uint8, device="cuda")
+    head = nvjsel.pack_lm_head_w4(q, s, z)
+    for bad in (16, 240, 255):
+        wrong = z.clone()
+        wrong[32, 3] = bad
+        with pytest.raises(ValueError, match="0..15"):
+            nvjsel.pack_lm_head_w4(q, s, wrong)
+    # by the C ABI, which does not wait: the low four bits count
+    packed, high = torch.empty_like(head.packed), z + 240
+    _lib.call("nvjsel_w4_pack", q.data_ptr(), s.data_ptr(), high.data_ptr(), 33, 128, 32, packed.data_ptr(),
+              packed.numel(), torch.cuda.current_stream().cuda_stream)
+    x = torch.randn(3, 128, device="cuda")
+    other = nvjsel.W4Weight(packed, 33, 128, 32, torch.float16, True)
+    assert torch.equal(nvjsel.lm_head_logits_hip(x, other), nvjsel.lm_head_logits_hip(x, head))
