@@ -282,7 +282,8 @@ int nvjsel_w4_pack(const void* qweight, const void* scales, const void* zeros, i
  * [batch, hidden_dim] f32, bf16 or f16, fp32 accumulation, the same workspace
  * (nvjsel_lm_head_workspace_size) and the same order of ids.  scale_dtype,
  * has_zeros and group as packed.  A hidden row that holds a NaN or an infinity
- * gets NaN for every logit.
+ * gets NaN for every logit.  bf16 and f32 values up to 2^115 (4e34) in magnitude keep the
+ * sums of a group within fp32; with larger ones its logits may be NaN or infinite too.
  */
 int nvjsel_lm_head_w4_top1(const void* hidden, int hidden_dtype, const void* packed, size_t packed_bytes,
                            int scale_dtype, int has_zeros, int group, int batch, int hidden_dim, int vocab,

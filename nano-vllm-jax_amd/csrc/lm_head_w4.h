@@ -9,7 +9,8 @@
 // exactly, so one shift and one and-or make two operands.  The accumulator of
 // a group starts at -(16 + z) times the group's sum of activations, so that
 // the offset is gone when the group ends; then it is scaled into the row's
-// total.  Sums are fp32 throughout.  The offset is the smallest one that an
+// total.  Sums are fp32 throughout: a group's, up to 2 x 31 x 128 |x| with the offset, stay
+// within it for |x| up to 2^115.  The offset is the smallest one that an
 // exponent's mantissa holds: with 128 + q (no shift for a quarter of the nibbles)
 // the partial sums are six times larger than the result's terms, and so is their
 // rounding.

@@ -13,7 +13,8 @@ loaded; the ``W4Weight`` it returns stands in for the weight tensor in
 The weight's values are not of a 16-bit type, so results round (``reduce_cast``
 None) to the activations' type alone: bf16 activations give bf16 logits, f16
 f16, f32 f32.  A hidden row holding a NaN or an infinity gets NaN for every
-logit.
+logit; bf16 and f32 values above 2^115 (4e34) in magnitude may take a group's sums out of
+fp32 and make its logits NaN or infinite too.
 """
 from __future__ import annotations
 

@@ -4,6 +4,7 @@ import torch
 
 import nvjsel
 from nvjsel import _lib
+from tests.test_lm_head_w4_gpu import exact, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +98,28 @@ def test_zero_points_are_0_to_15():
     x = torch.randn(3, 128, device="cuda")
     other = nvjsel.W4Weight(packed, 33, 128, 32, torch.float16, True)
     assert torch.equal(nvjsel.lm_head_logits_hip(x, other), nvjsel.lm_head_logits_hip(x, head))
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,group,act,zeros", [
+    (1, 300, 1024, 128, "bf16", False), (16, 300, 512, 64, "bf16", True), (64, 70000, 2048, 128, "bf16", False),
+    (3, 300, 1024, 128, "f32", True), (16, 40000, 1024, 128, "f32", False), (31, 70000, 2048, 32, "f32", True),
+    (5, 300, 1024, 128, "f16", True)])
+def test_largest_activations(rows, vocab, hidden, group, act, zeros):
+    """Values of 2^115 (f16: its largest) whose offsets, partial sums and products add up the most."""
+    size = torch.finfo(torch.float16).max if act == "f16" else 2.0 ** 115
+    g = torch.Generator().manual_seed(rows)
+    codes = torch.randint(0, 16, (vocab, hidden), generator=g, dtype=torch.uint8)
+    codes[0], codes[1] = 15, 0
+    scales = torch.full((vocab, hidden // group), 2.0 ** -10, dtype=torch.bfloat16)
+    z = torch.randint(0, 16, (vocab, hidden // group), generator=g, dtype=torch.uint8) if zeros else None
+    if zeros:
+        z[0], z[1] = 0, 15
+    x = (torch.randint(0, 2, (rows, hidden), generator=g) * 2 - 1) * size
+    x[0] = size
+    x[-1, hidden // 2:] = -size
+    x = x.to(DT[act])
+    q = codes[:, 0::2] | codes[:, 1::2] << 4
+    head = nvjsel.pack_lm_head_w4(q.cuda(), scales.cuda(), None if z is None else z.cuda())
+    got = nvjsel.lm_head_logits_hip(x.cuda(), head, reduce_cast=0)[:, :300].cpu()
+    want, mag = exact(codes[:300], scales[:300], None if z is None else z[:300], group, x)
+    assert bool(((got.double() - want).abs() <= tolerance(want, mag, torch.float32)).all())
