@@ -1057,23 +1057,28 @@ extern "C" int nvjsel_reorder_states(const nvjsel_state* states, int count, cons
       return fail(NVJSEL_EINVAL, "reorder_states: fewer rows than batch x beams");
   }
   const int vec = beams <= 16 ? 16 : 4;
+  auto describe = [&](const nvjsel_state& t) {
+    ReorderTensor r{};
+    r.data = (char*)t.data;
+    r.row_bytes = t.row_bytes;
+    r.rows = t.rows;
+    r.token = lengths ? t.token_bytes : 0;
+    r.outer = lengths ? t.outer : 1;
+    r.span = t.length * t.token_bytes * (lengths ? 1 : t.outer);
+    const int64_t c = (r.span + 256 * vec - 1) / (256 * vec);
+    r.chunks = c * (__int128)r.outer > 0xFFFFFF ? 0 : (int)c;  // 0: more than 2^32 threads
+    return r;
+  };
+  for (int i = 0; i < count; ++i)  // of all of them, before any is moved
+    if (describe(states[i]).chunks == 0) return fail(NVJSEL_EINVAL, "reorder_states: state too large");
   for (int i0 = 0; i0 < count; i0 += kReorderTensors) {
     const int n = count - i0 < kReorderTensors ? count - i0 : kReorderTensors;
     ReorderArgs a{};
     int64_t blocks = 1;
     for (int i = 0; i < n; ++i) {
-      const nvjsel_state& t = states[i0 + i];
-      ReorderTensor& r = a.t[i];
-      r.data = (char*)t.data;
-      r.row_bytes = t.row_bytes;
-      r.rows = t.rows;
-      r.token = lengths ? t.token_bytes : 0;
-      r.outer = lengths ? t.outer : 1;
-      r.span = t.length * t.token_bytes * (lengths ? 1 : t.outer);
-      const int64_t c = (r.span + 256 * vec - 1) / (256 * vec);
-      if (c * (__int128)r.outer > 0xFFFFFF) return fail(NVJSEL_EINVAL, "reorder_states: state too large");  // 2^32 threads
-      r.chunks = (int)c;
-      if (c * r.outer > blocks) blocks = c * r.outer;
+      a.t[i] = describe(states[i0 + i]);
+      const int64_t b = (int64_t)a.t[i].chunks * a.t[i].outer;
+      if (b > blocks) blocks = b;
     }
     a.parents = parents;
     a.parent_stride = parent_stride;
