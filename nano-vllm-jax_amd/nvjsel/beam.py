@@ -98,6 +98,8 @@ def _describe_state(t: torch.Tensor, rows: int | None, length_dim: int | None) -
         if not 1 <= at < t.ndim:
             raise ValueError(f"length_dim {length_dim} is not a dimension of a row of {tuple(shape)}")
         outer, length = math.prod(shape[1:at]), shape[at]
+    if max(shape[0], outer) >= 1 << 31:
+        raise ValueError("a state has less than 2^31 rows, and positions before length_dim")
     return (t.stride(0) if shape[0] > 1 else row) * size, length, row // (outer * length) * size, outer, shape[0]
 
 

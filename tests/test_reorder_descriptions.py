@@ -1,5 +1,8 @@
 """CPU: states that a reordering refuses by their sizes."""
-from nvjsel import _lib
+import pytest
+import torch
+
+from nvjsel import _lib, beam
 
 DUMMY = 0x1000  # never dereferenced: validation fails first
 
@@ -16,3 +19,12 @@ def test_a_state_too_large_is_refused_before_any_is_moved():
     table = _lib.states(small * 30 + many)
     assert lib.nvjsel_reorder_states(table, 31, DUMMY, 4, None, DUMMY, 2, 4, None) == -1
     assert b"too large" in lib.nvjsel_last_error()
+
+
+def test_sizes_beyond_32_bits():
+    wide = torch.empty(4, 1 << 31, 1, dtype=torch.uint8, device="meta")
+    assert _lib.states([DUMMY, *beam._describe_state(wide, 4, 1)])
+    with pytest.raises(ValueError, match="2\\^31"):
+        beam._describe_state(wide, 4, 2)
+    with pytest.raises(ValueError, match="2\\^31"):
+        beam._describe_state(torch.empty(1 << 31, 1, dtype=torch.uint8, device="meta"), None, None)
