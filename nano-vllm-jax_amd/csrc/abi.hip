@@ -19,6 +19,11 @@ void set_error(const char* fmt, ...) {
 
 void clear_error() { g_last_error[0] = '\0'; }
 
+std::mutex& launch_mutex() {
+  static std::mutex mu;
+  return mu;
+}
+
 int device_cu_count() {
   static std::mutex mu;
   static int cached[64] = {0};

@@ -13,8 +13,6 @@
 // are fp32 within a lane's 16 or 32 logits of a chunk and fp64 across chunks, lanes and parts.
 #include <float.h>
 
-#include <mutex>
-
 #include "nvjsel_device.h"
 #include "nvjsel_host.h"
 
@@ -845,14 +843,10 @@ static size_t beam_bytes(int batch, int beams, int shares, int cap) {
   return kBeamRequests * 4 + (size_t)batch * beams * shares * (sizeof(BeamPart) + cap * sizeof(uint2));
 }
 
-// Calls of several threads on one stream may share a workspace: no other call's launch,
-// of one kernel or of two, comes between a call's scan and the join that reads what it wrote.
-static std::mutex g_beam_mu;
-
 template <int DT>
 static int launch_beam(const BeamArgs& a, hipStream_t s) {
   const int64_t waves = (int64_t)a.batch * a.beams * a.shares;
-  std::lock_guard<std::mutex> lock(g_beam_mu);
+  std::lock_guard<std::mutex> lock(launch_mutex());
   if (waves <= kBeamOne && a.beams * a.shares <= kBeamFew) {
     hipLaunchKernelGGL(beam_select_kernel<DT>, dim3((unsigned)(a.batch * a.blocks)), dim3(kBeamThreads), 0, s, a);
     NVJSEL_CHECK_LAUNCH("beam_select_kernel");

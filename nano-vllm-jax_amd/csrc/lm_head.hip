@@ -1413,6 +1413,8 @@ static int lm_head_entry(int mode, const void* hidden, int hidden_dtype, const v
   const bool gemm3 = !mix3 && gemm_ok && hv_gemm_ok && eff_dtype == NVJSEL_F32 && batch > mix_rest;
   const bool fused_prenorm = prenorm && !gemm && !gemm3 && !mix3 &&
                              (gemv || (tile && (eff_dtype != NVJSEL_BF16 || batch <= kTilePrenormRows)));
+  std::unique_lock<std::mutex> lock(launch_mutex(), std::defer_lock);
+  if (need) lock.lock();
   if (prenorm && !fused_prenorm) {
     LmArgs p{};
     p.hidden = hidden;

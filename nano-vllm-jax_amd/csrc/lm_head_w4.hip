@@ -143,6 +143,8 @@ static int w4_entry(int mode, const void* hidden, int hidden_dtype, const void* 
   a.out_dtype = out_dtype;
   a.out_stride = out_stride;
   a.counter = mode == MODE_GREEDY ? (unsigned int*)((char*)workspace + align_up((size_t)batch * 8, 256)) : nullptr;
+  std::unique_lock<std::mutex> lock(launch_mutex(), std::defer_lock);
+  if (mode == MODE_GREEDY) lock.lock();  // logits take no workspace
   const int most = kW4Rows;
   for (int b0 = 0; b0 < batch; b0 += most) {
     a.B = batch - b0 < most ? batch - b0 : most;

@@ -6,6 +6,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <mutex>
+
 #include "../../include/nvjsel.h"
 
 namespace nvjsel {
@@ -17,6 +19,11 @@ void clear_error();
 int device_cu_count();
 // Largest LDS allocation one workgroup may request on the current device.
 size_t device_max_lds_per_block();
+
+// Held by every entry point that takes a workspace, from its first launch to its last:
+// threads that share a stream may share its workspaces, and no other call's launch may
+// come between two that pass data through one.
+std::mutex& launch_mutex();
 
 inline int fail(int code, const char* what) {
   set_error("%s", what);

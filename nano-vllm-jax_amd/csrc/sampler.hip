@@ -2442,6 +2442,7 @@ static int sample_impl(const void* logits, int dtype, int batch, int vocab, int6
   // one pass when the call has no top-k/top-p arrays and its blocks fit one
   // round on the device (4 per CU): a latency-bound call saves the scan and
   // select launches; larger ones keep the seeded, pruned Gumbel pass
+  std::lock_guard<std::mutex> lock(launch_mutex());
   const int nsub = (vocab + kThreads * kOnepassEPT - 1) / (kThreads * kOnepassEPT);
   if (!top_k && !top_p && batch <= kOnepassRows && (long long)batch * nsub <= 4LL * device_cu_count() &&
       (long long)batch * nsub <= kOnepassSlots) {
@@ -2512,6 +2513,7 @@ extern "C" int nvjsel_topk(const void* logits, int dtype, int batch, int vocab, 
   const int vec = (int)(16 / esz);
   const bool vec_ok = (vocab % vec) == 0 && (row_stride % vec) == 0 && (((uintptr_t)logits) & 15) == 0;
   const dim3 grid_chunks(a.nchunks, batch);
+  std::lock_guard<std::mutex> lock(launch_mutex());
   if (dtype == NVJSEL_F32) {
     if (vec_ok) hipLaunchKernelGGL((sample_scan_kernel<DT_F32, 4>), grid_chunks, dim3(kThreads), 0, s, a);
     else hipLaunchKernelGGL((sample_scan_kernel<DT_F32, 1>), grid_chunks, dim3(kThreads), 0, s, a);
