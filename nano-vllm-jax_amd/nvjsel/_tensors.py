@@ -68,6 +68,17 @@ class _WorkspacePool:
 _WS = _WorkspacePool()
 
 
+def _workspace(device: torch.device, stream: int, kind: str, nbytes: int, at_rest: int) -> torch.Tensor:
+    """The stream's workspace, or, under capture, one of the graph's own: graphs captured on
+    one stream may be replayed at the same time.  Every replay zeroes its first ``at_rest``
+    bytes again.  For a call with ``device`` the current one."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:at_rest].zero_()
+        return ws
+    return _WS.get(device, stream, kind, nbytes)
+
+
 _HERE = nullcontext()
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 

@@ -8,7 +8,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from ._tensors import _WS, _dtype_code, _on_device, _require_cuda, _stream_handle
+from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
 from .selection import lm_head_logits_hip, rms_norm_hip
 
 MAX_BEAMS = 64  # beams and candidates of a request
@@ -66,13 +66,7 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candid
     with _on_device(dev):
         nbytes = _select_bytes(dev.index, dt, batch, beams, vocab, k)
         stream = _stream_handle(dev)
-        if torch.cuda.is_current_stream_capturing():
-            # a graph keeps a workspace of its own: graphs captured on one stream may be
-            # replayed at the same time
-            ws = scores.new_empty((nbytes,), dtype=torch.uint8)
-            ws[:4 * batch].zero_()  # the requests' tickets
-        else:
-            ws = _WS.get(dev, stream, "beam", nbytes)
+        ws = _workspace(dev, stream, "beam", nbytes, 4 * batch)  # at rest: the requests' tickets
         _lib.call("nvjsel_beam_select", logits.data_ptr(), dt, batch, beams, vocab, logits.stride(0), logits.stride(1),
                   scores.data_ptr(), None if finished is None else finished.data_ptr(), end_token or 0, k,
                   out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes,

@@ -24,7 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _require_cuda, _stream_handle
+from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _require_cuda, _stream_handle, _workspace
 from .w4 import W4Weight, w4_greedy as _w4_greedy, w4_logits as _w4_logits
 
 
@@ -149,11 +149,22 @@ def _row_stride(logits: torch.Tensor) -> int:
     return int(logits.stride(0)) if int(logits.shape[0]) > 1 else int(logits.shape[1])
 
 
+_SAMPLER_AT_REST = 96 * 1024  # bytes of its workspace that are zero at rest (include/nvjsel.h)
+
+
 def sample_token_ids(logits: torch.Tensor, temperatures: torch.Tensor, rng_keys: torch.Tensor, *,
                      top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
                      noise: torch.Tensor | None = None) -> torch.Tensor:
     """Per-row temperature / top-k / top-p sampling over ``logits [B, V]``
     (or ``[B, 1, V]``).  Returns int32 ``[B]``."""
+    return _sample(logits, temperatures, rng_keys, top_k, top_p, noise, _WS.get)
+
+
+def _own_sampler_workspace(device, stream, kind, nbytes):
+    return _workspace(device, stream, kind, nbytes, _SAMPLER_AT_REST)
+
+
+def _sample(logits, temperatures, rng_keys, top_k, top_p, noise, workspace) -> torch.Tensor:
     if logits.ndim == 3:
         if int(logits.shape[1]) != 1:
             raise ValueError("sampler takes logits [B, V] or [B, 1, V]")
@@ -189,7 +200,7 @@ def sample_token_ids(logits: torch.Tensor, temperatures: torch.Tensor, rng_keys:
     out = torch.empty((batch,), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    ws = _WS.get(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
+    ws = workspace(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
     _lib.call("nvjsel_sample", logits.data_ptr(), dt, batch, vocab, _row_stride(logits),
               temps.data_ptr(), tk.data_ptr() if tk is not None else None,
               tp.data_ptr() if tp is not None else None, keys.data_ptr(),
@@ -219,7 +230,7 @@ def lm_head_sample_token_ids(hidden_norm: torch.Tensor, output_weight: torch.Ten
     if isinstance(output_weight, W4Weight):
         x = x if norm_weight is None else rms_norm_hip(x, norm_weight, rms_norm_eps, act_dtype)
         logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
-        return sample_token_ids(logits, temperatures, rng_keys, top_k=top_k, top_p=top_p)
+        return _sample(logits, temperatures, rng_keys, top_k, top_p, None, _own_sampler_workspace)
     hd = _dtype_code(x, "hidden")
     wd = _dtype_code(output_weight, "weight")
     w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
@@ -332,6 +343,10 @@ def topk_hip(logits: torch.Tensor, k: int):
     ``logits [B, V]`` (or ``[B, 1, V]``): values f32 ``[B, k]`` (the logits'
     own values) and indices int32 ``[B, k]``, by value descending then index
     ascending (NaN first, -0.0 == +0.0)."""
+    return _topk(logits, k, _WS.get)
+
+
+def _topk(logits, k, workspace):
     squeeze = logits.ndim == 3
     if squeeze:
         if int(logits.shape[1]) != 1:
@@ -353,7 +368,7 @@ def topk_hip(logits: torch.Tensor, k: int):
     indices = torch.empty((batch, k), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    ws = _WS.get(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
+    ws = workspace(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
     _lib.call("nvjsel_topk", logits.data_ptr(), dt, batch, vocab, _row_stride(logits), k, values.data_ptr(),
               indices.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     if squeeze:
@@ -383,15 +398,17 @@ def lm_head_token_ids_and_topk(hidden: torch.Tensor, output_weight: torch.Tensor
         ids = lm_head_greedy_top1_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
                                       norm_weight=norm_weight, rms_norm_eps=rms_norm_eps, act_dtype=act_dtype)
         return ids.reshape(batch, width), None, None
+    workspace = _WS.get
     if isinstance(output_weight, W4Weight):
         x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
         logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
+        workspace = _own_sampler_workspace
     else:
         w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
         x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
         rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
         logits = _dense_logits(x.contiguous(), w, layout, vocab, rc)
-    values, indices = topk_hip(logits, int(top_k))
+    values, indices = _topk(logits, int(top_k), workspace)
     ids = indices[:, 0].reshape(batch, width)
     return ids, values.reshape(batch, width, -1), indices.reshape(batch, width, -1)
 

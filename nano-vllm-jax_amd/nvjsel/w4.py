@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _on_device, _require_cuda, _stream_handle
+from ._tensors import _TORCH_DTYPES, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
 
 GROUP_SIZES = (32, 64, 128)
 _SCALE_DTYPES = (torch.bfloat16, torch.float16)
@@ -158,12 +158,7 @@ def w4_greedy(x: torch.Tensor, weight: W4Weight, weight_layout=None, reduce_cast
     nbytes = _lib.load().nvjsel_lm_head_workspace_size(batch)
     with _on_device(dev):
         stream = _stream_handle(dev)
-        if torch.cuda.is_current_stream_capturing():
-            # a graph keeps a workspace of its own, filled again by every replay:
-            # graphs captured on one stream may be replayed at the same time
-            ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        else:
-            ws = _WS.get(dev, stream, "lm_head", nbytes)
+        ws = _workspace(dev, stream, "lm_head", nbytes, nbytes)
         _lib.call("nvjsel_lm_head_w4_top1", *args, out.data_ptr(), best.data_ptr() if return_best else None,
                   ws.data_ptr(), ws.numel(), stream)
     return (out, best) if return_best else out

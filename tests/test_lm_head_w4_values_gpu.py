@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import nvjsel
-from nvjsel import _lib
+from nvjsel import _lib, _tensors
 from tests.test_lm_head_w4_gpu import exact, tolerance
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +123,41 @@ def test_largest_activations(rows, vocab, hidden, group, act, zeros):
     got = nvjsel.lm_head_logits_hip(x.cuda(), head, reduce_cast=0)[:, :300].cpu()
     want, mag = exact(codes[:300], scales[:300], None if z is None else z[:300], group, x)
     assert bool(((got.double() - want).abs() <= tolerance(want, mag, torch.float32)).all())
+
+
+def test_captured_routes_keep_their_own_workspaces(monkeypatch):
+    """Every route of a 4-bit weight, captured: none takes the stream's workspace, and replays with
+    eager calls between them give the eager results."""
+    weight = (torch.randn(20011, 256, generator=torch.Generator().manual_seed(6)) * 0.1).to(torch.bfloat16).cuda()
+    head = nvjsel.pack_lm_head_w4(*nvjsel.quantize_lm_head_w4(weight.T))
+    xs = [(torch.randn(9, 1, 256, generator=torch.Generator().manual_seed(i)) * 2).to(torch.bfloat16).cuda() for i in range(3)]
+    keys = nvjsel.derive_rng_keys(torch.arange(9, device="cuda", dtype=torch.int32),
+                                  torch.ones(9, device="cuda", dtype=torch.int32))[0]
+    temps = torch.full((9,), 0.9, device="cuda")
+    top_k = torch.full((9,), 12, device="cuda", dtype=torch.int32)
+    norm = 0.1 * torch.randn(256, generator=torch.Generator().manual_seed(9)).cuda()
+    scores = torch.zeros(3, 3, device="cuda")
+
+    def routes(x):
+        return [nvjsel.lm_head_greedy_top1_hip(x, head), nvjsel.lm_head_logits_hip(x, head),
+                nvjsel.lm_head_sample_token_ids(x, head, temperatures=temps, rng_keys=keys),
+                nvjsel.lm_head_sample_token_ids(x, head, temperatures=temps, rng_keys=keys, top_k=top_k, norm_weight=norm,
+                                                act_dtype=torch.bfloat16),
+                *nvjsel.lm_head_token_ids_and_topk(x.reshape(3, 3, 256), head, top_k=5),
+                nvjsel.mtp_greedy_top1_token_ids(x.reshape(3, 3, 256), head),
+                *nvjsel.lm_head_beam_search_step(x.reshape(3, 3, 256), head, scores)]
+
+    want = [[t.clone() for t in routes(x)] for x in xs]
+    fixed = xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with monkeypatch.context() as m:
+        m.setattr(type(_tensors._WS), "get", lambda *a: pytest.fail("a captured call took the stream's workspace"))
+        with torch.cuda.graph(graph):
+            out = routes(fixed)
+    for rep in range(4):
+        fixed.copy_(xs[rep % 3])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[rep % 3]))
+        assert all(torch.equal(a, b) for a, b in zip(routes(xs[1]), want[1]))
