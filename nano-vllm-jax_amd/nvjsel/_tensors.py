@@ -46,10 +46,13 @@ class _WorkspacePool:
     """Zero-filled scratch buffers per (device, stream, kind).
 
     Each entry point leaves its workspace zero-filled when it returns, so a
-    buffer is zeroed once at allocation and reused in stream order."""
+    buffer is zeroed once at allocation and reused in stream order.  A captured call may hold
+    a buffer for as long as its graph lives, so a larger one does not replace it but comes
+    beside it, at twice its size; beam search's, which no captured call takes, go."""
 
     def __init__(self):
         self._bufs: dict = {}
+        self._held: list = []
         self._lock = threading.Lock()
 
     def get(self, device: torch.device, stream: int, kind: str, nbytes: int) -> torch.Tensor:
@@ -60,7 +63,11 @@ class _WorkspacePool:
         with self._lock:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
-                buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
+                size = max(nbytes, 4096)
+                if buf is not None and kind != "beam":
+                    self._held.append(buf)
+                    size = max(size, 2 * buf.numel())
+                buf = torch.zeros(size, dtype=torch.uint8, device=device)
                 self._bufs[key] = buf
             return buf
 

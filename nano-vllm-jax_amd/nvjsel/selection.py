@@ -149,7 +149,7 @@ def _row_stride(logits: torch.Tensor) -> int:
     return int(logits.stride(0)) if int(logits.shape[0]) > 1 else int(logits.shape[1])
 
 
-_SAMPLER_AT_REST = 96 * 1024  # bytes of its workspace that are zero at rest (include/nvjsel.h)
+_SAMPLER_AT_REST = 96 * 1024  # bytes of its workspace that are zero at rest (ws_layout in csrc/sampler.hip)
 
 
 def sample_token_ids(logits: torch.Tensor, temperatures: torch.Tensor, rng_keys: torch.Tensor, *,
