@@ -24,7 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _require_cuda, _stream_handle, _workspace
+from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
 from .w4 import W4Weight, w4_greedy as _w4_greedy, w4_logits as _w4_logits
 
 
@@ -200,12 +200,13 @@ def _sample(logits, temperatures, rng_keys, top_k, top_p, noise, workspace) -> t
     out = torch.empty((batch,), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    ws = workspace(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
-    _lib.call("nvjsel_sample", logits.data_ptr(), dt, batch, vocab, _row_stride(logits),
-              temps.data_ptr(), tk.data_ptr() if tk is not None else None,
-              tp.data_ptr() if tp is not None else None, keys.data_ptr(),
-              nz.data_ptr() if nz is not None else None, out.data_ptr(), ws.data_ptr(), ws.numel(),
-              stream)
+    with _on_device(dev):
+        ws = workspace(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
+        _lib.call("nvjsel_sample", logits.data_ptr(), dt, batch, vocab, _row_stride(logits),
+                  temps.data_ptr(), tk.data_ptr() if tk is not None else None,
+                  tp.data_ptr() if tp is not None else None, keys.data_ptr(),
+                  nz.data_ptr() if nz is not None else None, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                  stream)
     return out
 
 
@@ -277,9 +278,10 @@ def _dense_logits(x: torch.Tensor, w: torch.Tensor, layout: int, vocab: int, rc:
     x = x.contiguous()
     out_dtype = {1: torch.bfloat16, 2: torch.float16}.get(rc, torch.float32)
     out = torch.empty((batch, vocab), dtype=out_dtype, device=dev)
-    _lib.call("nvjsel_lm_head_logits", x.data_ptr(), _dtype_code(x, "hidden"), w.data_ptr(),
-              _dtype_code(w, "weight"), layout, batch, hidden_dim, vocab, rc, out.data_ptr(),
-              _TORCH_DTYPES[out_dtype], vocab, _stream_handle(dev))
+    with _on_device(dev):
+        _lib.call("nvjsel_lm_head_logits", x.data_ptr(), _dtype_code(x, "hidden"), w.data_ptr(),
+                  _dtype_code(w, "weight"), layout, batch, hidden_dim, vocab, rc, out.data_ptr(),
+                  _TORCH_DTYPES[out_dtype], vocab, _stream_handle(dev))
     return out
 
 
@@ -317,8 +319,9 @@ def rms_norm_hip(hidden: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1
     if ad is None:
         raise ValueError(f"unsupported act dtype: {act_dtype}")
     out = torch.empty((batch, hidden_dim), dtype=act_dtype, device=dev)
-    _lib.call("nvjsel_rms_norm", x.data_ptr(), hd, nw.data_ptr(), nd, float(eps), ad, batch, hidden_dim,
-              out.data_ptr(), _stream_handle(dev))
+    with _on_device(dev):
+        _lib.call("nvjsel_rms_norm", x.data_ptr(), hd, nw.data_ptr(), nd, float(eps), ad, batch, hidden_dim,
+                  out.data_ptr(), _stream_handle(dev))
     return out
 
 
@@ -368,9 +371,10 @@ def _topk(logits, k, workspace):
     indices = torch.empty((batch, k), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    ws = workspace(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
-    _lib.call("nvjsel_topk", logits.data_ptr(), dt, batch, vocab, _row_stride(logits), k, values.data_ptr(),
-              indices.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    with _on_device(dev):
+        ws = workspace(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
+        _lib.call("nvjsel_topk", logits.data_ptr(), dt, batch, vocab, _row_stride(logits), k, values.data_ptr(),
+                  indices.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     if squeeze:
         return values[:, None, :], indices[:, None, :]
     return values, indices
