@@ -165,9 +165,10 @@ def lm_head_beam_search_step(hidden: torch.Tensor, output_weight, scores: torch.
         raise ValueError("hidden must be [B, W, H]")
     batch, beams, hidden_dim = hidden.shape
     flat = hidden.reshape(batch * beams, hidden_dim)
-    if norm_weight is not None:
-        flat = rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
-    logits = lm_head_logits_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast)
+    with _on_device(_require_cuda(flat)):
+        if norm_weight is not None:
+            flat = rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
+        logits = lm_head_logits_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast)
     new_scores, parents, tokens = beam_search_select(logits.reshape(batch, beams, -1), scores, finished=finished,
                                                      end_token=end_token)
     if states is not None:

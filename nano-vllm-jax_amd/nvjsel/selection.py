@@ -109,7 +109,7 @@ def lm_head_greedy_top1_hip(hidden_norm: torch.Tensor, output_weight: torch.Tens
     one launch on the streaming and bf16 tile paths."""
     x = _flatten_hidden(hidden_norm, require_3d=False)
     if isinstance(output_weight, W4Weight):
-        x = x if norm_weight is None else rms_norm_hip(x, norm_weight, rms_norm_eps, act_dtype)
+        x = x if norm_weight is None else _normed(x, norm_weight, rms_norm_eps, act_dtype)
         return _w4_greedy(x, output_weight, weight_layout, reduce_cast, return_best)
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
     if batch <= 0 or hidden_dim <= 0 or output_weight.numel() == 0:
@@ -200,13 +200,12 @@ def _sample(logits, temperatures, rng_keys, top_k, top_p, noise, workspace) -> t
     out = torch.empty((batch,), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    with _on_device(dev):
-        ws = workspace(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
-        _lib.call("nvjsel_sample", logits.data_ptr(), dt, batch, vocab, _row_stride(logits),
-                  temps.data_ptr(), tk.data_ptr() if tk is not None else None,
-                  tp.data_ptr() if tp is not None else None, keys.data_ptr(),
-                  nz.data_ptr() if nz is not None else None, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                  stream)
+    ws = workspace(dev, stream, "sample", lib.nvjsel_sample_workspace_size(batch, vocab))
+    _lib.call("nvjsel_sample", logits.data_ptr(), dt, batch, vocab, _row_stride(logits),
+              temps.data_ptr(), tk.data_ptr() if tk is not None else None,
+              tp.data_ptr() if tp is not None else None, keys.data_ptr(),
+              nz.data_ptr() if nz is not None else None, out.data_ptr(), ws.data_ptr(), ws.numel(),
+              stream)
     return out
 
 
@@ -229,9 +228,10 @@ def lm_head_sample_token_ids(hidden_norm: torch.Tensor, output_weight: torch.Ten
     if batch <= 0 or hidden_dim <= 0:
         raise ValueError("LM-head sampling requires non-empty dimensions")
     if isinstance(output_weight, W4Weight):
-        x = x if norm_weight is None else rms_norm_hip(x, norm_weight, rms_norm_eps, act_dtype)
+        x = x if norm_weight is None else _normed(x, norm_weight, rms_norm_eps, act_dtype)
         logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
-        return _sample(logits, temperatures, rng_keys, top_k, top_p, None, _own_sampler_workspace)
+        with _on_device(logits.device):
+            return _sample(logits, temperatures, rng_keys, top_k, top_p, None, _own_sampler_workspace)
     hd = _dtype_code(x, "hidden")
     wd = _dtype_code(output_weight, "weight")
     w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
@@ -278,10 +278,9 @@ def _dense_logits(x: torch.Tensor, w: torch.Tensor, layout: int, vocab: int, rc:
     x = x.contiguous()
     out_dtype = {1: torch.bfloat16, 2: torch.float16}.get(rc, torch.float32)
     out = torch.empty((batch, vocab), dtype=out_dtype, device=dev)
-    with _on_device(dev):
-        _lib.call("nvjsel_lm_head_logits", x.data_ptr(), _dtype_code(x, "hidden"), w.data_ptr(),
-                  _dtype_code(w, "weight"), layout, batch, hidden_dim, vocab, rc, out.data_ptr(),
-                  _TORCH_DTYPES[out_dtype], vocab, _stream_handle(dev))
+    _lib.call("nvjsel_lm_head_logits", x.data_ptr(), _dtype_code(x, "hidden"), w.data_ptr(),
+              _dtype_code(w, "weight"), layout, batch, hidden_dim, vocab, rc, out.data_ptr(),
+              _TORCH_DTYPES[out_dtype], vocab, _stream_handle(dev))
     return out
 
 
@@ -319,10 +318,15 @@ def rms_norm_hip(hidden: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1
     if ad is None:
         raise ValueError(f"unsupported act dtype: {act_dtype}")
     out = torch.empty((batch, hidden_dim), dtype=act_dtype, device=dev)
-    with _on_device(dev):
-        _lib.call("nvjsel_rms_norm", x.data_ptr(), hd, nw.data_ptr(), nd, float(eps), ad, batch, hidden_dim,
-                  out.data_ptr(), _stream_handle(dev))
+    _lib.call("nvjsel_rms_norm", x.data_ptr(), hd, nw.data_ptr(), nd, float(eps), ad, batch, hidden_dim,
+              out.data_ptr(), _stream_handle(dev))
     return out
+
+
+def _normed(x, norm_weight, eps, act_dtype):
+    """rms_norm_hip with ``x``'s device the current one, as the 4-bit product has it."""
+    with _on_device(_require_cuda(x)):
+        return rms_norm_hip(x, norm_weight, eps, act_dtype)
 
 
 def derive_rng_keys(slots: torch.Tensor, counters: torch.Tensor):
@@ -371,10 +375,9 @@ def _topk(logits, k, workspace):
     indices = torch.empty((batch, k), dtype=torch.int32, device=dev)
     stream = _stream_handle(dev)
     lib = _lib.load()
-    with _on_device(dev):
-        ws = workspace(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
-        _lib.call("nvjsel_topk", logits.data_ptr(), dt, batch, vocab, _row_stride(logits), k, values.data_ptr(),
-                  indices.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    ws = workspace(dev, stream, "sample", lib.nvjsel_topk_workspace_size(batch, vocab))
+    _lib.call("nvjsel_topk", logits.data_ptr(), dt, batch, vocab, _row_stride(logits), k, values.data_ptr(),
+              indices.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     if squeeze:
         return values[:, None, :], indices[:, None, :]
     return values, indices
@@ -402,17 +405,17 @@ def lm_head_token_ids_and_topk(hidden: torch.Tensor, output_weight: torch.Tensor
         ids = lm_head_greedy_top1_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
                                       norm_weight=norm_weight, rms_norm_eps=rms_norm_eps, act_dtype=act_dtype)
         return ids.reshape(batch, width), None, None
-    workspace = _WS.get
     if isinstance(output_weight, W4Weight):
-        x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
+        x = flat if norm_weight is None else _normed(flat, norm_weight, rms_norm_eps, act_dtype)
         logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
-        workspace = _own_sampler_workspace
+        with _on_device(logits.device):
+            values, indices = _topk(logits, int(top_k), _own_sampler_workspace)
     else:
         w, layout, vocab = _weight_operand(output_weight, weight_layout, hidden_dim)
         x = flat if norm_weight is None else rms_norm_hip(flat, norm_weight, rms_norm_eps, act_dtype)
         rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
         logits = _dense_logits(x.contiguous(), w, layout, vocab, rc)
-    values, indices = _topk(logits, int(top_k), workspace)
+        values, indices = topk_hip(logits, int(top_k))
     ids = indices[:, 0].reshape(batch, width)
     return ids, values.reshape(batch, width, -1), indices.reshape(batch, width, -1)
 
