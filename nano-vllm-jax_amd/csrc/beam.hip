@@ -267,7 +267,7 @@ __device__ __forceinline__ void beam_best(const char* base, int e0, int e1, int 
 // (V = 248,320, 256 rows, K = 16: 2 us more).
 //
 // Bound: the stream, and in part beside it an exponential and a maximum per logit and
-// the pieces set aside: 256 rows of 248,320 bf16 logits (127 MB) take 25 us, 5.1 TB/s, 20 with sums of
+// the pieces set aside: 256 rows of 248,320 bf16 logits (127 MB) take 26 us, 4.9 TB/s, 20 with sums of
 // the logits themselves, 18 with nothing set aside either.  The bound by halving between the least and
 // the greatest lane instead of bit by bit took 2 us more.
 struct BeamScanLds {
@@ -517,9 +517,10 @@ __device__ __forceinline__ uint64_t beam_ord(double x) {
 // candidates that reach it, seldom more than twice K, are ranked by counting, each
 // against all; where there are more than there is room for (many equal scores), every
 // wave keeps the best 64 of its share of them sorted and the waves' lists are merged.
-// Bound: the chain of memory round trips (parts, candidates) and barriers, 6-7 us
-// whatever the size (8 requests of 4 beams, 488 parts each: normalisers 2.0 us, bounds 1.6,
-// candidates 1.0, ranks 0.7).
+// Bound: a chain of memory round trips (parts, candidates), barriers and dependent
+// instructions (an fp64 exponential a part and logarithm a beam, the bound's bits), 7 us
+// whatever the size: with 256 rows its waves wait 70% of their time, and vector
+// instructions fill 1% of it.
 template <int LISTS>
 struct BeamJoinLds {
   static constexpr int RANKED = LISTS == kBeamFew ? 512 : 1024;
@@ -889,9 +890,10 @@ struct ReorderArgs {
 // another thread.  Beams that keep their place are not touched.  Memory bound:
 // each moved beam is written once; a source that several beams take comes from
 // the cache after its first read.  The loads of W beams are in flight together, 16
-// bytes a lane up to 16 beams and 4 above, so that they fit the registers.  12 bf16 states
-// of 64 rows x 1 MB with ragged lengths, 535 MB read and written: 111 us, 4.8 TB/s; whole
-// f32 rows, 1.07 GB: 202 us, 5.3 TB/s; a large copy runs at 5.1.
+// bytes a lane up to 16 beams and 4 above, so that they fit the registers.  Written and
+// read, 12 f32 states of 64 rows x 1 MB, of the bytes that random parents move: 4 and 8
+// beams 5.2 TB/s (1.12 GB 214 us; a large copy runs at 5.1), 16 beams 4.9, 17 to 64 beams, with
+// 4 bytes a lane, 3.1 to 3.7.
 template <int VEC, int WREG>
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   typedef typename std::conditional<VEC == 16, bm_u32x4, uint32_t>::type Vec;

@@ -23,14 +23,16 @@
 // scales follow, per block [row of 16][t][128 / group], and the zero points, 16 added,
 // in the same order.  Rows past V and k past H are zero with scale zero.
 //
-// What bounds it: the weights' stream (7 TB/s), and beside it the sum of vector
-// and matrix instructions, which overlap little on a SIMD: measured with two
-// waves, 2.5 clocks for a shift or an or, 4.5 for v_and_or_b32 or an fma, 17 for
-// the 16x16x32 product and 33 for the 32x32x16 one, so the smaller tile costs
-// half where up to 16 batch rows are there and nothing where there are more.  V =
-// 248,320, H = 1024, groups of 128: one row 26.6 us (131 MB, 4.9 TB/s), 16 rows 26.4; V = 151,936, H =
-// 2560, groups of 64 with zero points, 8 f16 rows 40.3 us (5.3 TB/s); V = 128,256, H = 2048, 64
-// rows 51 us (660 TFLOP/s).
+// What bounds it: up to 16 rows the weights' stream, V = 248,320, H = 1024, groups of
+// 128: one row 26.8 us (131 MB, 4.9 TB/s), 16 rows 25.7; V = 151,936, H = 2560, groups of 64
+// with zero points, 8 f16 rows 40.4 us (5.3 TB/s).  With more rows no unit is full: 64 rows,
+// V = 128,256, H = 2048, 50 us (670 TFLOP/s), the matrix pipe busy for 26% of it, other vector
+// instructions 37%, LDS 25% (more than half of that bank conflicts), and the two waves of a SIMD
+// wait for 31% of their time.  Vector and matrix instructions overlap little: of 32 additions
+// between four products less than half is hidden.  A shift or an or takes 2.5 to 2.8 clocks
+// of a SIMD, v_and_or_b32 or an fma 4 to 4.7, the 16x16x32 product 17 and the 32x32x16 one 33,
+// so the smaller tile costs half where up to 16 batch rows are there and nothing where there
+// are more.
 #pragma once
 #include "lm_head_common.h"
 
@@ -662,9 +664,9 @@ static inline W4Plan w4_plan(const W4Args& a, int group, int terms, int mb, int 
   p.blocks = need < most ? need : most;
 
   // us: a call (between logits' and greedy's, so that both add up in the same order), and
-  // per k block the hidden's staging and a round of all waves: a fit to 754 timings
-  // (5..64 rows, V 2,000..248,320, H 512..8192; 4-9% rms).  The shape that it picks took
-  // 0.3% longer than the fastest on average, the widest one 53%.
+  // per k block the hidden's staging and a round of all waves: a fit to timings of every
+  // shape.  Over 175 greedy calls (1..256 rows, V 8,000..248,320, H 1024..8192) the shape that
+  // it picks took 0.5% longer than the fastest on average and 12% at most, the widest one 32%.
   struct Fit {
     float call, stage, round, staged;
   };
@@ -709,13 +711,15 @@ static int launch_w4_group(const W4Args& a, int group, const W4Plan& p, hipStrea
 }
 
 // The widest tile reads and unpacks the weights the fewest times; narrower ones leave more
-// of the hidden in LDS, and stage it sooner (up to 8 rows of H = 8192, V = 50,000: 43 us with
-// 8 rows' slots, 65 with 16; 64 rows, V = 32,000, H = 4096: 38 us with 16 rows a tile, 76 with
-// 64, staged) and give a small vocabulary's tiles to more blocks (32 rows, V = 8000, H = 1024: 5.7 us
-// with 16 rows, 7.5 with 32), but a large one costs more with them (64 rows, V = 248,320, H =
-// 1024: 70 us with 16, 49 with 64).  f32: the terms apart where the hidden stays in LDS so
-// (16 rows, V = 248,320, H = 1024: 36 us, 67 in fours), rows in fours where not (V = 8000, H =
-// 4096: 16 us, 63 staged); two tiles of three terms were no faster than two groups of one.
+// of the hidden in LDS, and stage it sooner (us a call, its host time of some 9 among
+// them: 8 rows, V = 50,000, H = 8192: 46 with 8 rows' slots, 68 with 16; 64 rows, V = 32,000, H =
+// 4096: 41 with 16 rows a tile, 74 with 64, staged) and give a small vocabulary's tiles to more
+// blocks (48 rows, V = 8000, H = 1024: 11 with 16 rows, 22 with 64), but a large one costs more with
+// them (64 rows, V = 248,320, H = 1024: 70 with 16, 55 with 64).  f32: the terms apart where the
+// hidden stays in LDS so (16 rows, V = 248,320, H = 1024: 39, 75 in fours; 64 rows 107, 249 in
+// fours), rows in fours where not (16 rows, V = 8000, H = 4096: 21, 65 staged).  Every group of 16
+// f32 rows unpacks the weights again (V = 128,256, H = 2048: 16 / 32 / 64 / 128 rows 45 / 71 / 127 /
+// 236 us); two tiles of three terms were no faster than two groups of one.
 template <int FMT, int TERMS, int MODE>
 static int w4_pass(const W4Args& a, int group, hipStream_t s) {
   if constexpr (TERMS == 3) {
