@@ -348,6 +348,37 @@ int nvjsel_reorder_states(const nvjsel_state* states, int count, const int32_t* 
                           const int32_t* slots, const int32_t* lengths, int batch, int beams, void* stream);
 
 /*
+ * Log probabilities of given tokens (no counterpart in the reference): for every row of
+ * logits [rows, vocab] (row_stride elements apart),
+ *   out_logprobs[n] = log_softmax(logits[n])[tokens[n]],
+ *   out_entropy[n] (nullable) = -sum_v p[v] ln p[v],
+ *   out_top, out_top_ids [rows, num_top]: the num_top (0..64) likeliest tokens' log
+ *     probabilities, the best first, equal ones by token.
+ * tokens int32 or int64 (token_bytes 4 or 8); one outside 0..vocab-1 asks for nothing and
+ * gets 0.  Logits of -inf have no probability and are no alternatives: where fewer than
+ * num_top are left, the rest is -inf with token -1; a row with nothing left gets -inf,
+ * entropy 0.  A NaN or +inf in a row makes its results NaN, its alternatives the first
+ * tokens.  out_stats (nullable) f32 [rows, 3]: what the gradient needs of a row.  vocab at
+ * most 2^26, rows 2^23.  Workspace: its first 16 KB zero at rest, the rest scratch.
+ */
+size_t nvjsel_token_logprobs_workspace_size(int dtype, int64_t rows, int vocab, int num_top);
+int nvjsel_token_logprobs(const void* logits, int dtype, int64_t rows, int vocab, int64_t row_stride,
+                          const void* tokens, int token_bytes, int num_top, float* out_logprobs, float* out_entropy,
+                          float* out_top, int32_t* out_top_ids, float* out_stats, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * Its gradient: out_grad [rows, vocab] of the logits' type (out_row_stride elements apart) =
+ *   g (1[v = token] - p[v]) - h p[v] (ln p[v] + entropy)
+ * with g = grad_logprobs[n] and h = grad_entropy[n] (either nullable, not both; with
+ * grad_entropy the stats are of a call that asked for the entropy).  A row without a
+ * gradient (g of no token and h 0), or with nothing left, gets zeros and is not read.
+ */
+int nvjsel_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int vocab, int64_t row_stride,
+                               const void* tokens, int token_bytes, const float* stats, const float* grad_logprobs,
+                               const float* grad_entropy, void* out_grad, int64_t out_row_stride, void* stream);
+
+/*
  * Diagnostic (no counterpart in the reference): the Gumbel draw of every
  * 23-bit uniform mantissa m in [first, first + n), i.e. random bits
  * (m << 9), two ways -- fast[i] with the hardware fp32 log the kernels use to

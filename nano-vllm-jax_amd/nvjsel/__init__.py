@@ -6,6 +6,7 @@ and tests do this).  The compute lives in ``libnvjsel.so`` (HIP, gfx950); see
 """
 from ._lib import NativeLibraryMissing, NvjselError, load
 from .beam import beam_search_select, lm_head_beam_search_step, reorder_beam_states
+from .logprobs import TokenLogprobs, token_logprobs
 from .registry import (
     KernelBackendUnavailable,
     available_backends,
@@ -33,6 +34,7 @@ __all__ = [
     "NativeLibraryMissing",
     "NvjselError",
     "KernelBackendUnavailable",
+    "TokenLogprobs",
     "W4Weight",
     "available_backends",
     "beam_search_select",
@@ -55,5 +57,6 @@ __all__ = [
     "rms_norm_hip",
     "sample_token_ids",
     "select_token_selection_backend",
+    "token_logprobs",
     "topk_hip",
 ]

@@ -48,7 +48,9 @@ class _WorkspacePool:
     Each entry point leaves its workspace zero-filled when it returns, so a
     buffer is zeroed once at allocation and reused in stream order.  A captured call may hold
     a buffer for as long as its graph lives, so a larger one does not replace it but comes
-    beside it, at twice its size; beam search's, which no captured call takes, go."""
+    beside it, at twice its size; those that no captured call takes go."""
+
+    UNCAPTURED = ("beam", "logprobs")
 
     def __init__(self):
         self._bufs: dict = {}
@@ -64,7 +66,7 @@ class _WorkspacePool:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
                 size = max(nbytes, 4096)
-                if buf is not None and kind != "beam":
+                if buf is not None and kind not in self.UNCAPTURED:
                     self._held.append(buf)
                     size = max(size, 2 * buf.numel())
                 buf = torch.zeros(size, dtype=torch.uint8, device=device)

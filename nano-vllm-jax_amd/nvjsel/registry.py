@@ -75,6 +75,7 @@ _SPECS = {
             "lm_head_w4",
             "beam_search_select",
             "reorder_beam_states",
+            "token_logprobs",
         ),
         implemented=True,
         description="Hand-written HIP kernels for gfx950 behind the libnvjsel C ABI.",
