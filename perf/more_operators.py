@@ -248,7 +248,7 @@ def _plain_logits(s):
 
 
 def _plain_adapters(s):
-    out = s["base"].float()
+    out = s["base"].to(torch.float32, copy=True)  # fp32 base is not to be changed
     x = s["x"].float()
     for k in range(s["a"].shape[0]):
         of = (s["ids"] == k)[:, None]
