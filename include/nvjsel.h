@@ -379,6 +379,24 @@ int nvjsel_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int 
                                const float* grad_entropy, void* out_grad, int64_t out_row_stride, void* stream);
 
 /*
+ * Low-rank adapters beside a shared projection (no counterpart in the reference):
+ *   out[n] = base[n] + scales[a] (x[n] A_a^T) B_a^T,  a = ids[n];  base[n] where a is outside 0..count-1.
+ * x [rows, hidden] of x_dtype, base and out [rows, width] of out_dtype (rows their strides
+ * apart, out of at least width; out = base for in place, else they share no memory).  Tables of
+ * bf16 or f16, 16-byte aligned: a_table [count, rank, hidden rounded up to 32] and b_table
+ * [count, width, rank], zeros behind an adapter's own sizes, rank 8, 16 or a multiple of 32 up to
+ * 512; scales f32, ids int32.  fp32 sums, out rounded once.  A NaN or an infinity in a row of x or in
+ * its adapter makes that row NaN and no other.  rows at most 2^20, hidden 2^24, width 2^28.
+ * Workspace: scratch (16-byte aligned).
+ */
+size_t nvjsel_adapters_workspace_size(int table_dtype, int64_t rows, int rank);
+int nvjsel_apply_adapters(const void* x, int x_dtype, int64_t x_stride, const void* base, int out_dtype,
+                          int64_t base_stride, const void* a_table, const void* b_table, int table_dtype,
+                          const float* scales, int count, int rank, int hidden, int width, const int32_t* ids,
+                          int64_t rows, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
  * Diagnostic (no counterpart in the reference): the Gumbel draw of every
  * 23-bit uniform mantissa m in [first, first + n), i.e. random bits
  * (m << 9), two ways -- fast[i] with the hardware fp32 log the kernels use to

@@ -5,8 +5,9 @@ and tests do this).  The compute lives in ``libnvjsel.so`` (HIP, gfx950); see
 ``include/nvjsel.h`` for the C ABI.
 """
 from ._lib import NativeLibraryMissing, NvjselError, load
+from .adapters import AdapterTable, apply_adapters, pack_adapters
 from .beam import beam_search_select, lm_head_beam_search_step, reorder_beam_states
-from .logprobs import TokenLogprobs, token_logprobs
+from .logprobs import TokenLogprobs, lm_head_token_logprobs, token_logprobs
 from .registry import (
     KernelBackendUnavailable,
     available_backends,
@@ -31,11 +32,13 @@ from .selection import (
 from .w4 import W4Weight, pack_lm_head_w4, quantize_lm_head_w4
 
 __all__ = [
+    "AdapterTable",
     "NativeLibraryMissing",
     "NvjselError",
     "KernelBackendUnavailable",
     "TokenLogprobs",
     "W4Weight",
+    "apply_adapters",
     "available_backends",
     "beam_search_select",
     "derive_rng_keys",
@@ -47,8 +50,10 @@ __all__ = [
     "lm_head_logits_hip",
     "lm_head_sample_token_ids",
     "lm_head_token_ids_and_topk",
+    "lm_head_token_logprobs",
     "mtp_greedy_top1_token_ids",
     "mtp_lm_head_greedy_top1_impl",
+    "pack_adapters",
     "pack_lm_head_w4",
     "quantize_lm_head_w4",
     "reference_reduce_cast",

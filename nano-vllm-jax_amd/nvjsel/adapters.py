@@ -1,0 +1,158 @@
+"""Low-rank adapters of many requests at once beside a shared projection.
+
+``out[n] = base[n] + scales[a] * (x[n] @ A[a].T) @ B[a].T`` with ``a = adapter_ids[n]``, and
+``base[n]`` alone where that names no adapter.  ``pack_adapters`` lays the adapters out once,
+when they are loaded; the ``AdapterTable`` it returns is also taken by
+``lm_head_logits_hip``, ``lm_head_sample_token_ids``, ``lm_head_token_ids_and_topk`` and
+``lm_head_token_logprobs``, where the projection is the LM head.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._tensors import _TORCH_DTYPES, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
+
+MAX_RANK = 512
+MAX_ROWS = 1 << 20
+_TABLE_DTYPES = (torch.bfloat16, torch.float16)
+
+
+@dataclass(frozen=True)
+class AdapterTable:
+    """Adapters laid out for the kernels: ``rank`` and ``a``'s last dimension rounded up, zeros behind."""
+
+    a: torch.Tensor  # [count, rank, hidden rounded up to 32]
+    b: torch.Tensor  # [count, width, rank]
+    scales: torch.Tensor  # f32 [count]
+    hidden: int
+    width: int
+
+    @property
+    def count(self) -> int:
+        return int(self.a.shape[0])
+
+    @property
+    def rank(self) -> int:
+        return int(self.a.shape[1])
+
+
+def _no_gradient(who: str, *ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError(f"{who} is not differentiable: call it under torch.no_grad() or on detached tensors")
+
+
+def pack_adapters(a, b, scales=None) -> AdapterTable:
+    """Lay out ``a`` (``[L, R, H]``, or one ``[R_i, H]`` per adapter) and ``b`` (``[L, D, R]``, or one
+    ``[D, R_i]`` each) of bf16 or f16 for the kernels: a copy; the plain form may go.
+
+    ``scales`` (f32 ``[L]`` or numbers; 1 where None) multiply the adapters' parts, ``alpha / R`` as
+    a rule.  Ranks may differ, up to 512."""
+    a, b = list(a), list(b)
+    if not a or len(a) != len(b):
+        raise ValueError("pack_adapters takes one a and one b for every adapter, at least one")
+    if any(t.ndim != 2 for t in a + b):
+        raise ValueError("an adapter is a [R, H] and b [D, R]")
+    hidden, width = int(a[0].shape[1]), int(b[0].shape[0])
+    if hidden == 0 or width == 0 or any(t.shape[0] == 0 for t in a):
+        raise ValueError("pack_adapters requires non-empty dimensions")
+    if any(t.shape[1] != hidden for t in a) or any(t.shape[0] != width for t in b):
+        raise ValueError("all adapters of a table have one hidden size and one width")
+    if any(s.shape[0] != t.shape[1] for s, t in zip(a, b)):
+        raise ValueError("a's and b's ranks must match")
+    dtype = a[0].dtype
+    if dtype not in _TABLE_DTYPES or any(t.dtype != dtype for t in a + b):
+        raise ValueError("adapters must be bfloat16 or float16, a and b alike")
+    most = max(int(t.shape[0]) for t in a)
+    if most > MAX_RANK:
+        raise ValueError(f"ranks must be at most {MAX_RANK} (got {most})")
+    if hidden > 1 << 24 or width > 1 << 28:
+        raise ValueError("hidden must be at most 2^24 and width 2^28")
+    dev = _require_cuda(*a, *b)
+    rank = 8 if most <= 8 else 16 if most <= 16 else (most + 31) // 32 * 32
+    with torch.no_grad():
+        pa = torch.zeros((len(a), rank, (hidden + 31) // 32 * 32), dtype=dtype, device=dev)
+        pb = torch.zeros((len(b), width, rank), dtype=dtype, device=dev)
+        for i, (s, t) in enumerate(zip(a, b)):
+            pa[i, : s.shape[0], :hidden] = s
+            pb[i, :, : t.shape[1]] = t
+        if scales is None:
+            ps = torch.ones((len(a),), dtype=torch.float32, device=dev)
+        else:
+            ps = torch.as_tensor(scales, dtype=torch.float32, device=dev).detach().reshape(-1).clone()
+            if ps.numel() != len(a):
+                raise ValueError("scales must have one value for every adapter")
+    return AdapterTable(pa, pb, ps, hidden, width)
+
+
+def _rows(t: torch.Tensor, rows: int) -> torch.Tensor:
+    """``[rows, D]`` with unit column stride, a copy where a view cannot be."""
+    t = t if t.ndim == 2 else t.reshape(rows, t.shape[-1])
+    return t.contiguous() if t.stride(1) != 1 and t.shape[1] > 1 else t
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _meet(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether two [rows, D] tensors may share memory."""
+    size = s.element_size()
+    first, other = sorted((s, t), key=lambda u: u.data_ptr())
+    apart = other.data_ptr() - first.data_ptr()
+    pitch, width = _stride(first) * size, first.shape[1] * size
+    if apart >= (first.shape[0] - 1) * pitch + width:
+        return False
+    side_by_side = pitch == _stride(other) * size and pitch > 0
+    return not (side_by_side and width <= apart % pitch <= pitch - width)
+
+
+def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, adapter_ids: torch.Tensor, *,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``base`` with every row's own adapter added: ``base + scale (x A^T) B^T``.
+
+    ``x [..., H]`` are the projection's inputs and ``base [..., D]`` its outputs (f32, bf16 or
+    f16 each, rows with unit stride as they lie), ``adapter_ids`` int32 of the shape before H, one
+    outside 0..L-1 (the -1 of a row without an adapter) leaves its row as it is.  Any order and
+    mixture of adapters.  Sums are fp32; the result, of ``base``'s type, is rounded once.
+    ``out`` receives it (``base`` itself for in place), a new tensor where None.  A NaN or an infinity
+    in a row of ``x``, or in its own adapter, makes that row's results NaN and no other's.
+    Not differentiable."""
+    if x.ndim < 1 or base.ndim != x.ndim or x.shape[:-1] != base.shape[:-1] or adapter_ids.shape != x.shape[:-1]:
+        raise ValueError("apply_adapters takes x [..., H], base [..., D] and one adapter id for every row")
+    if x.numel() == 0 or base.numel() == 0:
+        raise ValueError("apply_adapters requires non-empty dimensions")
+    if x.shape[-1] != adapters.hidden or base.shape[-1] != adapters.width:
+        raise ValueError(f"the adapters are of hidden {adapters.hidden} and width {adapters.width} "
+                         f"(got {x.shape[-1]} and {base.shape[-1]})")
+    xd, od = _dtype_code(x, "x"), _dtype_code(base, "base")
+    if adapter_ids.dtype != torch.int32:
+        raise ValueError(f"adapter_ids must be int32 (got {adapter_ids.dtype})")
+    rows = adapter_ids.numel()
+    if rows > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows (got {rows})")
+    if out is not None and (out.shape != base.shape or out.dtype != base.dtype):
+        raise ValueError("out must have base's shape and type")
+    _no_gradient("apply_adapters", x, base, out, adapters.a, adapters.b, adapters.scales)
+    dev = _require_cuda(x, base, adapters.a, adapters.b, adapters.scales, adapter_ids, out)
+    result = torch.empty(base.shape, dtype=base.dtype, device=dev) if out is None else out
+    try:
+        flat = result.view(rows, adapters.width)
+    except RuntimeError:
+        raise ValueError("out's rows must be apart by one stride") from None
+    if (flat.stride(1) != 1 and adapters.width > 1) or _stride(flat) < adapters.width:
+        raise ValueError("out's rows must be contiguous and must not overlap")
+    x, base, ids = _rows(x, rows), _rows(base, rows), adapter_ids.reshape(rows).contiguous()
+    if out is not None and (base.data_ptr(), _stride(base)) != (flat.data_ptr(), _stride(flat)) and _meet(base, flat):
+        raise ValueError("out must be base itself or share no memory with it")
+    with _on_device(dev):
+        nbytes = _lib.load().nvjsel_adapters_workspace_size(_TORCH_DTYPES[adapters.a.dtype], rows, adapters.rank)
+        stream = _stream_handle(dev)
+        ws = _workspace(dev, stream, "adapters", nbytes, 0)
+        _lib.call("nvjsel_apply_adapters", x.data_ptr(), xd, _stride(x), base.data_ptr(), od, _stride(base),
+                  adapters.a.data_ptr(), adapters.b.data_ptr(), _TORCH_DTYPES[adapters.a.dtype],
+                  adapters.scales.data_ptr(), adapters.count, adapters.rank, adapters.hidden, adapters.width,
+                  ids.data_ptr(), rows, flat.data_ptr(), _stride(flat), ws.data_ptr(), nbytes, stream)
+    return result

@@ -1,5 +1,5 @@
-"""Log probabilities of given tokens, with entropies and top alternatives, and
-their gradient."""
+"""Log probabilities of given tokens, with entropies and top alternatives: over
+logits, with their gradient, and from the hidden states."""
 from __future__ import annotations
 
 from functools import lru_cache
@@ -8,6 +8,9 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from .adapters import AdapterTable, _no_gradient
+from .selection import _adapter_ids, _flatten_hidden, _normed, lm_head_logits_hip
+from .w4 import W4Weight
 from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
 
 MAX_TOP = 64  # alternatives of a row
@@ -133,3 +136,48 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
         if top is not None:
             top, ids = top.reshape(*shape, num_top), ids.reshape(*shape, num_top)
     return TokenLogprobs(lp, ent, top, ids)
+
+
+_LOGIT_BYTES = 1 << 28  # of logits that are formed at a time
+
+
+def lm_head_token_logprobs(hidden: torch.Tensor, output_weight, tokens: torch.Tensor, *, num_top: int = 0,
+                           entropy: bool = False, weight_layout: str | None = None, reduce_cast: int | None = None,
+                           norm_weight: torch.Tensor | None = None, rms_norm_eps: float = 1e-6,
+                           act_dtype: torch.dtype = torch.float32, adapters: AdapterTable | None = None,
+                           adapter_ids: torch.Tensor | None = None) -> TokenLogprobs:
+    """``token_logprobs`` of the LM head's logits, from the hidden states: the score of a prompt or a draft.
+
+    ``hidden [..., H]``, ``tokens`` int32 or int64 of the shape before H; ``output_weight``,
+    ``weight_layout``, ``reduce_cast``, ``adapters`` and ``adapter_ids`` (one for every row) as in ``lm_head_logits_hip``, whose logits'
+    log probabilities these are; ``norm_weight``: pre-norm hidden, as in ``lm_head_greedy_top1_hip``.
+    The logits are formed for some rows at a time and never kept.  Not differentiable."""
+    if hidden.ndim < 1 or tokens.shape != hidden.shape[:-1]:
+        raise ValueError("lm_head_token_logprobs takes hidden [..., H] and one token for every row")
+    if hidden.numel() == 0:
+        raise ValueError("LM-head log probabilities require non-empty dimensions")
+    if not 0 <= int(num_top) <= MAX_TOP:
+        raise ValueError(f"num_top must be in 0..{MAX_TOP} (got {num_top})")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tokens must be int32 or int64 (got {tokens.dtype})")
+    weight = output_weight.packed if isinstance(output_weight, W4Weight) else output_weight
+    _no_gradient("lm_head_token_logprobs", hidden, weight, norm_weight)
+    shape, rows = tokens.shape, tokens.numel()
+    x = hidden.reshape(rows, hidden.shape[-1])
+    tokens = tokens.reshape(rows)
+    dev = _require_cuda(x, tokens)
+    if adapters is not None:
+        adapter_ids = _adapter_ids(adapter_ids, x)
+    with _on_device(dev):
+        if norm_weight is not None:
+            x = _normed(x, norm_weight, rms_norm_eps, act_dtype)
+        vocab = output_weight.vocab if isinstance(output_weight, W4Weight) else max(output_weight.shape)
+        step = max(64, _LOGIT_BYTES // (4 * vocab) // 64 * 64)
+        parts = []
+        for i in range(0, rows, step):
+            logits = lm_head_logits_hip(x[i:i + step], output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
+                                        adapters=adapters,
+                                        adapter_ids=None if adapters is None else adapter_ids[i:i + step])
+            parts.append(token_logprobs(logits, tokens[i:i + step], num_top=num_top, entropy=entropy))
+    r = [None if p[0] is None else p[0] if len(parts) == 1 else torch.cat(p) for p in zip(*parts)]
+    return TokenLogprobs(*(t if t is None else t.reshape(*shape, *t.shape[1:]) for t in r))

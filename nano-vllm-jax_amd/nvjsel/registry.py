@@ -76,6 +76,8 @@ _SPECS = {
             "beam_search_select",
             "reorder_beam_states",
             "token_logprobs",
+            "lm_head_token_logprobs",
+            "apply_adapters",
         ),
         implemented=True,
         description="Hand-written HIP kernels for gfx950 behind the libnvjsel C ABI.",

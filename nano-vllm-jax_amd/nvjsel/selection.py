@@ -25,6 +25,7 @@ import torch
 
 from . import _lib
 from ._tensors import _TORCH_DTYPES, _WS, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
+from .adapters import AdapterTable, apply_adapters
 from .w4 import W4Weight, w4_greedy as _w4_greedy, w4_logits as _w4_logits
 
 
@@ -215,18 +216,26 @@ def lm_head_sample_token_ids(hidden_norm: torch.Tensor, output_weight: torch.Ten
                              weight_layout: str | None = None,
                              reduce_cast: int | None = None, norm_weight: torch.Tensor | None = None,
                              rms_norm_eps: float = 1e-6,
-                             act_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+                             act_dtype: torch.dtype = torch.float32, adapters: AdapterTable | None = None,
+                             adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
     """Sample token ids from the LM head (model.py:901-938).
 
     Without top-k/top-p the projection and the Gumbel-max are fused and no
     logits are written.  With them, the logits are formed once by the
     library's LM-head kernels (rounded as the reference's dot) and handed to
     the sampler.
-    ``norm_weight`` selects the pre-norm input as in lm_head_greedy_top1_hip."""
+    ``norm_weight`` selects the pre-norm input as in lm_head_greedy_top1_hip.  With ``adapters`` and
+    ``adapter_ids`` the logits are formed as ``lm_head_logits_hip`` gives them."""
     x = _flatten_hidden(hidden_norm, require_3d=False)
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
     if batch <= 0 or hidden_dim <= 0:
         raise ValueError("LM-head sampling requires non-empty dimensions")
+    if adapters is not None:
+        x = x if norm_weight is None else _normed(x, norm_weight, rms_norm_eps, act_dtype)
+        logits = lm_head_logits_hip(x, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
+                                    adapters=adapters, adapter_ids=adapter_ids)
+        with _on_device(logits.device):
+            return _sample(logits, temperatures, rng_keys, top_k, top_p, None, _own_sampler_workspace)
     if isinstance(output_weight, W4Weight):
         x = x if norm_weight is None else _normed(x, norm_weight, rms_norm_eps, act_dtype)
         logits = _w4_logits(x, output_weight, weight_layout, reduce_cast)
@@ -284,12 +293,28 @@ def _dense_logits(x: torch.Tensor, w: torch.Tensor, layout: int, vocab: int, rc:
     return out
 
 
+def _adapter_ids(adapter_ids: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
+    if adapter_ids is None or adapter_ids.numel() != x.shape[0]:
+        raise ValueError("adapters need adapter_ids, one for every row")
+    return adapter_ids.reshape(-1)
+
+
 def lm_head_logits_hip(hidden_norm: torch.Tensor, output_weight: torch.Tensor, *,
-                       weight_layout: str | None = None, reduce_cast: int | None = None) -> torch.Tensor:
+                       weight_layout: str | None = None, reduce_cast: int | None = None,
+                       adapters: AdapterTable | None = None,
+                       adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
     """Dense LM-head logits ``[B, V]`` (``jnp.dot(hidden_norm, W)``,
     model.py:765-780): fp32 accumulation; bf16 x bf16 gives bf16 logits and f16 x f16 f16 logits (the
-    reference's dot output), other operand types f32 logits."""
+    reference's dot output), other operand types f32 logits.
+
+    With ``adapters`` and ``adapter_ids`` (int32 ``[B]``) every row's own adapter of the LM head is
+    added to them (``apply_adapters``, in place): 16-bit logits are rounded by the dot and once more by
+    the sum, ``reduce_cast=0`` keeps both in fp32."""
     x = _flatten_hidden(hidden_norm, require_3d=False)
+    if adapters is not None:
+        with _on_device(_require_cuda(x)):
+            logits = lm_head_logits_hip(x, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast)
+        return apply_adapters(x, logits, adapters, _adapter_ids(adapter_ids, x), out=logits)
     if isinstance(output_weight, W4Weight):
         return _w4_logits(x, output_weight, weight_layout, reduce_cast)
     batch, hidden_dim = int(x.shape[0]), int(x.shape[1])
@@ -386,7 +411,8 @@ def _topk(logits, k, workspace):
 def lm_head_token_ids_and_topk(hidden: torch.Tensor, output_weight: torch.Tensor, *, top_k: int = 0,
                                norm_weight: torch.Tensor | None = None, rms_norm_eps: float = 1e-6,
                                act_dtype: torch.dtype = torch.float32, weight_layout: str | None = None,
-                               reduce_cast: int | None = None):
+                               reduce_cast: int | None = None, adapters: AdapterTable | None = None,
+                               adapter_ids: torch.Tensor | None = None):
     """Greedy token ids and optional top-k of the LM head (model.py:833-898).
 
     ``hidden [B, W, H]`` (W > 1: MTP / verifier width, flattened to B*W rows as
@@ -394,13 +420,25 @@ def lm_head_token_ids_and_topk(hidden: torch.Tensor, output_weight: torch.Tensor
     ``top_k == 0``: the fused greedy route, returns ``(ids int32[B, W], None,
     None)``.  ``top_k > 0``: dense logits (the reference's dot: bf16 x bf16
     rounds to bf16) and ``topk_hip``; returns ``(ids, values f32[B, W, k],
-    indices int32[B, W, k])`` with ``ids = indices[..., 0]``, the argmax."""
+    indices int32[B, W, k])`` with ``ids = indices[..., 0]``, the argmax.  With ``adapters`` and
+    ``adapter_ids`` (int32, ``[B * W]`` or ``[B, W]``) dense logits as ``lm_head_logits_hip`` gives them, for ``top_k ==
+    0`` too."""
     if hidden.ndim == 2:
         hidden = hidden[:, None, :]
     if hidden.ndim != 3:
         raise ValueError("hidden must be [B, W, H] or [B, H]")
     batch, width, hidden_dim = (int(d) for d in hidden.shape)
     flat = hidden.reshape(batch * width, hidden_dim)
+    if adapters is not None:
+        x = flat if norm_weight is None else _normed(flat, norm_weight, rms_norm_eps, act_dtype)
+        logits = lm_head_logits_hip(x, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
+                                    adapters=adapters, adapter_ids=adapter_ids)
+        with _on_device(logits.device):
+            values, indices = _topk(logits, max(int(top_k), 1), _own_sampler_workspace)
+        ids = indices[:, 0].reshape(batch, width)
+        if int(top_k) == 0:
+            return ids, None, None
+        return ids, values.reshape(batch, width, -1), indices.reshape(batch, width, -1)
     if int(top_k) == 0:
         ids = lm_head_greedy_top1_hip(flat, output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
                                       norm_weight=norm_weight, rms_norm_eps=rms_norm_eps, act_dtype=act_dtype)
