@@ -379,6 +379,19 @@ int nvjsel_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int 
                                const float* grad_entropy, void* out_grad, int64_t out_row_stride, void* stream);
 
 /*
+ * nvjsel_token_logprobs of the LM head's logits hidden [rows, hidden_dim] x weight, rounded by
+ * reduce_cast, which are not written: 16-bit weights [V, H] (hidden_dim a multiple of 64, hidden and
+ * weight 16-byte aligned), hidden of their type, or f32 beside bf16; other calls return
+ * NVJSEL_EUNSUPPORTED (the query 0).  rows at most 2^23.  Workspace: scratch (16-byte aligned).
+ */
+size_t nvjsel_lm_head_token_logprobs_workspace_size(int hidden_dtype, int weight_dtype, int weight_layout, int64_t rows,
+                                                    int hidden_dim, int vocab);
+int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtype, const void* weight, int weight_dtype,
+                                  int weight_layout, int64_t rows, int hidden_dim, int vocab, int reduce_cast,
+                                  const void* tokens, int token_bytes, float* out_logprobs, float* out_entropy,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Low-rank adapters beside a shared projection (no counterpart in the reference):
  *   out[n] = base[n] + scales[a] (x[n] A_a^T) B_a^T,  a = ids[n];  base[n] where a is outside 0..count-1.
  * x [rows, hidden] of x_dtype, base and out [rows, width] of out_dtype (rows their strides

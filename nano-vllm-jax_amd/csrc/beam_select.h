@@ -411,7 +411,7 @@ __device__ __forceinline__ void beam_token(const BeamArgs& a, const BeamJoinLds<
   }
   r.sum = wave_sum_f64(r.sum);
   if constexpr (LP == LP_ENTROPY) r.ent = wave_sum_f64(r.ent);
-  if (tid == 0) row_answer<DT>(a.answers, a.logits, (int64_t)row * a.batch_stride, a.vocab, row, m, r);
+  if (tid == 0) row_answer_from<DT>(a.answers, a.logits, (int64_t)row * a.batch_stride, a.vocab, row, m, r);
 }
 
 template <int DT, int LISTS, int THREADS, bool ONE, int LP>

@@ -1,0 +1,173 @@
+// Log probabilities of given tokens from the hidden states: the staged GEMM of
+// lm_head_ring.h, whose tiles end in sums of exponentials instead of logits.
+//
+//   l[n, v] = x[n] . W[v],   logprob = (l[n, t] - m) - ln S,   entropy = ln S - T / S   (row_sums.h)
+//
+// The logits never leave the registers: 2048 rows of 248,320 would be 1 GB written and read
+// (bf16; 2 GB f32) beside a product of 1.04 TFLOP.  A lane holds 16 logits of one column (batch row) per
+// 32-row tile, so that the sums cross no lanes until a block's share of the vocabulary
+// ends; a share's parts are joined by a second kernel, a wave a row.
+#include "lm_head_ring.h"
+
+namespace nvjsel {
+
+__global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, const float* token_logits, const RowPart* parts,
+                                                           int rows, int shares, int vocab) {
+  const int row = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  if (row >= rows) return;
+  const RowPart* p = parts + (size_t)row * shares;
+  float m = -INFINITY;
+  for (int i = lane; i < shares; i += 64) m = fmaxf(m, p[i].max);
+  m = wave_max_f32(m);
+  RowSum r{0.0, 0.0};
+  for (int i = lane; i < shares; i += 64) row_join(r, RowSum{p[i].sum, p[i].ent}, p[i].max, m);
+  r.sum = wave_sum_f64(r.sum);
+  r.ent = wave_sum_f64(r.ent);
+  if (lane != 0) return;
+  const int64_t t = row_token(answers, row);
+  const bool asked = t >= 0 && t < vocab;
+  row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r);
+}
+
+// Rows of a block: 256 while more than 128 are left (64 of f32 activations, three products each).
+static int score_block_rows(bool f32, int64_t left) {
+  if (f32) return left > 32 ? 64 : 32;
+  return left > 128 ? 256 : left > 64 ? 128 : left > 32 ? 64 : 32;
+}
+
+// Row blocks of a launch: as many of those left as give the most rows per round of tiles, where
+// every CU has one block (5 of 51 shares each fill 255 CUs, 29 of 8 fill 232, 16 and 13 256 and 247);
+// a launch costs about as much as half a tile.
+static int score_row_blocks(int64_t left, int vocab, int cus) {
+  int best = 1;
+  double most = 0.0;
+  for (int r = 1; r <= 32 && r <= left && r <= cus; ++r) {
+    const double rate = r / (0.5 + ring_tiles(ring_share(vocab, cus / r)));
+    if (rate >= most) {
+      most = rate;
+      best = r;
+    }
+  }
+  return best;
+}
+
+static size_t score_bytes(int64_t rows, int cus) {  // parts: at most `cus` shares x row blocks of 256 rows
+  return align_up((size_t)rows * 4, 16) + (size_t)cus * 256 * sizeof(RowPart);
+}
+
+template <int WT, int MODE, int NBR, int NS>
+static int launch_score_rows(const LmArgs& a, ScoreArgs sc, const RowAnswers& answers, hipStream_t s) {
+  const int rows = ring_share(a.V, device_cu_count() / sc.row_blocks);
+  sc.shares = (a.V + rows - 1) / rows;
+  hipLaunchKernelGGL((lm_head_ring_kernel<WT, MODE, NBR, NS>), dim3((unsigned)(sc.shares * sc.row_blocks)),
+                     dim3(RingShape<MODE, NBR, NS>::NW * 64), 0, s, a, rows, sc);
+  NVJSEL_CHECK_LAUNCH("lm_head_ring_kernel");
+  hipLaunchKernelGGL(score_finish_kernel, dim3((unsigned)((a.B + 3) / 4)), dim3(256), 0, s, answers,
+                     (const float*)sc.token_logits, (const RowPart*)sc.parts, a.B, sc.shares, a.V);
+  NVJSEL_CHECK_LAUNCH("score_finish_kernel");
+  return NVJSEL_OK;
+}
+
+template <int MODE>
+static int launch_score(const LmArgs& a, const ScoreArgs& sc, const RowAnswers& w, int block_rows, hipStream_t s) {
+  if (a.hidden_dtype == DT_F32) {
+    if (block_rows == 32) return launch_score_rows<DT_BF16, MODE, 32, 3>(a, sc, w, s);
+    return launch_score_rows<DT_BF16, MODE, 64, 3>(a, sc, w, s);
+  }
+  auto by_rows = [&](auto T) -> int {
+    constexpr int WT = decltype(T)::value;
+    if (block_rows == 32) return launch_score_rows<WT, MODE, 32, 1>(a, sc, w, s);
+    if (block_rows == 64) return launch_score_rows<WT, MODE, 64, 1>(a, sc, w, s);
+    if (block_rows == 128) return launch_score_rows<WT, MODE, 128, 1>(a, sc, w, s);
+    return launch_score_rows<WT, MODE, 256, 1>(a, sc, w, s);
+  };
+  if (a.weight_dtype == DT_F16) return by_rows(std::integral_constant<int, DT_F16>{});
+  return by_rows(std::integral_constant<int, DT_BF16>{});
+}
+
+}  // namespace nvjsel
+
+using namespace nvjsel;
+
+static int score_check(int hidden_dtype, int weight_dtype, int layout, int64_t rows, int H, int V) {
+  if (rows <= 0 || H <= 0 || V <= 0) {
+    set_error("lm_head_token_logprobs requires non-empty dimensions (rows=%lld hidden=%d vocab=%d)", (long long)rows, H, V);
+    return NVJSEL_EINVAL;
+  }
+  if (!valid_dtype(hidden_dtype) || !valid_dtype(weight_dtype)) {
+    set_error("lm_head_token_logprobs: unsupported dtype (hidden=%d weight=%d)", hidden_dtype, weight_dtype);
+    return NVJSEL_EINVAL;
+  }
+  if (layout != NVJSEL_W_VH && layout != NVJSEL_W_HV) {
+    set_error("lm_head_token_logprobs: bad weight layout %d", layout);
+    return NVJSEL_EINVAL;
+  }
+  if (rows > 1 << 23) return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: at most 2^23 rows");
+  const bool types = weight_dtype != NVJSEL_F32 && (hidden_dtype == weight_dtype ||
+                                                    (hidden_dtype == NVJSEL_F32 && weight_dtype == NVJSEL_BF16));
+  if (layout != NVJSEL_W_VH || !types || H % kRingKC != 0 || H > (1 << 20) || V >= 0x7FFFFF00) {
+    set_error("lm_head_token_logprobs: takes a 16-bit weight [V, H], H a multiple of 64, hidden of its type or f32 beside bf16");
+    return NVJSEL_EUNSUPPORTED;
+  }
+  return NVJSEL_OK;
+}
+
+extern "C" size_t nvjsel_lm_head_token_logprobs_workspace_size(int hidden_dtype, int weight_dtype, int weight_layout,
+                                                               int64_t rows, int hidden_dim, int vocab) {
+  clear_error();
+  if (score_check(hidden_dtype, weight_dtype, weight_layout, rows, hidden_dim, vocab) != NVJSEL_OK) return 0;
+  return score_bytes(rows, device_cu_count());
+}
+
+extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtype, const void* weight, int weight_dtype,
+                                             int weight_layout, int64_t rows, int hidden_dim, int vocab, int reduce_cast,
+                                             const void* tokens, int token_bytes, float* out_logprobs, float* out_entropy,
+                                             void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const int rc = score_check(hidden_dtype, weight_dtype, weight_layout, rows, hidden_dim, vocab);
+  if (rc != NVJSEL_OK) return rc;
+  if (!hidden || !weight || !tokens || !out_logprobs) return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: null pointer");
+  if (reduce_cast < 0 || reduce_cast > 2) return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: reduce_cast must be 0, 1 or 2");
+  if ((token_bytes != 4 && token_bytes != 8) || ((uintptr_t)tokens & (token_bytes - 1)))
+    return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: tokens must be int32 or int64, aligned");
+  if ((((uintptr_t)hidden) | ((uintptr_t)weight)) & 15)
+    return fail(NVJSEL_EUNSUPPORTED, "lm_head_token_logprobs: hidden and weight must be 16-byte aligned");
+  const int cus = device_cu_count();
+  const size_t need = score_bytes(rows, cus);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+    set_error("lm_head_token_logprobs: workspace %zu bytes (16-byte aligned) < required %zu", workspace_bytes, need);
+    return NVJSEL_EWORKSPACE;
+  }
+  std::lock_guard<std::mutex> lock(launch_mutex());
+  hipStream_t s = (hipStream_t)stream;
+  int64_t n = 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += n) {
+    const int64_t left = rows - r0;
+    const int block_rows = score_block_rows(hidden_dtype == NVJSEL_F32, left);
+    ScoreArgs sc{};
+    // a last block that a smaller shape takes is left to the next launch
+    const int64_t blocks = block_rows == 256 ? (left + 127) / 256 : (left + block_rows - 1) / block_rows;
+    sc.row_blocks = score_row_blocks(blocks, vocab, cus);
+    n = (int64_t)sc.row_blocks * block_rows < left ? (int64_t)sc.row_blocks * block_rows : left;
+    sc.tokens = (const char*)tokens + r0 * token_bytes;
+    sc.token64 = token_bytes == 8;
+    sc.token_logits = (float*)workspace + r0;
+    sc.parts = (RowPart*)((char*)workspace + align_up((size_t)rows * 4, 16));
+    LmArgs a{};
+    a.W = weight;
+    a.hidden = (const char*)hidden + (size_t)r0 * hidden_dim * dtype_size(hidden_dtype);
+    a.hidden_dtype = hidden_dtype;
+    a.act_dtype = hidden_dtype;
+    a.weight_dtype = weight_dtype;
+    a.layout = weight_layout;
+    a.B = (int)n;
+    a.H = hidden_dim;
+    a.V = vocab;
+    a.reduce_cast = reduce_cast;
+    const RowAnswers answers{sc.tokens, sc.token64, out_logprobs + r0, out_entropy ? out_entropy + r0 : nullptr, nullptr};
+    const int st = out_entropy ? launch_score<MODE_SCORE_ENTROPY>(a, sc, answers, block_rows, s)
+                               : launch_score<MODE_SCORE>(a, sc, answers, block_rows, s);
+    if (st != NVJSEL_OK) return st;
+  }
+  return NVJSEL_OK;
+}

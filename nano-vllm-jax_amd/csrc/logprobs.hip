@@ -21,12 +21,6 @@ static constexpr int kRowTickets = 4096;                 // rows of several bloc
 static constexpr int64_t kTopRows = 8192;                // rows of one scan and join
 static constexpr int64_t kLaunchBlocks = 1 << 23;        // of 256 threads: a launch has less than 2^32
 
-struct RowPart {  // of one block's share of a row
-  double sum, ent;
-  float max;
-  int pad;
-};
-
 struct RowArgs {
   const void* logits;
   int vocab;
@@ -107,7 +101,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_sums_kernel(RowArgs a) {
     for (int i = 0; i < kRowBlockWaves; ++i) row_join(r, RowSum{parts[i].sum, parts[i].ent}, parts[i].max, bm);
   }
   if (a.blocks == 1) {
-    if (tid == 0) row_answer<DT>(a.answers, a.logits, row * a.row_stride, a.vocab, row, bm, r);
+    if (tid == 0) row_answer_from<DT>(a.answers, a.logits, row * a.row_stride, a.vocab, row, bm, r);
     return;
   }
   if (tid == 0) {  // passed on at the device's coherence point, before the block's ticket is drawn
@@ -135,7 +129,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) row_sums_kernel(RowArgs a) {
   row_join(r, own, om, rm);
   r.sum = wave_sum_f64(r.sum);
   if constexpr (ENT) r.ent = wave_sum_f64(r.ent);
-  if (lane == 0) row_answer<DT>(a.answers, a.logits, row * a.row_stride, a.vocab, row, rm, r);
+  if (lane == 0) row_answer_from<DT>(a.answers, a.logits, row * a.row_stride, a.vocab, row, rm, r);
 }
 
 // ---------------------------------------------------------------- the gradient

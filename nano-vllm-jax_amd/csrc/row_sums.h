@@ -125,6 +125,11 @@ __device__ __forceinline__ row_u32x4 row_piece(const char* base, int o, int e1) 
 struct RowSum {
   double sum, ent;
 };
+struct RowPart {  // with its maximum, as parts of a row are passed on
+  double sum, ent;
+  float max;
+  int pad;
+};
 
 // Adds V pieces per lane, whose maximum is x, to the lane's sums.  Relative to 2^ref,
 // with y = l log2 e - ref: sum of 2^y, ent of 2^y y; both move to another reference by
@@ -219,19 +224,13 @@ __device__ __forceinline__ void row_join(RowSum& r, const RowSum& part, float ma
   r.sum += f * part.sum;
 }
 
-// logprob = (l[t] - m) - ln S, entropy = ln S - T / S (r: S and T, relative to m).  Nothing
-// left: -inf and 0; NaN or +inf among the logits: NaN; a token outside 0..V-1, of a row
-// that asks for none: 0.
-template <int DT>
-__device__ __forceinline__ void row_answer(const RowAnswers& a, const void* logits, int64_t at, int vocab, int64_t row,
-                                           float m, const RowSum& r) {
+// logprob = (x - m) - ln S for the token's logit x, entropy = ln S - T / S (r: S and T,
+// relative to m).  Nothing left: -inf and 0; NaN or +inf among the logits: NaN; a row that
+// asks for no token: 0.
+__device__ __forceinline__ void row_answer(const RowAnswers& a, int64_t row, bool asked, float x, float m, const RowSum& r) {
   const bool nan = !(r.sum < INFINITY), none = !nan && r.sum == 0.0;
   const double ls = nan ? (double)NAN : none ? 0.0 : log(r.sum);
-  const int64_t t = a.token64 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
-  float lp = 0.0f;
-  if (t >= 0 && t < vocab)
-    lp = nan ? NAN : none ? -INFINITY : (float)(((double)load_as_f32(logits, DT, (size_t)(at + t)) - (double)m) - ls);
-  a.logprobs[row] = lp;
+  a.logprobs[row] = !asked ? 0.0f : nan ? NAN : none ? -INFINITY : (float)(((double)x - (double)m) - ls);
   const double h = nan ? (double)NAN : none ? 0.0 : fmax(ls - r.ent / r.sum, 0.0);
   if (a.entropy) a.entropy[row] = (float)h;
   if (a.stats) {
@@ -239,6 +238,18 @@ __device__ __forceinline__ void row_answer(const RowAnswers& a, const void* logi
     a.stats[3 * row + 1] = (float)ls;
     a.stats[3 * row + 2] = (float)h;
   }
+}
+// The token asked of a row; one outside 0..vocab-1 asks for nothing.
+__device__ __forceinline__ int64_t row_token(const RowAnswers& a, int64_t row) {
+  return a.token64 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
+}
+// The same, the token's logit from the row at element `at`.
+template <int DT>
+__device__ __forceinline__ void row_answer_from(const RowAnswers& a, const void* logits, int64_t at, int vocab, int64_t row,
+                                                float m, const RowSum& r) {
+  const int64_t t = row_token(a, row);
+  const bool asked = t >= 0 && t < vocab;
+  row_answer(a, row, asked, asked ? load_as_f32(logits, DT, (size_t)(at + t)) : 0.0f, m, r);
 }
 
 }  // namespace nvjsel

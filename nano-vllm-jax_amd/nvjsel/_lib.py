@@ -54,6 +54,8 @@ SIGNATURES = {
     "nvjsel_token_logprobs_workspace_size": (_sz, [_i, _i64, _i, _i]),
     "nvjsel_token_logprobs": (_i, [_vp, _i, _i64, _i, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nvjsel_token_logprobs_grad": (_i, [_vp, _i, _i64, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nvjsel_lm_head_token_logprobs_workspace_size": (_sz, [_i, _i, _i, _i64, _i, _i]),
+    "nvjsel_lm_head_token_logprobs": (_i, [_vp, _i, _vp, _i, _i, _i64, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
     "nvjsel_adapters_workspace_size": (_sz, [_i, _i64, _i]),
     "nvjsel_apply_adapters": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _i64, _vp, _i64,
                                    _vp, _sz, _vp]),

@@ -50,7 +50,7 @@ class _WorkspacePool:
     a buffer for as long as its graph lives, so a larger one does not replace it but comes
     beside it, at twice its size; those that no captured call takes go."""
 
-    UNCAPTURED = ("beam", "logprobs", "adapters")
+    UNCAPTURED = ("beam", "logprobs", "score", "adapters")
 
     def __init__(self):
         self._bufs: dict = {}

@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .adapters import AdapterTable, _no_gradient
-from .selection import _adapter_ids, _flatten_hidden, _normed, lm_head_logits_hip
+from .selection import _adapter_ids, _normed, _weight_operand, lm_head_logits_hip, reference_reduce_cast
 from .w4 import W4Weight
 from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
 
@@ -151,33 +151,73 @@ def lm_head_token_logprobs(hidden: torch.Tensor, output_weight, tokens: torch.Te
     ``hidden [..., H]``, ``tokens`` int32 or int64 of the shape before H; ``output_weight``,
     ``weight_layout``, ``reduce_cast``, ``adapters`` and ``adapter_ids`` (one for every row) as in ``lm_head_logits_hip``, whose logits'
     log probabilities these are; ``norm_weight``: pre-norm hidden, as in ``lm_head_greedy_top1_hip``.
-    The logits are formed for some rows at a time and never kept.  Not differentiable."""
+    Logits are not written for a 16-bit weight ``[V, H]`` (the tied table) with H a multiple of 64 and
+    hidden of its type, or f32 beside bf16, without alternatives or adapters; other calls form them for some
+    rows at a time.  Not differentiable."""
     if hidden.ndim < 1 or tokens.shape != hidden.shape[:-1]:
         raise ValueError("lm_head_token_logprobs takes hidden [..., H] and one token for every row")
     if hidden.numel() == 0:
         raise ValueError("LM-head log probabilities require non-empty dimensions")
-    if not 0 <= int(num_top) <= MAX_TOP:
+    num_top = int(num_top)
+    if not 0 <= num_top <= MAX_TOP:
         raise ValueError(f"num_top must be in 0..{MAX_TOP} (got {num_top})")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64 (got {tokens.dtype})")
+    if tokens.numel() > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows (got {tokens.numel()})")
     weight = output_weight.packed if isinstance(output_weight, W4Weight) else output_weight
     _no_gradient("lm_head_token_logprobs", hidden, weight, norm_weight)
     shape, rows = tokens.shape, tokens.numel()
     x = hidden.reshape(rows, hidden.shape[-1])
-    tokens = tokens.reshape(rows)
+    tokens = tokens.reshape(rows).contiguous()
     dev = _require_cuda(x, tokens)
     if adapters is not None:
         adapter_ids = _adapter_ids(adapter_ids, x)
     with _on_device(dev):
         if norm_weight is not None:
             x = _normed(x, norm_weight, rms_norm_eps, act_dtype)
-        vocab = output_weight.vocab if isinstance(output_weight, W4Weight) else max(output_weight.shape)
-        step = max(64, _LOGIT_BYTES // (4 * vocab) // 64 * 64)
-        parts = []
-        for i in range(0, rows, step):
-            logits = lm_head_logits_hip(x[i:i + step], output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
-                                        adapters=adapters,
-                                        adapter_ids=None if adapters is None else adapter_ids[i:i + step])
-            parts.append(token_logprobs(logits, tokens[i:i + step], num_top=num_top, entropy=entropy))
-    r = [None if p[0] is None else p[0] if len(parts) == 1 else torch.cat(p) for p in zip(*parts)]
+        r = None
+        if adapters is None and num_top == 0 and not isinstance(output_weight, W4Weight):
+            r = _scored(x, output_weight, tokens, entropy, weight_layout, reduce_cast)
+        if r is None:
+            r = _scored_by_logits(x, output_weight, tokens, num_top, entropy, weight_layout, reduce_cast, adapters,
+                                  adapter_ids)
     return TokenLogprobs(*(t if t is None else t.reshape(*shape, *t.shape[1:]) for t in r))
+
+
+def _scored(x, output_weight, tokens, entropy, weight_layout, reduce_cast):
+    """Without logits; None for a call that the kernel does not take."""
+    w, layout, vocab = _weight_operand(output_weight, weight_layout, int(x.shape[1]))
+    hd, wd = _dtype_code(x, "hidden"), _dtype_code(w, "weight")
+    dev = _require_cuda(x, w)
+    x = x.contiguous()
+    if vocab == 0 or (x.data_ptr() | w.data_ptr()) & 15:
+        return None
+    nbytes = _score_bytes(dev.index, hd, wd, layout, int(x.shape[0]), int(x.shape[1]), vocab)
+    if nbytes == 0:
+        return None
+    rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
+    logprobs = torch.empty((x.shape[0],), dtype=torch.float32, device=dev)
+    ent = torch.empty_like(logprobs) if entropy else None
+    stream = _stream_handle(dev)
+    ws = _workspace(dev, stream, "score", nbytes, 0)
+    _lib.call("nvjsel_lm_head_token_logprobs", x.data_ptr(), hd, w.data_ptr(), wd, layout, x.shape[0], x.shape[1], vocab, rc,
+              tokens.data_ptr(), tokens.element_size(), logprobs.data_ptr(), _ptr(ent), ws.data_ptr(), nbytes, stream)
+    return logprobs, ent, None, None
+
+
+@lru_cache(maxsize=1024)
+def _score_bytes(device: int, *shape: int) -> int:
+    return _lib.load().nvjsel_lm_head_token_logprobs_workspace_size(*shape)
+
+
+def _scored_by_logits(x, output_weight, tokens, num_top, entropy, weight_layout, reduce_cast, adapters, adapter_ids):
+    vocab = output_weight.vocab if isinstance(output_weight, W4Weight) else max(output_weight.shape)
+    step = max(64, _LOGIT_BYTES // (4 * vocab) // 64 * 64)
+    parts = []
+    for i in range(0, x.shape[0], step):
+        ids = None if adapters is None else adapter_ids[i:i + step]
+        logits = lm_head_logits_hip(x[i:i + step], output_weight, weight_layout=weight_layout, reduce_cast=reduce_cast,
+                                    adapters=adapters, adapter_ids=ids)
+        parts.append(token_logprobs(logits, tokens[i:i + step], num_top=num_top, entropy=entropy))
+    return [None if p[0] is None else p[0] if len(parts) == 1 else torch.cat(p) for p in zip(*parts)]
