@@ -21,13 +21,17 @@ _SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 VOCAB, HIDDEN = 248320, 1024  # the served model's LM head
 
 
-def _nvjsel():
-    pkg = os.path.abspath("nano-vllm-jax_amd")  # the package's folder is not importable by its own name
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import nvjsel
+_package = None
 
-    return nvjsel
+
+def _nvjsel():
+    global _package
+    if _package is None:  # looked up once, not at every call
+        pkg = os.path.abspath("nano-vllm-jax_amd")  # the package's folder is not importable by its own name
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        import nvjsel as _package
+    return _package
 
 
 def _logprobs(name, rows, vocab, top, entropy, dtype, masked=False, grad=False, padded=False):
