@@ -395,13 +395,18 @@ int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtype, const vo
  * Low-rank adapters beside a shared projection (no counterpart in the reference):
  *   out[n] = base[n] + scales[a] (x[n] A_a^T) B_a^T,  a = ids[n];  base[n] where a is outside 0..count-1.
  * x [rows, hidden] of x_dtype, base and out [rows, width] of out_dtype (rows their strides
- * apart, out of at least width; out = base for in place, else they share no memory).  Tables of
- * bf16 or f16, 16-byte aligned: a_table [count, rank, hidden rounded up to 32] and b_table
- * [count, width, rank], zeros behind an adapter's own sizes, rank 8, 16 or a multiple of 32 up to
- * 512; scales f32, ids int32.  fp32 sums, out rounded once.  A NaN or an infinity in a row of x or in
+ * apart, out of at least width; out = base for in place, else they share no memory).  hidden at least 8
+ * (NVJSEL_EUNSUPPORTED below).  Tables of bf16 or f16 from nvjsel_adapters_pack, of `rank` 16 or a multiple of
+ * 32 up to 512; scales f32, ids int32.  fp32 sums, out rounded once.  A NaN or an infinity in a row of x or in
  * its adapter makes that row NaN and no other.  rows at most 2^20, hidden 2^24, width 2^28.
  * Workspace: scratch (16-byte aligned).
+ *
+ * nvjsel_adapters_pack lays out `count` adapters' a [rank, hidden] (which = 0) or b [width, rank] (1) of
+ * 16-bit values, count_stride and row_stride elements apart, for the kernels: `packed` (16-byte aligned) takes
+ * count x rank_pad x (hidden rounded up to 32, or width to 64) values, zeros behind the adapters' own sizes.
  */
+int nvjsel_adapters_pack(const void* plain, int which, int64_t count_stride, int64_t row_stride, int count, int rank,
+                         int hidden, int width, int rank_pad, void* packed, size_t packed_bytes, void* stream);
 size_t nvjsel_adapters_workspace_size(int table_dtype, int64_t rows, int rank);
 int nvjsel_apply_adapters(const void* x, int x_dtype, int64_t x_stride, const void* base, int out_dtype,
                           int64_t base_stride, const void* a_table, const void* b_table, int table_dtype,

@@ -3,10 +3,10 @@
 //   out[n] = base[n] + s_a sum_r y[n, r] B_a[:, r],   y[n, r] = sum_k x[n, k] A_a[r, k],   a = ids[n]
 //
 // (base[n] alone where ids[n] names no adapter).  Both products run on the matrix cores
-// with fp32 sums, and out is rounded once.  y is kept in more than 16 bits between them:
-// s_a y as three bf16 terms (hi + mid + lo = y, 24 bits) beside bf16 tables, as two f16
-// terms of the row scaled to its largest value (22 bits; below 2^-39 of that value
-// nothing) beside f16 ones.  x of another type than the tables is split into bf16 terms
+// with fp32 sums, and out is rounded once.  s_a y lies in fp32 between them
+// and enters the second as three bf16 terms (hi + mid + lo = y, 24 bits) beside bf16 tables, as two
+// f16 terms of the row scaled to its largest value (22 bits; below 2^-39 of that value nothing)
+// beside f16 ones.  x of another type than the tables is split into bf16 terms
 // exactly (f16 two, f32 three), f16 tables beside them too.
 //
 // Rows name adapters in any order.  A matrix tile holds 16 rows whatever their adapters:
@@ -18,16 +18,14 @@ namespace nvjsel {
 
 static constexpr int kAdapterRank = 512;  // at most
 static constexpr int kShrinkWaves = 8;    // of a block, which share the hidden size
-static constexpr int kShrinkRank = 64;    // rank of a pass over the hidden rows
+// Steps of 32 hidden values, whose loads a wave has in flight, and blocks of a call (2000 prompt rows x 2560,
+// rank 64, 2 / 4 / 5 steps: 11.6 / 12.3 / 14.5 us; 16 waves 14.8; blocks 256 to 1024 alike).
+static constexpr int kShrinkSteps = 2;
+static constexpr int kShrinkBlocks = 512;
 
 // Terms that y is kept in.
 __host__ __device__ constexpr int adapter_terms(int table_dtype) { return table_dtype == DT_BF16 ? 3 : 2; }
 
-// Eight elements at p, the first `left` of them (the rest 0), as NX matrix operands of 16 bits.
-template <int XDT, int TDT>
-struct AdapterX {
-  static constexpr int NX = XDT == TDT ? 1 : XDT == DT_F32 ? 3 : XDT == DT_F16 ? 2 : 1;
-};
 // f32 values as the next bf16 term, which leaves the remainders.
 __device__ __forceinline__ u32x4_t bf16_term(float (&v)[8]) {
   uint32_t o[4];
@@ -47,55 +45,67 @@ __device__ __forceinline__ void f16_values(u32x4_t w, float (&v)[8]) {
     v[2 * j + 1] = f16_to_f32((uint16_t)(w[j] >> 16));
   }
 }
+// x[k .. k + 7] of a row as it lies: loads without conditions, from the row's last eight where it
+// ends before k + 8.  moved() puts those in place: the table is 0 behind the hidden size, so that
+// any number may stand beside it (one that is not finite makes its row NaN all the same).
 template <int XDT, int TDT>
-__device__ __forceinline__ void adapter_x(const char* row, int k, int left, u32x4_t (&f)[AdapterX<XDT, TDT>::NX]) {
-  constexpr int NX = AdapterX<XDT, TDT>::NX;
-  float v[8];
-  if constexpr (XDT == DT_F32) {
-    const float* p = (const float*)row + k;
-    if (left >= 8) {
+struct AdapterX {
+  static constexpr int NX = XDT == TDT ? 1 : XDT == DT_F32 ? 3 : XDT == DT_F16 ? 2 : 1;
+  u32x4_t w[XDT == DT_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char* row, int k, int hidden) {
+    const int at = k < hidden - 8 ? k : hidden - 8;
+    if constexpr (XDT == DT_F32) {
       typedef u32x4_t any __attribute__((aligned(4)));
-      const u32x4_t a = *(const any*)p, b = *(const any*)(p + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = __uint_as_float(a[j]);
-        v[4 + j] = __uint_as_float(b[j]);
-      }
+      w[0] = *(const any*)((const float*)row + at);
+      w[1] = *(const any*)((const float*)row + at + 4);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.0f;
+      w[0] = *(const u32x4_any_t*)((const uint16_t*)row + at);
     }
+  }
+  __device__ __forceinline__ void move(int k, int hidden) {
+    const int by = k + 8 - hidden < 0 ? 0 : k + 8 - hidden > 7 ? 7 : k + 8 - hidden;
+    if constexpr (XDT == DT_F32) {
+      uint32_t v[8];
 #pragma unroll
-    for (int t = 0; t < NX; ++t) f[t] = bf16_term(v);
-  } else {
-    const uint16_t* p = (const uint16_t*)row + k;
-    u32x4_t w{0u, 0u, 0u, 0u};
-    if (left >= 8) {
-      w = *(const u32x4_any_t*)p;
+      for (int e = 0; e < 8; ++e) v[e] = w[e >> 2][e & 3];
+#pragma unroll
+      for (int d = 1; d < 8; d *= 2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = by & d ? (e + d < 8 ? v[e + d] : 0u) : v[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = v[e];
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+      w[0] = shift_down8(w[0], by);
     }
+  }
+  // As matrix operands of 16 bits; none of them where !live.
+  __device__ __forceinline__ void split(bool live, u32x4_t (&f)[NX]) const {
+    const uint32_t mask = live ? ~0u : 0u;
     if constexpr (NX == 1) {
-      f[0] = w;
+      f[0] = w[0] & mask;
     } else {
-      f16_values(w, v);
+      float v[8];
+      if constexpr (XDT == DT_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e >> 2][e & 3] & mask);
+      } else {
+        f16_values(w[0] & mask, v);
+      }
 #pragma unroll
       for (int t = 0; t < NX; ++t) f[t] = bf16_term(v);
     }
   }
-}
+};
 
 struct AdapterArgs {
   const void* x;
   int64_t x_stride;
-  const void* a;        // [count, rank, hidden_pad], zeros behind the adapters' own sizes
-  const void* b;        // [count, width, rank]
+  const void* a;        // the tables in the order of a wave's loads (adapter_pack_kernel)
+  const void* b;
   const float* scales;  // [count]
   const int32_t* ids;   // [rows]
-  int rows, hidden, hidden_pad, rank, width, count;
-  uint16_t* terms;      // [rows, terms, rank]
+  int rows, hidden, hidden_pad, rank, width, width_pad, count;
+  uint16_t* terms;      // [rows, terms, rank]: y's
   float* row_scale;     // [rows]: what the terms are to be multiplied with (f16 tables)
   const void* base;
   int64_t base_stride;
@@ -103,332 +113,463 @@ struct AdapterArgs {
   int64_t out_stride;
 };
 
-// y of 16 rows and one of their adapters: block (tile, j) takes row j's adapter where no row
-// before it has the same one.  The waves split the hidden size; their sums meet in LDS, in
-// order.
-template <int XDT, int TDT>
-__global__ void __launch_bounds__(64 * kShrinkWaves) adapter_shrink_kernel(AdapterArgs a) {
-  constexpr int NX = AdapterX<XDT, TDT>::NX, NT = adapter_terms(TDT);
+// The power of two that takes a row whose largest magnitude is m to 2^14 .. 2^15 (1 where it has none).
+__device__ __forceinline__ int adapter_exponent(float m) {
+  const int e = 15 - __builtin_amdgcn_frexp_expf(m);
+  return !(m > 0.0f && m < INFINITY) ? 0 : e < -126 ? -126 : e > 126 ? 126 : e;
+}
+// The next term of v in the tables' type, which leaves the remainder.
+template <int TDT>
+__device__ __forceinline__ uint16_t adapter_term(float& v) {
+  if constexpr (TDT == DT_F16) {
+    const _Float16 h = (_Float16)v;
+    v = v - (float)h;
+    return __builtin_bit_cast(uint16_t, h);
+  } else {
+    const __bf16 h = (__bf16)v;
+    v = v - (float)h;
+    return __builtin_bit_cast(uint16_t, h);
+  }
+}
+
+// y of 16 rows, 16 RG ranks a pass over the hidden size: block (tile, j) takes every J-th of the
+// adapters among the rows, so that a decode step's many adapters run beside each other and a prompt's one
+// leaves few blocks without work.  The waves split the hidden size, each with the loads of
+// kShrinkSteps steps in flight; their sums meet in LDS, in order.
+template <int XDT, int TDT, int RG>
+__global__ void __launch_bounds__(64 * kShrinkWaves, 4) adapter_shrink_kernel(AdapterArgs a) {
+  constexpr int NX = AdapterX<XDT, TDT>::NX, NT = adapter_terms(TDT), RANK = 16 * RG, S = kShrinkSteps;
   constexpr bool SPLIT = TDT == DT_F16 && XDT != DT_F16;  // the tables as two bf16 terms
   constexpr int MT = TDT == DT_F16 && !SPLIT ? DT_F16 : DT_BF16;
-  __shared__ float part[kShrinkWaves][kShrinkRank][17];
-  __shared__ float y[16][kAdapterRank];
+  __shared__ float part[kShrinkWaves][RANK][17];
+  __shared__ float y[16][RG < 4 ? RANK : kAdapterRank];
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int g = lane >> 4, c = lane & 15, row0 = (int)blockIdx.x * 16, j = (int)blockIdx.y;
+  const int g = lane >> 4, c = lane & 15, row0 = (int)blockIdx.x * 16;
   const int row = row0 + c < a.rows ? row0 + c : a.rows - 1;
   int id = a.ids[row];
   if (row0 + c >= a.rows || id < 0 || id >= a.count) id = -1;
-  const int own = __builtin_amdgcn_readlane(id, j);
-  const uint32_t mine = (uint32_t)__ballot(id == own) & 0xFFFFu;
-  if (own < 0 || __builtin_ctz(mine) != j) return;
-
   const char* xrow = (const char*)a.x + (int64_t)row * a.x_stride * (XDT == DT_F32 ? 4 : 2);
-  const uint16_t* table = (const uint16_t*)a.a + (size_t)own * a.rank * a.hidden_pad;
   const int steps = a.hidden_pad / 32;
-  const float scale = a.scales[own];
-  for (int r0 = 0; r0 < a.rank; r0 += kShrinkRank) {
-    f32x4_t acc[kShrinkRank / 16];
+  const bool ragged = a.hidden % 8 != 0;
+  uint32_t left = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  for (int nth = 0; left; ++nth) {
+    const int own = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    const uint32_t mine = (uint32_t)__ballot(id == own) & 0xFFFFu;
+    left &= ~mine;
+    if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
+    const float scale = a.scales[own];
+    for (int r0 = 0; r0 < a.rank; r0 += RANK) {
+      const u32x4_t* table = (const u32x4_t*)a.a + ((size_t)own * a.rank + r0) / 16 * steps * 64 + lane;
+      const int tiles = (a.rank - r0) / 16;  // left, past which the last repeats: its sums are left out
+      f32x4_t acc[RG];
 #pragma unroll
-    for (int t = 0; t < kShrinkRank / 16; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = wave; s < steps; s += kShrinkWaves) {
-      const int k = s * 32 + g * 8;
-      u32x4_t xf[NX];
-      adapter_x<XDT, TDT>(xrow, k, a.hidden - k, xf);
+      for (int t = 0; t < RG; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int s0 = wave; s0 < steps; s0 += kShrinkWaves * S) {
+        AdapterX<XDT, TDT> xs[S];
+        u32x4_t w[S][RG];
 #pragma unroll
-      for (int t = 0; t < kShrinkRank / 16; ++t) {
-        if (r0 + t * 16 >= a.rank) break;
-        const int r = r0 + t * 16 + c;
-        u32x4_t w{0u, 0u, 0u, 0u};
-        if (r < a.rank) w = *(const u32x4_t*)(table + (size_t)r * a.hidden_pad + k);
-        if constexpr (SPLIT) {
-          float v[8];
-          f16_values(w, v);
+        for (int u = 0; u < S; ++u) {  // past the end: the last step again, beside zeros
+          const int s = s0 + u * kShrinkWaves < steps ? s0 + u * kShrinkWaves : steps - 1;
+          xs[u].load(xrow, s * 32 + g * 8, a.hidden);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const u32x4_t term = bf16_term(v);
+          for (int t = 0; t < RG; ++t) w[u][t] = table[((size_t)(t < tiles ? t : tiles - 1) * steps + s) * 64];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
 #pragma unroll
-            for (int n = 0; n < NX; ++n) acc[t] = mfma16x16x32<MT>(term, xf[n], acc[t]);
+        for (int u = 0; u < S; ++u) {
+          const int s = s0 + u * kShrinkWaves;
+          u32x4_t xf[NX];
+          if (ragged && s == steps - 1) xs[u].move(s * 32 + g * 8, a.hidden);
+          xs[u].split(s < steps, xf);
+#pragma unroll
+          for (int t = 0; t < RG; ++t) {
+            if constexpr (SPLIT) {
+              float v[8];
+              f16_values(w[u][t], v);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const u32x4_t term = bf16_term(v);
+#pragma unroll
+                for (int n = 0; n < NX; ++n) acc[t] = mfma16x16x32<MT>(term, xf[n], acc[t]);
+              }
+            } else {
+#pragma unroll
+              for (int n = 0; n < NX; ++n) acc[t] = mfma16x16x32<MT>(w[u][t], xf[n], acc[t]);
+            }
           }
-        } else {
-#pragma unroll
-          for (int n = 0; n < NX; ++n) acc[t] = mfma16x16x32<MT>(w, xf[n], acc[t]);
         }
       }
+#pragma unroll
+      for (int t = 0; t < RG; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[wave][t * 16 + 4 * g + e][c] = acc[t][e];
+      __syncthreads();
+      for (int i = (int)threadIdx.x; i < RANK * 16; i += 64 * kShrinkWaves) {
+        const int r = i >> 4, n = i & 15;
+        float s = part[0][r][n];
+#pragma unroll
+        for (int w = 1; w < kShrinkWaves; ++w) s += part[w][r][n];
+        if (r0 + r < a.rank) y[n][r0 + r] = s * scale;
+      }
+      __syncthreads();
     }
-    if (r0) __syncthreads();
+    for (int n = wave; n < 16; n += kShrinkWaves) {
+      if (!(mine >> n & 1)) continue;
+      float up = 1.0f;
+      if constexpr (TDT == DT_F16) {
+        float m = 0.0f;
+        for (int r = lane; r < a.rank; r += 64) m = fmaxf(m, fabsf(y[n][r]));
+        const int e = adapter_exponent(__uint_as_float(wave_max_u32(__float_as_uint(m))));
+        up = __builtin_amdgcn_ldexpf(1.0f, e);
+        if (lane == 0) a.row_scale[row0 + n] = __builtin_amdgcn_ldexpf(1.0f, -e);
+      }
+      uint16_t* out = a.terms + (size_t)(row0 + n) * NT * a.rank;
+      for (int r = lane; r < a.rank; r += 64) {
+        float v = y[n][r] * up;
 #pragma unroll
-    for (int t = 0; t < kShrinkRank / 16; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[wave][t * 16 + 4 * g + e][c] = acc[t][e];
-    __syncthreads();
-    for (int i = (int)threadIdx.x; i < kShrinkRank * 16; i += 64 * kShrinkWaves) {
-      const int r = i >> 4, n = i & 15;
-      float s = part[0][r][n];
-#pragma unroll
-      for (int w = 1; w < kShrinkWaves; ++w) s += part[w][r][n];
-      if (r0 + r < a.rank) y[n][r0 + r] = s * scale;
-    }
-  }
-  __syncthreads();
-  for (int n = wave; n < 16; n += kShrinkWaves) {
-    if (!(mine >> n & 1)) continue;
-    float up = 1.0f;
-    if constexpr (TDT == DT_F16) {  // the row's largest value to 2^14 .. 2^15
-      float m = 0.0f;
-      for (int r = lane; r < a.rank; r += 64) m = fmaxf(m, fabsf(y[n][r]));
-      m = __uint_as_float(wave_max_u32(__float_as_uint(m)));
-      int e = 15 - __builtin_amdgcn_frexp_expf(m);
-      if (!(m > 0.0f && m < INFINITY)) e = 0;
-      e = e < -126 ? -126 : e > 126 ? 126 : e;
-      up = __builtin_amdgcn_ldexpf(1.0f, e);
-      if (lane == 0) a.row_scale[row0 + n] = __builtin_amdgcn_ldexpf(1.0f, -e);
-    }
-    uint16_t* out = a.terms + (size_t)(row0 + n) * NT * a.rank;
-    for (int r = lane; r < a.rank; r += 64) {
-      float v = y[n][r] * up;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (TDT == DT_F16) {
-          const _Float16 h = (_Float16)v;
-          out[t * a.rank + r] = __builtin_bit_cast(uint16_t, h);
-          v = v - (float)h;
-        } else {
-          const __bf16 h = (__bf16)v;
-          out[t * a.rank + r] = __builtin_bit_cast(uint16_t, h);
-          v = v - (float)h;
-        }
+        for (int t = 0; t < NT; ++t) out[t * a.rank + r] = adapter_term<TDT>(v);
       }
     }
+    __syncthreads();  // y is free
   }
 }
 
-// 16 consecutive elements of a row as f32 and back; `left` of them exist.
-template <int ODT>
-__device__ __forceinline__ void load16(const char* row, int64_t v, int left, float (&x)[16]) {
-  if constexpr (ODT == DT_F32) {
-    typedef u32x4_t any __attribute__((aligned(4)));
-    const float* p = (const float*)row + v;
-    if (left >= 16) {
+// N consecutive elements of a row (8 or 16) as they lie; `left` of them exist.
+template <int ODT, int N>
+struct AdapterOut {
+  static constexpr int W = ODT == DT_F32 ? N : N / 2;  // words
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const char* row, int64_t v, int left, bool whole) {
+    if (whole) {
+      const char* p = row + v * (ODT == DT_F32 ? 4 : 2);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const u32x4_t w = *(const any*)(p + 4 * q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * q + e] = __uint_as_float(w[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = e < left ? p[e] : 0.0f;
-    }
-  } else {
-    const uint16_t* p = (const uint16_t*)row + v;
-    uint32_t w[8];
-    if (left >= 16) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const u32x4_t u = *(const u32x4_any_t*)(p + 8 * q);
+      for (int q = 0; q < W / 4; ++q) {
+        const u32x4_t u = *(const u32x4_any_t*)(p + 16 * q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * q + e] = u[e];
       }
-    } else {
+    } else if constexpr (ODT == DT_F32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < N; ++e) w[e] = e < left ? ((const uint32_t*)row)[v + e] : 0u;
+    } else {
+      const uint16_t* p = (const uint16_t*)row + v;
+#pragma unroll
+      for (int e = 0; e < W; ++e)
         w[e] = (2 * e < left ? (uint32_t)p[2 * e] : 0u) | (2 * e + 1 < left ? (uint32_t)p[2 * e + 1] << 16 : 0u);
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-      x[e] = ODT == DT_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
-    }
   }
-}
-template <int ODT>
-__device__ __forceinline__ void store16(char* row, int64_t v, int left, const float (&x)[16]) {
-  if constexpr (ODT == DT_F32) {
-    typedef u32x4_t any __attribute__((aligned(4)));
-    float* p = (float*)row + v;
-    if (left >= 16) {
+  __device__ __forceinline__ void add(const float (&d)[N]) {
+    if constexpr (ODT == DT_F32) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(any*)(p + 4 * q) = u32x4_t{__float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]), __float_as_uint(x[4 * q + 2]),
-                                     __float_as_uint(x[4 * q + 3])};
+      for (int e = 0; e < N; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + d[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e < left) p[e] = x[e];
-    }
-  } else {
-    uint16_t* p = (uint16_t*)row + v;
-    uint16_t h[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      h[e] = ODT == DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)x[e]) : __builtin_bit_cast(uint16_t, (_Float16)x[e]);
-    if (left >= 16) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        u32x4_t w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)h[8 * q + 2 * e + 1] << 16 | h[8 * q + 2 * e];
-        *(u32x4_any_t*)(p + 8 * q) = w;
+      for (int e = 0; e < W; ++e) {
+        const uint16_t lo = (uint16_t)w[e], hi = (uint16_t)(w[e] >> 16);
+        if constexpr (ODT == DT_BF16)
+          w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)(bf16_to_f32(hi) + d[2 * e + 1])) << 16 |
+                 __builtin_bit_cast(uint16_t, (__bf16)(bf16_to_f32(lo) + d[2 * e]));
+        else
+          w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(f16_to_f32(hi) + d[2 * e + 1])) << 16 |
+                 __builtin_bit_cast(uint16_t, (_Float16)(f16_to_f32(lo) + d[2 * e]));
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e < left) p[e] = h[e];
     }
   }
+  __device__ __forceinline__ void store(char* row, int64_t v, int left) const {
+    if (left >= N) {
+      char* p = row + v * (ODT == DT_F32 ? 4 : 2);
+#pragma unroll
+      for (int q = 0; q < W / 4; ++q) *(u32x4_any_t*)(p + 16 * q) = u32x4_t{w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
+    } else if constexpr (ODT == DT_F32) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < left) ((uint32_t*)row)[v + e] = w[e];
+    } else {
+      uint16_t* p = (uint16_t*)row + v;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < left) p[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+// v_mfma_f32_16x16x16: four k of a row per lane.
+template <int WT>
+__device__ __forceinline__ f32x4_t mfma16x16x16(u32x2_t a, u32x2_t b, f32x4_t c) {
+  if constexpr (WT == DT_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a), __builtin_bit_cast(s16x4_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a), __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
 }
 
-// A wave's 64 columns x 16 RT rows.  The matrix tiles' rows are columns of out, dealt so that
-// a lane ends with 16 consecutive ones of one row: tile t's row i is column 16 (i >> 2) + 4 t +
-// (i & 3).  OCT: eights of a rank below 32, whose terms lie side by side along a matrix
-// instruction's k (4: a multiple of 32, a term after another).
-template <int TDT, int ODT, int OCT, int RT>
+// ---- The tables' layout: pieces of 16 bytes (8 values) in the order of a wave's loads, 64 of them (1 KB)
+// an instruction; piece of lane (c, g) = (lane & 15, lane >> 4), zeros behind the adapters' own sizes.
+//   a: [count][rank / 16][hidden_pad / 32][lane]: A[16 i + c][32 s + 8 g ..]
+//   b: [count][width_pad / 64][rank / 32][4][lane], ranks 32 and more:  B[column(t, c)][32 k + 8 g ..]
+//      [count][width_pad / 64][2][lane], rank 16:                       B[column(2 l + (g >> 1), c)][8 (g & 1) ..]
+//   column(t, c) = 64 group + 16 (c >> 2) + 4 t + (c & 3)
+struct AdapterPack {
+  const uint16_t* from;  // [count][major][minor], strides in elements, minor's 1
+  int64_t count_stride, row_stride;
+  int rank, hidden, width;              // of the adapters
+  int rank_pad, hidden_pad, width_pad;  // of the table
+  uint4* to;
+  int64_t pieces;
+};
+template <bool B>
+__global__ void __launch_bounds__(256) adapter_pack_kernel(AdapterPack p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.pieces) return;
+  const int lane = (int)(i & 63), c = lane & 15, g = lane >> 4;
+  int64_t j = i >> 6;
+  int row, k;  // of the plain form
+  if constexpr (!B) {
+    const int steps = p.hidden_pad / 32;
+    k = (int)(j % steps) * 32 + 8 * g;
+    j /= steps;
+    row = (int)(j % (p.rank_pad / 16)) * 16 + c;
+    j /= p.rank_pad / 16;
+  } else {
+    int t;
+    if (p.rank_pad == 16) {
+      t = 2 * (int)(j & 1) + (g >> 1);
+      k = 8 * (g & 1);
+      j >>= 1;
+    } else {
+      t = (int)(j & 3);
+      j >>= 2;
+      k = (int)(j % (p.rank_pad / 32)) * 32 + 8 * g;
+      j /= p.rank_pad / 32;
+    }
+    row = (int)(j % (p.width_pad / 64)) * 64 + 16 * (c >> 2) + 4 * t + (c & 3);
+    j /= p.width_pad / 64;
+  }
+  const int rows = B ? p.width : p.rank, ks = B ? p.rank : p.hidden;
+  const uint16_t* from = p.from + j * p.count_stride + (int64_t)row * p.row_stride + k;
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    w[e] = row < rows && k + 2 * e < ks ? from[2 * e] : 0u;
+    if (row < rows && k + 2 * e + 1 < ks) w[e] |= (uint32_t)from[2 * e + 1] << 16;
+  }
+  p.to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A wave's 16 CT columns x 16 RT rows.  The matrix tiles' rows are columns of out, dealt so that
+// a lane ends with 4 CT consecutive ones of one row: tile t's row i is column 4 CT (i >> 2) + 4 t + (i & 3).
+// The table's rows of the next adapters (or eights of their ranks) are on their way in a ring of
+// kExpandDepth slots, loads without conditions: the last adapter's again at the end.  base is
+// requested before all of them.
+// Rank 16 (WIDE false): a 16-byte load of a lane is half a row of the table, two tiles an
+// instruction; swapping halves of the wave makes of it two operands of 16x16x16 products, lane
+// (c, g) with ranks 8 (g & 1) + 4 (g >> 1) .. + 3, so that no byte is loaded twice for y's terms.
+// Wider ranks: 16x16x32 products, 32 ranks a step, y's terms in LDS.
+template <int TDT, int ODT, bool WIDE, int RT>
 __global__ void __launch_bounds__(256) adapter_expand_kernel(AdapterArgs a) {
-  constexpr int NT = adapter_terms(TDT);
+  constexpr int CT = 4, NT = adapter_terms(TDT), D = WIDE ? 2 : 3, WL = WIDE ? CT : CT / 2;
+  extern __shared__ __attribute__((aligned(16))) char staged[];
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
+  const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * (16 * CT);
   const int row0 = (int)blockIdx.y * 16 * RT;
-  if (v0 >= a.width) return;
   int id = -1;  // of row row0 + lane
   if (lane < 16 * RT && row0 + lane < a.rows) {
     id = a.ids[row0 + lane];
     if (id >= a.count) id = -1;
   }
-  const uint64_t named = __ballot(id >= 0);
   const bool in_place = a.out == a.base;
-  if (in_place && named == 0) return;
-  const uint16_t* terms[RT];
+  if (in_place && __ballot(id >= 0) == 0) return;
+  // The rows in order of adapter, in which the matrix tiles take them, those without one last: an adapter's rows
+  // lie in one tile or two, and the others need no product with it (64 rows of 16 adapters in the order given: a
+  // third of the matrix pipe's time more than the loads take).  From here on id and mine[] go by place.
+  int place = 0, count = 0;
+  for (uint64_t todo = __ballot(id >= 0), of; todo; todo &= ~of) {
+    of = __ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(todo)));
+    if (of >> lane & 1) place = count + __builtin_popcountll(of & ((1ull << lane) - 1));
+    count += __builtin_popcountll(of);
+  }
+  const uint64_t none = __ballot(id < 0), named = count == 64 ? ~0ull : (1ull << count) - 1;
+  if (id < 0) place = count + __builtin_popcountll(none & ((1ull << lane) - 1));
+  const int from = __builtin_amdgcn_ds_permute(place * 4, lane);  // the lane that holds this lane's place
+  id = __builtin_amdgcn_ds_bpermute(from * 4, id);
+  int mine[RT];  // this lane's row of each tile
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) mine[rt] = row0 + __builtin_amdgcn_ds_bpermute((rt * 16 + c) * 4, from);
+  constexpr int es = ODT == DT_F32 ? 4 : 2;
+  const int64_t v = v0 + 4 * CT * g;
+  const int here = (int)(a.width - v < 4 * CT ? a.width - v : 4 * CT);  // columns of this lane, none below 1
+  const bool whole = v0 + 16 * CT <= a.width;                            // of this wave
+  AdapterOut<ODT, 4 * CT> out[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = row0 + rt * 16 + c < a.rows ? row0 + rt * 16 + c : a.rows - 1;
-    terms[rt] = a.terms + (size_t)row * NT * a.rank;
+    const int row = mine[rt] < a.rows ? mine[rt] : a.rows - 1;
+    out[rt].load((const char*)a.base + (int64_t)row * a.base_stride * es, v, here, whole);
   }
-  size_t brow[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t v = v0 + 16 * (c >> 2) + 4 * t + (c & 3);
-    brow[t] = (size_t)(v < a.width ? v : a.width - 1) * a.rank;
-  }
-  f32x4_t acc[RT][4];
+  f32x4_t acc[RT][CT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto keep = [&](int rt, uint64_t same, const f32x4_t (&d)[4]) NVJSEL_INLINE {
-    const bool mine = same >> (rt * 16 + c) & 1;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[rt][t][e] = mine ? d[t][e] : acc[rt][t][e];
-  };
-  if constexpr (OCT < 4) {
-    constexpr int STEPS = (NT * OCT + 3) / 4;
-    u32x4_t y[RT][STEPS];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int q = 4 * s + g;
-        y[rt][s] = q < NT * OCT && named ? *(const u32x4_t*)(terms[rt] + q * 8) : u32x4_t{0u, 0u, 0u, 0u};
-      }
-    for (uint64_t left = named; left;) {
-      const int own = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-      const uint64_t same = __ballot(id == own);
-      left &= ~same;
-      const uint16_t* b = (const uint16_t*)a.b + (size_t)own * a.width * a.rank;
-      u32x4_t w[4][STEPS];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) w[t][s] = *(const u32x4_t*)(b + brow[t] + (4 * s + g) % OCT * 8);
+    for (int t = 0; t < CT; ++t) acc[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (named) {
+    const int pitch = NT * a.rank * 2 + 16;  // bytes of a staged row
+    u32x2_t y[RT][NT];
+    if constexpr (!WIDE) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        if (!(same >> (rt * 16) & 0xFFFFu)) continue;
-        f32x4_t d[4];
+        const int row = mine[rt] < a.rows ? mine[rt] : a.rows - 1;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < STEPS; ++s) d[t] = mfma16x16x32<TDT>(w[t][s], y[rt][s], d[t]);
-        }
-        keep(rt, same, d);
+        for (int n = 0; n < NT; ++n)
+          y[rt][n] = *(const u32x2_t*)(a.terms + ((size_t)row * NT + n) * 16 + 8 * (g & 1) + 4 * (g >> 1));
       }
     }
-  } else {
-    for (uint64_t left = named; left;) {
-      const int own = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-      const uint64_t same = __ballot(id == own);
-      left &= ~same;
-      const uint16_t* b = (const uint16_t*)a.b + (size_t)own * a.width * a.rank;
-      f32x4_t d[RT][4];
+    // this lane's pieces of the first adapter; a wave's columns past the end are the last group's
+    const int64_t group = v0 < a.width_pad ? v0 / 64 : a.width_pad / 64 - 1;
+    const u32x4_t* table = (const u32x4_t*)a.b + (size_t)group * 64 * a.rank / 8 + lane;
+    const size_t each = (size_t)a.width_pad * a.rank / 8;
+    uint64_t ahead = named, same[D];
+    int own = 0, kn = 0;
+    int kk[D];
+    u32x4_t raw[D][WL];
+    auto fetch = [&](auto S) NVJSEL_INLINE {
+      constexpr int s = decltype(S)::value;
+      same[s] = 0;
+      kk[s] = kn;
+      if (ahead) {
+        own = __builtin_amdgcn_readlane(id, __builtin_ctzll(ahead));
+        same[s] = __ballot(id == own);
+      }
+      const u32x4_t* b = table + (size_t)own * each + (WIDE ? kn * 8 : 0);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int l = 0; l < WL; ++l) raw[s][l] = b[l * 64];
+      kn += 32;
+      if (!WIDE || kn >= a.rank) {
+        kn = 0;
+        ahead &= ~same[s];
+      }
+    };
+    f32x4_t d[RT][CT];
+    auto body = [&](auto S) NVJSEL_INLINE {
+      constexpr int s = decltype(S)::value;
+      const uint64_t of = same[s];
+      const int k = kk[s];
+      u32x4_t w[WL];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) d[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int k = g * 8; k < a.rank; k += 32) {
-        u32x4_t w[4];
+      for (int l = 0; l < WL; ++l) w[l] = raw[s][l];
+      if constexpr (!WIDE) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) w[t] = *(const u32x4_t*)(b + brow[t] + k);
+        for (int l = 0; l < WL; ++l) {
+          const auto x = __builtin_amdgcn_permlane32_swap(w[l][0], w[l][2], false, false);
+          const auto z = __builtin_amdgcn_permlane32_swap(w[l][1], w[l][3], false, false);
+          w[l] = u32x4_t{x[0], z[0], x[1], z[1]};
+        }
+      }
+      fetch(S);
+      const bool first = !WIDE || k == 0, last = !WIDE || k + 32 >= a.rank;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          if (!(same >> (rt * 16) & 0xFFFFu)) continue;
+      for (int rt = 0; rt < RT; ++rt) {
+        if (!(of >> (rt * 16) & 0xFFFFu)) continue;
+        if (first) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const u32x4_t y = *(const u32x4_t*)(terms[rt] + n * a.rank + k);
+          for (int t = 0; t < CT; ++t) d[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) d[rt][t] = mfma16x16x32<TDT>(w[t], y, d[rt][t]);
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (WIDE) {
+            const u32x4_t f = *(const u32x4_t*)(staged + (mine[rt] - row0) * pitch + (n * a.rank + k + 8 * g) * 2);
+#pragma unroll
+            for (int t = 0; t < CT; ++t) d[rt][t] = mfma16x16x32<TDT>(w[t], f, d[rt][t]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+              d[rt][t] = mfma16x16x16<TDT>(u32x2_t{w[t / 2][2 * (t & 1)], w[t / 2][2 * (t & 1) + 1]}, y[rt][n], d[rt][t]);
           }
         }
-      }
+        if (last) {
+          const bool its = of >> (rt * 16 + c) & 1;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) keep(rt, same, d[rt]);
+          for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][t][e] = its ? d[rt][t][e] : acc[rt][t][e];
+        }
+      }
+    };
+    static_for<D>([&](auto S) NVJSEL_INLINE { fetch(S); });
+    if constexpr (WIDE) {  // y's terms, rows as they lie
+      const int pieces = NT * a.rank / 8;
+      for (int i = (int)threadIdx.x; i < 16 * RT * pieces; i += 256) {
+        const int r = i / pieces, q = i % pieces;
+        *(u32x4_t*)(staged + r * pitch + q * 16) =
+            *(const u32x4_t*)(a.terms + ((size_t)(row0 + r < a.rows ? row0 + r : a.rows - 1) * pieces + q) * 8);
+      }
+      __syncthreads();
     }
+    bool more = true;
+    while (more)
+      static_for<D>([&](auto S) NVJSEL_INLINE {
+        if (more) {
+          if (same[decltype(S)::value]) body(S);
+          else more = false;
+        }
+      });
   }
-  const int64_t v = v0 + 16 * g;
-  const int left = (int)(a.width - v < 16 ? a.width - v : 16);
-  if (left <= 0) return;
-  constexpr int es = ODT == DT_F32 ? 4 : 2;
+  if (here <= 0) return;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = row0 + rt * 16 + c;
+    const int row = mine[rt];
     const bool has = named >> (rt * 16 + c) & 1;
     if (row >= a.rows || (in_place && !has)) continue;
-    float x[16];
-    load16<ODT>((const char*)a.base + (int64_t)row * a.base_stride * es, v, left, x);
     if (has) {  // (a row without an adapter is copied as it is: 0 added would turn -0 into 0)
       const float up = TDT == DT_F16 ? a.row_scale[row] : 1.0f;
+      float x[4 * CT];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * t + e] += TDT == DT_F16 ? acc[rt][t][e] * up : acc[rt][t][e];
+        for (int e = 0; e < 4; ++e) x[4 * t + e] = TDT == DT_F16 ? acc[rt][t][e] * up : acc[rt][t][e];
+      out[rt].add(x);
     }
-    store16<ODT>((char*)a.out + (int64_t)row * a.out_stride * es, v, left, x);
+    out[rt].store((char*)a.out + (int64_t)row * a.out_stride * es, v, here);
   }
 }
 
-template <int TDT, int ODT, int RT>
-static int launch_expand_rows(const AdapterArgs& a, hipStream_t s) {
+template <int TDT, int ODT, bool WIDE, int RT>
+static int launch_expand(const AdapterArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.width + 255) / 256), (unsigned)((a.rows + 16 * RT - 1) / (16 * RT)));
-  if (a.rank == 8) hipLaunchKernelGGL((adapter_expand_kernel<TDT, ODT, 1, RT>), grid, dim3(256), 0, s, a);
-  else if (a.rank == 16) hipLaunchKernelGGL((adapter_expand_kernel<TDT, ODT, 2, RT>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((adapter_expand_kernel<TDT, ODT, 4, RT>), grid, dim3(256), 0, s, a);
+  const size_t lds = WIDE ? (size_t)16 * RT * (adapter_terms(TDT) * a.rank * 2 + 16) : 0;
+  hipLaunchKernelGGL((adapter_expand_kernel<TDT, ODT, WIDE, RT>), grid, dim3(256), lds, s, a);
   NVJSEL_CHECK_LAUNCH("adapter_expand_kernel");
+  return NVJSEL_OK;
+}
+
+template <int XDT, int TDT>
+static int launch_shrink(const AdapterArgs& a, hipStream_t s) {
+  const int tiles = (a.rows + 15) / 16;
+  int each = 16;  // blocks of a tile
+  while (each > 1 && tiles * each > kShrinkBlocks) each /= 2;
+  const dim3 grid((unsigned)tiles, (unsigned)each), block(64 * kShrinkWaves);
+  if (a.rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XDT, TDT, 1>), grid, block, 0, s, a);
+  else if (a.rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XDT, TDT, 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((adapter_shrink_kernel<XDT, TDT, 4>), grid, block, 0, s, a);
+  NVJSEL_CHECK_LAUNCH("adapter_shrink_kernel");
   return NVJSEL_OK;
 }
 
 template <int TDT>
 static int launch_adapters(const AdapterArgs& a, int x_dtype, int out_dtype, hipStream_t s) {
-  const dim3 grid((unsigned)((a.rows + 15) / 16), 16), block(64 * kShrinkWaves);
-  if (x_dtype == DT_F32) hipLaunchKernelGGL((adapter_shrink_kernel<DT_F32, TDT>), grid, block, 0, s, a);
-  else if (x_dtype == DT_BF16) hipLaunchKernelGGL((adapter_shrink_kernel<DT_BF16, TDT>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((adapter_shrink_kernel<DT_F16, TDT>), grid, block, 0, s, a);
-  NVJSEL_CHECK_LAUNCH("adapter_shrink_kernel");
+  const int rc = x_dtype == DT_F32    ? launch_shrink<DT_F32, TDT>(a, s)
+                 : x_dtype == DT_BF16 ? launch_shrink<DT_BF16, TDT>(a, s)
+                                      : launch_shrink<DT_F16, TDT>(a, s);
+  if (rc != NVJSEL_OK) return rc;
   auto expand = [&](auto O) -> int {
     constexpr int ODT = decltype(O)::value;
-    if (a.rows <= 16) return launch_expand_rows<TDT, ODT, 1>(a, s);
-    return launch_expand_rows<TDT, ODT, 2>(a, s);
+    if (a.rank == 16) {
+      if (a.rows <= 16) return launch_expand<TDT, ODT, false, 1>(a, s);
+      if (a.rows <= 32) return launch_expand<TDT, ODT, false, 2>(a, s);
+      return launch_expand<TDT, ODT, false, 4>(a, s);
+    }
+    if (a.rows <= 16 || a.rank > 256) return launch_expand<TDT, ODT, true, 1>(a, s);
+    return launch_expand<TDT, ODT, true, 2>(a, s);
   };
   if (out_dtype == DT_F32) return expand(std::integral_constant<int, DT_F32>{});
   if (out_dtype == DT_BF16) return expand(std::integral_constant<int, DT_BF16>{});
@@ -441,7 +582,7 @@ using namespace nvjsel;
 
 static bool adapter_sizes_ok(int table_dtype, int64_t rows, int rank) {
   return (table_dtype == NVJSEL_BF16 || table_dtype == NVJSEL_F16) && rows > 0 && rows <= (1 << 20) &&
-         (rank == 8 || rank == 16 || (rank > 0 && rank <= kAdapterRank && rank % 32 == 0));
+         (rank == 16 || (rank > 0 && rank <= kAdapterRank && rank % 32 == 0));
 }
 
 extern "C" size_t nvjsel_adapters_workspace_size(int table_dtype, int64_t rows, int rank) {
@@ -451,6 +592,37 @@ extern "C" size_t nvjsel_adapters_workspace_size(int table_dtype, int64_t rows, 
     return 0;
   }
   return align_up((size_t)rows * adapter_terms(table_dtype) * rank * 2, 16) + (size_t)rows * 4;
+}
+
+extern "C" int nvjsel_adapters_pack(const void* plain, int which, int64_t count_stride, int64_t row_stride, int count, int rank,
+                                    int hidden, int width, int rank_pad, void* packed, size_t packed_bytes, void* stream) {
+  clear_error();
+  if (which != 0 && which != 1) return fail(NVJSEL_EINVAL, "adapters_pack: which must be 0 (a) or 1 (b)");
+  if (count <= 0 || rank <= 0 || hidden <= 0 || width <= 0) return fail(NVJSEL_EINVAL, "adapters_pack requires non-empty dimensions");
+  if (!adapter_sizes_ok(NVJSEL_BF16, 1, rank_pad) || rank > rank_pad || hidden > (1 << 24) || width > (1 << 28))
+    return fail(NVJSEL_EINVAL, "adapters_pack: bad sizes");
+  if (!plain || !packed) return fail(NVJSEL_EINVAL, "adapters_pack: null pointer");
+  if (((uintptr_t)plain & 1) || ((uintptr_t)packed & 15)) return fail(NVJSEL_EINVAL, "adapters_pack: unaligned pointer");
+  if (count_stride < 0 || row_stride < 0) return fail(NVJSEL_EINVAL, "adapters_pack: negative stride");
+  AdapterPack p{};
+  p.from = (const uint16_t*)plain;
+  p.count_stride = count_stride;
+  p.row_stride = row_stride;
+  p.rank = rank;
+  p.hidden = hidden;
+  p.width = width;
+  p.rank_pad = rank_pad;
+  p.hidden_pad = (hidden + 31) / 32 * 32;
+  p.width_pad = (width + 63) / 64 * 64;
+  p.to = (uint4*)packed;
+  p.pieces = (int64_t)count * rank_pad * (which ? p.width_pad : p.hidden_pad) / 8;
+  if (packed_bytes < (size_t)p.pieces * 16) return fail(NVJSEL_EINVAL, "adapters_pack: the table is too small");
+  if (p.pieces / 256 >= 1 << 23) return fail(NVJSEL_EINVAL, "adapters_pack: too many values for a call");
+  const dim3 grid((unsigned)((p.pieces + 255) / 256));
+  if (which) hipLaunchKernelGGL((adapter_pack_kernel<true>), grid, dim3(256), 0, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL((adapter_pack_kernel<false>), grid, dim3(256), 0, (hipStream_t)stream, p);
+  NVJSEL_CHECK_LAUNCH("adapter_pack_kernel");
+  return NVJSEL_OK;
 }
 
 extern "C" int nvjsel_apply_adapters(const void* x, int x_dtype, int64_t x_stride, const void* base, int out_dtype,
@@ -469,10 +641,11 @@ extern "C" int nvjsel_apply_adapters(const void* x, int x_dtype, int64_t x_strid
     return NVJSEL_EINVAL;
   }
   if (!adapter_sizes_ok(table_dtype, rows, rank)) {
-    set_error("apply_adapters: rank (%d) must be 8, 16 or a multiple of 32 up to %d, rows (%lld) at most 2^20", rank,
+    set_error("apply_adapters: rank (%d) must be 16 or a multiple of 32 up to %d, rows (%lld) at most 2^20", rank,
               kAdapterRank, (long long)rows);
     return NVJSEL_EINVAL;
   }
+  if (hidden < 8) return fail(NVJSEL_EUNSUPPORTED, "apply_adapters: hidden below 8 (pad x with zeros)");
   if (hidden > (1 << 24) || width > (1 << 28)) return fail(NVJSEL_EINVAL, "apply_adapters: hidden or width too large");
   if (!x || !base || !a_table || !b_table || !scales || !ids || !out) return fail(NVJSEL_EINVAL, "apply_adapters: null pointer");
   if ((((uintptr_t)a_table) | ((uintptr_t)b_table)) & 15) return fail(NVJSEL_EINVAL, "apply_adapters: unaligned tables");
@@ -500,6 +673,7 @@ extern "C" int nvjsel_apply_adapters(const void* x, int x_dtype, int64_t x_strid
   g.rank = rank;
   g.width = width;
   g.count = count;
+  g.width_pad = (width + 63) / 64 * 64;
   g.terms = (uint16_t*)workspace;
   g.row_scale = (float*)((char*)workspace + align_up((size_t)rows * adapter_terms(table_dtype) * rank * 2, 16));
   g.base = base;

@@ -57,6 +57,7 @@ SIGNATURES = {
     "nvjsel_lm_head_token_logprobs_workspace_size": (_sz, [_i, _i, _i, _i64, _i, _i]),
     "nvjsel_lm_head_token_logprobs": (_i, [_vp, _i, _vp, _i, _i, _i64, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
     "nvjsel_adapters_workspace_size": (_sz, [_i, _i64, _i]),
+    "nvjsel_adapters_pack": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "nvjsel_apply_adapters": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _i64, _vp, _i64,
                                    _vp, _sz, _vp]),
     "nvjsel_debug_gumbel_draws": (_i, [ctypes.c_uint32, _i, _vp, _vp, _vp]),

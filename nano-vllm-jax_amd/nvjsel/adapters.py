@@ -9,6 +9,7 @@ when they are loaded; the ``AdapterTable`` it returns is also taken by
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -17,30 +18,30 @@ from ._tensors import _TORCH_DTYPES, _dtype_code, _on_device, _require_cuda, _st
 
 MAX_RANK = 512
 MAX_ROWS = 1 << 20
+_MIN_HIDDEN = 8
 _TABLE_DTYPES = (torch.bfloat16, torch.float16)
 
 
 @dataclass(frozen=True)
 class AdapterTable:
-    """Adapters laid out for the kernels: ``rank`` and ``a``'s last dimension rounded up, zeros behind."""
+    """Adapters laid out for the kernels."""
 
-    a: torch.Tensor  # [count, rank, hidden rounded up to 32]
-    b: torch.Tensor  # [count, width, rank]
+    a: torch.Tensor  # [count, rank * hidden], both rounded up
+    b: torch.Tensor  # [count, width * rank], likewise
     scales: torch.Tensor  # f32 [count]
     hidden: int
     width: int
+    rank: int  # rounded up to 16 or a multiple of 32
 
     @property
     def count(self) -> int:
         return int(self.a.shape[0])
 
-    @property
-    def rank(self) -> int:
-        return int(self.a.shape[1])
-
 
 def _no_gradient(who: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+    if not torch.is_grad_enabled():
+        return
+    if any(t is not None and t.requires_grad for t in ts):
         raise ValueError(f"{who} is not differentiable: call it under torch.no_grad() or on detached tensors")
 
 
@@ -50,6 +51,10 @@ def pack_adapters(a, b, scales=None) -> AdapterTable:
 
     ``scales`` (f32 ``[L]`` or numbers; 1 where None) multiply the adapters' parts, ``alpha / R`` as
     a rule.  Ranks may differ, up to 512."""
+    if torch.is_tensor(a) and torch.is_tensor(b) and a.ndim == b.ndim == 3 and a.shape[0] == b.shape[0]:
+        plain = [(a, b)]  # all of one rank: one launch each
+    else:
+        plain = [(s[None], t[None]) for s, t in zip(a, b)]
     a, b = list(a), list(b)
     if not a or len(a) != len(b):
         raise ValueError("pack_adapters takes one a and one b for every adapter, at least one")
@@ -71,20 +76,32 @@ def pack_adapters(a, b, scales=None) -> AdapterTable:
     if hidden > 1 << 24 or width > 1 << 28:
         raise ValueError("hidden must be at most 2^24 and width 2^28")
     dev = _require_cuda(*a, *b)
-    rank = 8 if most <= 8 else 16 if most <= 16 else (most + 31) // 32 * 32
-    with torch.no_grad():
-        pa = torch.zeros((len(a), rank, (hidden + 31) // 32 * 32), dtype=dtype, device=dev)
-        pb = torch.zeros((len(b), width, rank), dtype=dtype, device=dev)
-        for i, (s, t) in enumerate(zip(a, b)):
-            pa[i, : s.shape[0], :hidden] = s
-            pb[i, :, : t.shape[1]] = t
-        if scales is None:
-            ps = torch.ones((len(a),), dtype=torch.float32, device=dev)
-        else:
-            ps = torch.as_tensor(scales, dtype=torch.float32, device=dev).detach().reshape(-1).clone()
-            if ps.numel() != len(a):
-                raise ValueError("scales must have one value for every adapter")
-    return AdapterTable(pa, pb, ps, hidden, width)
+    rank = 16 if most <= 16 else (most + 31) // 32 * 32
+    pa = torch.empty((len(a), rank * ((hidden + 31) // 32 * 32)), dtype=dtype, device=dev)
+    pb = torch.empty((len(a), rank * ((width + 63) // 64 * 64)), dtype=dtype, device=dev)
+    if scales is None:
+        ps = torch.ones((len(a),), dtype=torch.float32, device=dev)
+    else:
+        ps = torch.as_tensor(scales, dtype=torch.float32, device=dev).detach().reshape(-1).clone()
+        if ps.numel() != len(a):
+            raise ValueError("scales must have one value for every adapter")
+    with _on_device(dev):
+        at = 0
+        for s, t in plain:
+            n, own = int(s.shape[0]), int(s.shape[1])
+            for which, (p, to) in enumerate(((s, pa[at:]), (t, pb[at:]))):
+                if p.stride(2) != 1 and p.shape[2] > 1:
+                    p = p.contiguous()
+                _lib.call("nvjsel_adapters_pack", p.data_ptr(), which, p.stride(0) if n > 1 else 0,
+                          p.stride(1) if p.shape[1] > 1 else 0, n, own, hidden, width, rank, to.data_ptr(),
+                          to.numel() * to.element_size(), _stream_handle(dev))
+            at += n
+    return AdapterTable(pa, pb, ps, hidden, width, rank)
+
+
+@lru_cache(maxsize=1024)
+def _bytes(*shape: int) -> int:
+    return _lib.load().nvjsel_adapters_workspace_size(*shape)
 
 
 def _rows(t: torch.Tensor, rows: int) -> torch.Tensor:
@@ -120,39 +137,47 @@ def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, 
     ``out`` receives it (``base`` itself for in place), a new tensor where None.  A NaN or an infinity
     in a row of ``x``, or in its own adapter, makes that row's results NaN and no other's.
     Not differentiable."""
-    if x.ndim < 1 or base.ndim != x.ndim or x.shape[:-1] != base.shape[:-1] or adapter_ids.shape != x.shape[:-1]:
+    rows_shape, hidden, width = adapter_ids.shape, adapters.hidden, adapters.width
+    if x.ndim < 1 or base.ndim < 1 or x.shape[:-1] != rows_shape or base.shape[:-1] != rows_shape:
         raise ValueError("apply_adapters takes x [..., H], base [..., D] and one adapter id for every row")
-    if x.numel() == 0 or base.numel() == 0:
+    rows = adapter_ids.numel()
+    if rows == 0:
         raise ValueError("apply_adapters requires non-empty dimensions")
-    if x.shape[-1] != adapters.hidden or base.shape[-1] != adapters.width:
-        raise ValueError(f"the adapters are of hidden {adapters.hidden} and width {adapters.width} "
-                         f"(got {x.shape[-1]} and {base.shape[-1]})")
+    if x.shape[-1] != hidden or base.shape[-1] != width:
+        raise ValueError(f"the adapters are of hidden {hidden} and width {width} (got {x.shape[-1]} and {base.shape[-1]})")
     xd, od = _dtype_code(x, "x"), _dtype_code(base, "base")
     if adapter_ids.dtype != torch.int32:
         raise ValueError(f"adapter_ids must be int32 (got {adapter_ids.dtype})")
-    rows = adapter_ids.numel()
     if rows > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows (got {rows})")
-    if out is not None and (out.shape != base.shape or out.dtype != base.dtype):
-        raise ValueError("out must have base's shape and type")
-    _no_gradient("apply_adapters", x, base, out, adapters.a, adapters.b, adapters.scales)
-    dev = _require_cuda(x, base, adapters.a, adapters.b, adapters.scales, adapter_ids, out)
-    result = torch.empty(base.shape, dtype=base.dtype, device=dev) if out is None else out
-    try:
-        flat = result.view(rows, adapters.width)
-    except RuntimeError:
-        raise ValueError("out's rows must be apart by one stride") from None
-    if (flat.stride(1) != 1 and adapters.width > 1) or _stride(flat) < adapters.width:
+    _no_gradient("apply_adapters", x, base, out)
+    a = adapters.a
+    dev = _require_cuda(x, base, a, adapter_ids)
+    if out is None:
+        result = flat = torch.empty(base.shape, dtype=base.dtype, device=dev)
+    else:
+        if out.shape != base.shape or out.dtype != base.dtype or out.device != dev:
+            raise ValueError("out must have base's shape, type and device")
+        result, flat = out, out
+    if x.ndim != 2:
+        try:
+            flat = result.view(rows, width)
+        except RuntimeError:
+            raise ValueError("out's rows must be apart by one stride") from None
+    if out is not None and ((flat.stride(1) != 1 and width > 1) or _stride(flat) < width):
         raise ValueError("out's rows must be contiguous and must not overlap")
     x, base, ids = _rows(x, rows), _rows(base, rows), adapter_ids.reshape(rows).contiguous()
     if out is not None and (base.data_ptr(), _stride(base)) != (flat.data_ptr(), _stride(flat)) and _meet(base, flat):
         raise ValueError("out must be base itself or share no memory with it")
+    if hidden < _MIN_HIDDEN:  # zeros beside the table's zeros
+        x = torch.nn.functional.pad(x, (0, _MIN_HIDDEN - hidden))
+        hidden = _MIN_HIDDEN
     with _on_device(dev):
-        nbytes = _lib.load().nvjsel_adapters_workspace_size(_TORCH_DTYPES[adapters.a.dtype], rows, adapters.rank)
+        td = _TORCH_DTYPES[a.dtype]
+        nbytes = _bytes(td, rows, adapters.rank)
         stream = _stream_handle(dev)
         ws = _workspace(dev, stream, "adapters", nbytes, 0)
-        _lib.call("nvjsel_apply_adapters", x.data_ptr(), xd, _stride(x), base.data_ptr(), od, _stride(base),
-                  adapters.a.data_ptr(), adapters.b.data_ptr(), _TORCH_DTYPES[adapters.a.dtype],
-                  adapters.scales.data_ptr(), adapters.count, adapters.rank, adapters.hidden, adapters.width,
+        _lib.call("nvjsel_apply_adapters", x.data_ptr(), xd, _stride(x), base.data_ptr(), od, _stride(base), a.data_ptr(),
+                  adapters.b.data_ptr(), td, adapters.scales.data_ptr(), a.shape[0], adapters.rank, hidden, width,
                   ids.data_ptr(), rows, flat.data_ptr(), _stride(flat), ws.data_ptr(), nbytes, stream)
     return result

@@ -33,9 +33,8 @@ def test_pack_refusals(a, b, kw, what):
         nvjsel.pack_adapters(a, b, **kw)
 
 
-def _table(hidden=8, width=6, rank=8, count=2):
-    return nvjsel.AdapterTable(_t(count, rank, (hidden + 31) // 32 * 32), _t(count, width, rank),
-                               _t(count, dtype=torch.float32), hidden, width)
+def _table(hidden=8, width=6, rank=16, count=2):
+    return nvjsel.AdapterTable(_t(count, rank * 32), _t(count, 64 * rank), _t(count, dtype=torch.float32), hidden, width, rank)
 
 
 @pytest.mark.parametrize("change,what", [
@@ -43,8 +42,7 @@ def _table(hidden=8, width=6, rank=8, count=2):
     ({"base": _t(2, 6)}, "one adapter id"), ({"x": _t(0, 8), "base": _t(0, 6), "ids": _t(0, dtype=torch.int32)}, "non-empty"),
     ({"x": _t(3, 9)}, "hidden 8 and width 6"), ({"base": _t(3, 7)}, "hidden 8 and width 6"),
     ({"x": _t(3, 8, dtype=torch.float64)}, "unsupported x"), ({"base": _t(3, 6, dtype=torch.int16)}, "unsupported base"),
-    ({"ids": _t(3, dtype=torch.int64)}, "int32"), ({"out": _t(3, 7)}, "shape and type"),
-    ({"out": _t(3, 6, dtype=torch.float32)}, "shape and type"), ({"x": _t(3, 8).requires_grad_()}, "not differentiable"),
+    ({"ids": _t(3, dtype=torch.int64)}, "int32"),  ({"x": _t(3, 8).requires_grad_()}, "not differentiable"),
     ({"base": _t(3, 6).requires_grad_()}, "not differentiable"), ({}, "device tensors"),
     ({"x": _t(1, 8).expand((1 << 20) + 1, 8), "base": _t(1, 6).expand((1 << 20) + 1, 6),
       "ids": _t(1, dtype=torch.int32).expand((1 << 20) + 1)}, "at most"),
@@ -60,6 +58,9 @@ def test_outputs_that_meet_the_base(monkeypatch):
     monkeypatch.setattr(module, "_require_cuda", lambda *ts: ts[0].device)
     buf = _t(10, 40)
     ids = _t(3, dtype=torch.int32)
+    for out in (_t(3, 7), _t(3, 6, dtype=torch.float32)):
+        with pytest.raises(ValueError, match="shape, type and device"):
+            nvjsel.apply_adapters(_t(3, 8), _t(3, 6), _table(), ids, out=out)
     for base, out, what in ((buf[:3, :6], buf[1:4, :6], "share no memory"), (buf[:3, :6], buf[:3, 3:9], "share no memory"),
                             (buf[:3, :6], buf[0:6:2, :6], "share no memory"), (_t(3, 6), _t(1, 6).expand(3, 6), "must not overlap"),
                             (_t(3, 6), _t(6, 3).T, "contiguous")):
@@ -96,6 +97,7 @@ P = 1 << 20  # an address that nothing reads: every call here is refused
     ({"a": P + 8}, "unaligned tables"), ({"b": P + 2}, "unaligned tables"), ({"x": P + 1}, "unaligned rows"),
     ({"out": P + 1}, "unaligned rows"), ({"xs": -1}, "negative"), ({"bs": -4}, "negative"), ({"os": 5}, "stride < width"),
     ({"base": P, "out": P, "bs": 7, "os": 6}, "another stride"), ({"ws": None}, "workspace"), ({"wsb": 16}, "workspace"),
+    ({"hidden": 7}, "below 8"), ({"rank": 8}, "rank"),
     ({"hidden": (1 << 24) + 1}, "too large"), ({"width": (1 << 28) + 1, "os": 1 << 30}, "too large"),
 ])
 def test_c_refusals(change, what):
@@ -104,6 +106,21 @@ def test_c_refusals(change, what):
     a.update(change)
     lib = nvjsel.load()
     assert lib.nvjsel_apply_adapters(*a.values()) < 0 and what in lib.nvjsel_last_error().decode()
+
+
+@pytest.mark.parametrize("change,what", [
+    ({"which": 2}, "which"), ({"count": 0}, "non-empty"), ({"rank": 0}, "non-empty"), ({"hidden": 0}, "non-empty"),
+    ({"width": 0}, "non-empty"), ({"rank": 17}, "bad sizes"), ({"pad": 24}, "bad sizes"), ({"pad": 544, "rank": 530}, "bad sizes"),
+    ({"plain": None}, "null"), ({"packed": None}, "null"), ({"plain": P + 1}, "unaligned"), ({"packed": P + 8}, "unaligned"),
+    ({"cs": -1}, "negative"), ({"rs": -1}, "negative"), ({"bytes": 2 * 16 * 32 * 2 - 1}, "too small"),
+    ({"width": 1 << 28, "which": 1, "bytes": 1 << 60, "pad": 512}, "too many"),
+])
+def test_c_pack_refusals(change, what):
+    a = {"plain": P, "which": 0, "cs": 128, "rs": 8, "count": 2, "rank": 16, "hidden": 8, "width": 6, "pad": 16, "packed": P,
+         "bytes": 1 << 20, "stream": None}
+    a.update(change)
+    lib = nvjsel.load()
+    assert lib.nvjsel_adapters_pack(*a.values()) < 0 and what in lib.nvjsel_last_error().decode()
 
 
 def test_workspace_sizes():
