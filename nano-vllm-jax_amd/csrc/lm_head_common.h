@@ -36,7 +36,8 @@ __device__ __forceinline__ u32x4_t shift_down8(u32x4_t w, int s) {
 // GREEDY: argmax id per row; SAMPLE: Gumbel-max id per row; LOGITS: the
 // (REDUCE_CAST-rounded) logits themselves, written to out_logits; SCORE: log
 // probabilities of given tokens (and entropies), lm_head_score.hip.
-enum { MODE_GREEDY = 0, MODE_SAMPLE = 1, MODE_LOGITS = 2, MODE_SCORE = 3, MODE_SCORE_ENTROPY = 4 };
+enum { MODE_GREEDY = 0, MODE_SAMPLE = 1, MODE_LOGITS = 2, MODE_SCORE = 8 };
+enum { SCORE_ENTROPY = 1, SCORE_CAST = 2 };  // added to MODE_SCORE
 
 struct LmArgs {
   const void* W;

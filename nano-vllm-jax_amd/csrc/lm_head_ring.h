@@ -64,7 +64,8 @@ template <int MODE, int NBR, int NS>
 struct RingShape {
   static_assert(NS == 1 || (NS == 3 && NBR <= 64), "the terms' slots fit the LDS");
   static constexpr bool SMP = MODE == MODE_SAMPLE;
-  static constexpr bool SCORE = MODE == MODE_SCORE || MODE == MODE_SCORE_ENTROPY, ENT = MODE == MODE_SCORE_ENTROPY;
+  // scoring: with the entropy, of logits rounded to the weight's type
+  static constexpr bool SCORE = MODE >= MODE_SCORE, ENT = SCORE && (MODE & SCORE_ENTROPY), CAST = SCORE && (MODE & SCORE_CAST);
   static constexpr int NW = 8;                        // waves; one block per CU
   static constexpr int BV = 256;                      // vocabulary rows of a block tile
   static constexpr int TB = NBR <= 32 || NS == 3 ? 1 : 2;  // 32-row batch tiles per wave
@@ -253,11 +254,15 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       for (int t = 0; t < 3; ++t) *(uint2*)(at + t * (NBR * kRingKC * 2)) = next_term(v);
     }
   };
-  auto issue_w = [&]() NVJSEL_INLINE {
+  auto issue_w_part = [&](auto FROM, auto TO) NVJSEL_INLINE {
     const uint32_t dst = ring0 + (uint32_t)(lw * WBYTES);
     const char* src = wtile + lko;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) dma16_nt(src, woff[i], dst + (uint32_t)((i * NW + wave) * 1024));
+    for (int i = decltype(FROM)::value; i < decltype(TO)::value; ++i)
+      dma16_nt(src, woff[i], dst + (uint32_t)((i * NW + wave) * 1024));
+  };
+  auto issue_w_from = [&](auto FROM) NVJSEL_INLINE {
+    issue_w_part(FROM, std::integral_constant<int, WL>{});
     lw = lw + 1 == RW ? 0 : lw + 1;
     lko += lstep;
     if (--lleft == 0) {
@@ -276,6 +281,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       }
     }
   };
+  auto issue_w = [&]() NVJSEL_INLINE { issue_w_from(std::integral_constant<int, 0>{}); };
   f32x16_t acc[TV][TB];
   const int h = lane >> 5, c32 = lane & 31, sw = (c32 >> 1) & 7;
   // Fragments are read one 16-wide k-step ahead of the products, across the
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       for (int tb = 0; tb < TB; ++tb) fb[f][t][tb] = *(const u32x4_t*)(xbuf + (t * NBR + tb * 32) * (kRingKC * 2));
 #pragma unroll
     for (int tv = 0; tv < TV; ++tv) fa[f][tv] = *(const u32x4_t*)(wbuf + tv * 32 * (kRingKC * 2));
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!S::SCORE) __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](auto set) NVJSEL_INLINE {
     constexpr int f = decltype(set)::value;
@@ -306,6 +312,13 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
         for (int tb = 0; tb < TB; ++tb)
           acc[tv][tb] = MODE == MODE_LOGITS ? mfma32x32x16<WT>(fb[f][t][tb], fa[f][tv], acc[tv][tb])
                                             : mfma32x32x16<WT>(fa[f][tv], fb[f][t][tb], acc[tv][tb]);
+    if constexpr (S::SCORE) {  // the next step's reads between this step's products
+#pragma unroll
+      for (int i = 0; i < TV * TB * NS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
   using I0 = std::integral_constant<int, 0>;
@@ -319,15 +332,20 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       issue_raw();
     else
       issue_x();
-    issue_w();
+    constexpr bool PARTS = S::SCORE && NS == 1;  // W's requests in two parts, among the products
+    using Half = std::integral_constant<int, WL / 2>;
+    if constexpr (!PARTS) issue_w();
     read_step(I0{}, I0{});
     if constexpr (decltype(rest)::value) multiply(I1{});
+    else if constexpr (S::SCORE) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (PARTS) issue_w_part(I0{}, Half{});
     read_step(I1{}, I1{});
     multiply(I0{});
     if constexpr (NS == 3) {
       wave_wait<WL>();  // the W stage requested behind the raw values stays in flight
       split_raw();
     }
+    if constexpr (PARTS) issue_w_from(Half{});
     read_step(I0{}, I2{});
     multiply(I1{});
     read_step(I1{}, I3{});
@@ -539,8 +557,11 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     }
   }
   // Adds a tile's logits: differences from the new maximum, so that no size of logits is far
-  // off; -inf (a row past the end) is 0 in both sums.
+  // off; -inf (a row past the end starts there) is 0 in both sums.  The products' registers are
+  // read, never written, by one path: copies of them spill (2048 rows 950 us; with the rounding and
+  // the rows past the end as paths of their own 1032, writing them 1209).
   auto score_tile = [&](int v0) NVJSEL_INLINE {
+    auto logit = [&](int tv, int tb, int e) NVJSEL_INLINE { return apply_cast(acc[tv][tb][e], S::CAST ? (WT == DT_BF16 ? 1 : 2) : 0); };
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
       const int rel = stok[tb] - v0;
@@ -549,20 +570,20 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
         const int at = (rel >> 5) * 16 + ((rel & 31) >> 3) * 4 + (rel & 3);
 #pragma unroll
         for (int i = 0; i < TV * 16; ++i)
-          if (i == at) x = acc[i / 16][tb][i % 16];
+          if (i == at) x = logit(i / 16, tb, i % 16);
         if (rel >= 0 && rel < TV * 32 && (rel >> 2 & 1) == h) sc.token_logits[b0 + wb * 32 * TB + tb * 32 + c32] = x;
       }
-      float m = acc[0][tb][0];
+      float m = smax[tb];
 #pragma unroll
-      for (int i = 1; i < TV * 16; ++i) m = __builtin_elementwise_maximum(m, acc[i / 16][tb][i % 16]);
-      const float to = __builtin_elementwise_maximum(smax[tb], m), base = to == -INFINITY ? 0.0f : to;
+      for (int i = 0; i < TV * 16; ++i) m = __builtin_elementwise_maximum(m, logit(i / 16, tb, i % 16));
+      const float base = m == -INFINITY ? 0.0f : m;
       float s = 0.0f, u = 0.0f;
 #pragma unroll
-      for (int g = 0; g < TV * 2; ++g) {  // eight at a time, so that few registers hold terms
+      for (int q = 0; q < TV * 2; ++q) {  // eight at a time, so that few registers hold terms
         float e[8], p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float y = (acc[g / 2][tb][g % 2 * 8 + i] - base) * kLog2e;
+          const float y = (logit(q / 2, tb, q % 2 * 8 + i) - base) * kLog2e;
           e[i] = __builtin_amdgcn_exp2f(y);
           if constexpr (S::ENT) p[i] = e[i] * fmaxf(y, -200.0f);
         }
@@ -574,7 +595,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       const double f = (double)__builtin_amdgcn_exp2f(d);
       if constexpr (S::ENT) ssum[tb].ent = f * (ssum[tb].ent + ssum[tb].sum * (double)d) + (double)u;
       ssum[tb].sum = f * ssum[tb].sum + (double)s;
-      smax[tb] = to;
+      smax[tb] = m;
     }
   };
   auto epilogue = [&](int t) NVJSEL_INLINE {
@@ -590,6 +611,15 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
           v = v0 + tv * 32 + (MODE == MODE_LOGITS ? c32 : row);
           return b < b0 + B && v < vend;
         });
+      if constexpr (S::SCORE) {  // (a row past the end may have met an infinity's terms)
+        if (__builtin_amdgcn_ballot_w64(m != m)) {
+#pragma unroll
+          for (int tv = 0; tv < TV; ++tv)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (v0 + tv * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= vend) acc[tv][0][e] = -INFINITY;
+        }
+      }
     }
     if constexpr (MODE == MODE_LOGITS) {
       // operands swapped: D[batch 8 (e >> 2) + 4 h + (e & 3)][vocab c32], so
@@ -638,6 +668,8 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
       pvend = vend;
       punit = 0;
       credit = wave >= NW / 2 ? nkc / 2 : 0;
+    } else if constexpr (S::SCORE) {
+      score_tile(v0);
     } else {
       if (v0 + TV * 32 > vend) {  // rows past the tile's end repeat its last row
 #pragma unroll
@@ -648,18 +680,6 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
 #pragma unroll
               for (int tb = 0; tb < TB; ++tb) acc[tv][tb][e] = -INFINITY;
             }
-      }
-      if constexpr (S::SCORE) {
-        if (a.reduce_cast) {
-#pragma unroll
-          for (int tv = 0; tv < TV; ++tv)
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) acc[tv][tb][e] = apply_cast(acc[tv][tb][e], a.reduce_cast);
-        }
-        score_tile(v0);
-        return;
       }
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) {
@@ -726,6 +746,19 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
         for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[tv][tb][e] = 0.f;
+      if constexpr (S::SCORE) {  // rows past the share's end, which repeat its last row, start and stay at -inf
+        const int past = r1 - (tile_row(t) + wv * TV * 32) - 4 * h;
+        if (t == my_tiles - 1) {
+#pragma unroll
+          for (int tv = 0; tv < TV; ++tv)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float start = tv * 32 + 8 * (e >> 2) + (e & 3) < past ? 0.0f : -INFINITY;
+#pragma unroll
+              for (int tb = 0; tb < TB; ++tb) acc[tv][tb][e] = start;
+            }
+        }
+      }
       stage(std::false_type{});
       for (int kc = 1; kc < nkc; ++kc) {
         if constexpr (S::SMP) score_share();

@@ -7,7 +7,7 @@
 // (bf16; 2 GB f32) beside a product of 1.04 TFLOP.  A lane holds 16 logits of one column (batch row) per
 // 32-row tile, so that the sums cross no lanes until a block's share of the vocabulary
 // ends; a share's parts are joined by a second kernel, a wave a row.
-#include "lm_head_ring.h"
+#include "lm_head_score.h"
 
 namespace nvjsel {
 
@@ -29,60 +29,48 @@ __global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, c
   row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r);
 }
 
+int launch_score_finish(const RowAnswers& answers, const ScoreArgs& sc, int rows, int vocab, hipStream_t s) {
+  hipLaunchKernelGGL(score_finish_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, answers,
+                     (const float*)sc.token_logits, (const RowPart*)sc.parts, rows, sc.shares, vocab);
+  NVJSEL_CHECK_LAUNCH("score_finish_kernel");
+  return NVJSEL_OK;
+}
+
 // Rows of a block: 256 while more than 128 are left (64 of f32 activations, three products each).
 static int score_block_rows(bool f32, int64_t left) {
   if (f32) return left > 32 ? 64 : 32;
   return left > 128 ? 256 : left > 64 ? 128 : left > 32 ? 64 : 32;
 }
 
-// Row blocks of a launch: as many of those left as give the most rows per round of tiles, where
-// every CU has one block (5 of 51 shares each fill 255 CUs, 29 of 8 fill 232, 16 and 13 256 and 247);
-// a launch costs about as much as half a tile.
+// Row blocks of the next launch: a call of n blocks is cut so that the rounds of tiles, half a tile for a
+// launch, are fewest over all (every CU has one block: 5 of 51 shares each fill 255 CUs, 29 of 8
+// fill 232, 16 and 13 256 and 247).
+static constexpr int kScoreBlocks = 32;  // of a launch at most
 static int score_row_blocks(int64_t left, int vocab, int cus) {
-  int best = 1;
-  double most = 0.0;
-  for (int r = 1; r <= 32 && r <= left && r <= cus; ++r) {
-    const double rate = r / (0.5 + ring_tiles(ring_share(vocab, cus / r)));
-    if (rate >= most) {
-      most = rate;
-      best = r;
-    }
+  const int most = cus < kScoreBlocks ? cus : kScoreBlocks;
+  double cost[kScoreBlocks + 1], total[2 * kScoreBlocks + 1];
+  int first[2 * kScoreBlocks + 1];
+  int whole = 1;  // the launch of most rows a round, while more than two of the largest are left
+  for (int r = 1; r <= most; ++r) {
+    cost[r] = 0.5 + ring_tiles(ring_share(vocab, cus / r));
+    if (r * cost[whole] >= whole * cost[r]) whole = r;
   }
-  return best;
+  if (left > 2 * most) return whole;
+  total[0] = 0.0;
+  for (int n = 1; n <= (int)left; ++n) {
+    first[n] = 1;
+    total[n] = 1e30;
+    for (int r = 1; r <= most && r <= n; ++r)
+      if (cost[r] + total[n - r] <= total[n]) {
+        total[n] = cost[r] + total[n - r];
+        first[n] = r;
+      }
+  }
+  return first[left];
 }
 
 static size_t score_bytes(int64_t rows, int cus) {  // parts: at most `cus` shares x row blocks of 256 rows
   return align_up((size_t)rows * 4, 16) + (size_t)cus * 256 * sizeof(RowPart);
-}
-
-template <int WT, int MODE, int NBR, int NS>
-static int launch_score_rows(const LmArgs& a, ScoreArgs sc, const RowAnswers& answers, hipStream_t s) {
-  const int rows = ring_share(a.V, device_cu_count() / sc.row_blocks);
-  sc.shares = (a.V + rows - 1) / rows;
-  hipLaunchKernelGGL((lm_head_ring_kernel<WT, MODE, NBR, NS>), dim3((unsigned)(sc.shares * sc.row_blocks)),
-                     dim3(RingShape<MODE, NBR, NS>::NW * 64), 0, s, a, rows, sc);
-  NVJSEL_CHECK_LAUNCH("lm_head_ring_kernel");
-  hipLaunchKernelGGL(score_finish_kernel, dim3((unsigned)((a.B + 3) / 4)), dim3(256), 0, s, answers,
-                     (const float*)sc.token_logits, (const RowPart*)sc.parts, a.B, sc.shares, a.V);
-  NVJSEL_CHECK_LAUNCH("score_finish_kernel");
-  return NVJSEL_OK;
-}
-
-template <int MODE>
-static int launch_score(const LmArgs& a, const ScoreArgs& sc, const RowAnswers& w, int block_rows, hipStream_t s) {
-  if (a.hidden_dtype == DT_F32) {
-    if (block_rows == 32) return launch_score_rows<DT_BF16, MODE, 32, 3>(a, sc, w, s);
-    return launch_score_rows<DT_BF16, MODE, 64, 3>(a, sc, w, s);
-  }
-  auto by_rows = [&](auto T) -> int {
-    constexpr int WT = decltype(T)::value;
-    if (block_rows == 32) return launch_score_rows<WT, MODE, 32, 1>(a, sc, w, s);
-    if (block_rows == 64) return launch_score_rows<WT, MODE, 64, 1>(a, sc, w, s);
-    if (block_rows == 128) return launch_score_rows<WT, MODE, 128, 1>(a, sc, w, s);
-    return launch_score_rows<WT, MODE, 256, 1>(a, sc, w, s);
-  };
-  if (a.weight_dtype == DT_F16) return by_rows(std::integral_constant<int, DT_F16>{});
-  return by_rows(std::integral_constant<int, DT_BF16>{});
 }
 
 }  // namespace nvjsel
@@ -128,6 +116,8 @@ extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtyp
   if (rc != NVJSEL_OK) return rc;
   if (!hidden || !weight || !tokens || !out_logprobs) return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: null pointer");
   if (reduce_cast < 0 || reduce_cast > 2) return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: reduce_cast must be 0, 1 or 2");
+  if (reduce_cast && reduce_cast != (hidden_dtype == NVJSEL_F32 ? 0 : weight_dtype))
+    return fail(NVJSEL_EUNSUPPORTED, "lm_head_token_logprobs: reduce_cast must be 0 or the type of 16-bit operands");
   if ((token_bytes != 4 && token_bytes != 8) || ((uintptr_t)tokens & (token_bytes - 1)))
     return fail(NVJSEL_EINVAL, "lm_head_token_logprobs: tokens must be int32 or int64, aligned");
   if ((((uintptr_t)hidden) | ((uintptr_t)weight)) & 15)
@@ -165,8 +155,9 @@ extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtyp
     a.V = vocab;
     a.reduce_cast = reduce_cast;
     const RowAnswers answers{sc.tokens, sc.token64, out_logprobs + r0, out_entropy ? out_entropy + r0 : nullptr, nullptr};
-    const int st = out_entropy ? launch_score<MODE_SCORE_ENTROPY>(a, sc, answers, block_rows, s)
-                               : launch_score<MODE_SCORE>(a, sc, answers, block_rows, s);
+    const int st = hidden_dtype == NVJSEL_F32    ? launch_score_f32(a, sc, answers, block_rows, out_entropy, false, s)
+                   : weight_dtype == NVJSEL_BF16 ? launch_score_bf16(a, sc, answers, block_rows, out_entropy, reduce_cast, s)
+                                                 : launch_score_f16(a, sc, answers, block_rows, out_entropy, reduce_cast, s);
     if (st != NVJSEL_OK) return st;
   }
   return NVJSEL_OK;

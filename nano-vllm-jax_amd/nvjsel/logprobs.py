@@ -196,7 +196,10 @@ def _scored(x, output_weight, tokens, entropy, weight_layout, reduce_cast):
     nbytes = _score_bytes(dev.index, hd, wd, layout, int(x.shape[0]), int(x.shape[1]), vocab)
     if nbytes == 0:
         return None
-    rc = reference_reduce_cast(x.dtype, w.dtype) if reduce_cast is None else int(reduce_cast)
+    own = reference_reduce_cast(x.dtype, w.dtype)
+    rc = own if reduce_cast is None else int(reduce_cast)
+    if rc not in (0, own):
+        return None
     logprobs = torch.empty((x.shape[0],), dtype=torch.float32, device=dev)
     ent = torch.empty_like(logprobs) if entropy else None
     stream = _stream_handle(dev)

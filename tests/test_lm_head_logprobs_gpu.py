@@ -99,7 +99,7 @@ def test_many_row_blocks():
     check(*make(33 * 256 + 5, 64, 300, seed=6), reduce_cast=0)
 
 
-@pytest.mark.parametrize("kind", ["f32w", "mixed", "odd_hidden", "hv", "unaligned"])
+@pytest.mark.parametrize("kind", ["f32w", "mixed", "odd_hidden", "hv", "cast", "unaligned"])
 def test_other_calls_by_logits(kind):
     if kind == "f32w":
         check(*make(40, 96, 700, "f32", "f32"), route="logits")
@@ -107,6 +107,8 @@ def test_other_calls_by_logits(kind):
         check(*make(40, 128, 700, "bf16", "f16"), route="logits", reduce_cast=0)
     elif kind == "odd_hidden":
         check(*make(40, 100, 700), route="logits", reduce_cast=0)
+    elif kind == "cast":
+        check(*make(40, 128, 700), cast=torch.float16, route="logits", reduce_cast=2)
     elif kind == "hv":
         check(*make(40, 128, 704), route="logits", reduce_cast=0, weight_layout="hv")
     else:
@@ -158,6 +160,20 @@ def test_tokens_and_bad_values(act):
     w[10] = math.nan  # a row of the table: every row's sum
     got = nvjsel.lm_head_token_logprobs(x.cuda(), w.cuda(), t.cuda(), weight_layout="vh", reduce_cast=0)
     assert bool(torch.isnan(got.logprobs[(t >= 0) & (t < 900)]).all()) and got.logprobs[3] == 0
+
+
+def test_an_infinity_whose_logits_are_all_below():
+    """f32 hidden: an infinity's terms hold a NaN; its logits are -inf here, and nothing is left."""
+    g = torch.Generator().manual_seed(20)
+    x = torch.randn(5, 64, generator=g)
+    w = (torch.randn(301, 64, generator=g) * 0.02).to(torch.bfloat16)
+    w[:, 9] = -w[:, 9].abs() - 0.01
+    x[2, 9] = math.inf
+    r = nvjsel.lm_head_token_logprobs(x.cuda(), w.cuda(), torch.tensor([1, 2, 3, -1, 300]).cuda(), weight_layout="vh", entropy=True)
+    assert float(r.logprobs[2]) == -math.inf and float(r.entropy[2]) == 0.0
+    keep = [0, 1, 3, 4]
+    lp, _, tol, _ = oracle(x[keep], w, torch.tensor([1, 2, -1, 300]))
+    assert bool(((r.logprobs.double().cpu()[keep] - lp).abs() <= tol + SUM + lp.abs() * 2.0 ** -23).all())
 
 
 def test_far_logits():

@@ -38,7 +38,7 @@ P = 1 << 20  # an address that nothing reads: every call here is refused
     ({"xd": 4}, -1, "dtype"), ({"wd": 4}, -1, "dtype"), ({"layout": 2}, -1, "layout"), ({"rows": 0}, -1, "non-empty"),
     ({"h": 0}, -1, "non-empty"), ({"v": 0}, -1, "non-empty"), ({"rc": 3}, -1, "reduce_cast"), ({"tb": 2}, -1, "tokens"),
     ({"t": P + 2}, -1, "tokens"), ({"rows": (1 << 23) + 1}, -1, "at most"), ({"layout": 1}, -2, "takes"),
-    ({"wd": 0}, -2, "takes"), ({"xd": 2}, -2, "takes"), ({"h": 96}, -2, "takes"), ({"x": P + 2}, -2, "aligned"),
+    ({"rc": 2}, -2, "reduce_cast"), ({"wd": 0}, -2, "takes"), ({"xd": 2}, -2, "takes"), ({"h": 96}, -2, "takes"), ({"x": P + 2}, -2, "aligned"),
     ({"w": P + 8}, -2, "aligned"), ({"ws": None}, -3, "workspace"), ({"wsb": 64}, -3, "workspace"), ({"ws": P + 8}, -3, "workspace"),
 ])
 def test_c_refusals(change, code, what):
