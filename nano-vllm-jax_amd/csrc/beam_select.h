@@ -393,14 +393,15 @@ struct BeamJoinLds {
   int found;
 };
 
-// The row's sums from its parts, by one wave, and its answers.
-template <int DT, int LISTS, bool ONE, int LP>
-__device__ __forceinline__ void beam_token(const BeamArgs& a, const BeamJoinLds<LISTS>& lds, int row, int tid) {
-  if (tid >= 64) return;
+// A row's sums from its parts, by one wave.
+template <int LISTS, bool ONE, int LP>
+__device__ __forceinline__ RowSum beam_row_sum(const BeamArgs& a, const BeamJoinLds<LISTS>& lds, int row, float& m, int lane) {
   const int S = a.shares;
-  const float m = lds.rmax[0];
+  m = -INFINITY;
+  for (int i = lane; i < S; i += 64) m = fmaxf(m, lds.part[i].max);
+  m = wave_max_f32(m);
   RowSum r{0.0, 0.0};
-  for (int i = tid; i < S; i += 64) {
+  for (int i = lane; i < S; i += 64) {
     const BeamPart& p = lds.part[i];
     RowSum own{p.sum, 0.0};
     if constexpr (LP == LP_ENTROPY) {
@@ -411,7 +412,7 @@ __device__ __forceinline__ void beam_token(const BeamArgs& a, const BeamJoinLds<
   }
   r.sum = wave_sum_f64(r.sum);
   if constexpr (LP == LP_ENTROPY) r.ent = wave_sum_f64(r.ent);
-  if (tid == 0) row_answer_from<DT>(a.answers, a.logits, (int64_t)row * a.batch_stride, a.vocab, row, m, r);
+  return r;
 }
 
 template <int DT, int LISTS, int THREADS, bool ONE, int LP>
@@ -431,6 +432,15 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
   const int lane = tid & 63, wave = tid >> 6;
   const int W = a.beams, S = a.shares, k = a.k, lists = W * S;
 
+  bool asked = false;      // LP: whether the row asks for a token, and its logit
+  float own_logit = 0.0f;
+  if constexpr (LP != LP_NONE) {
+    if (tid == 0) {
+      const int64_t t = row_token(a.answers, req);
+      asked = t >= 0 && t < a.vocab;
+      if (asked) own_logit = load_as_f32(a.logits, DT, (size_t)((int64_t)req * a.batch_stride + t));
+    }
+  }
   if (tid < kBeamClasses) best_of[tid] = 0;
   if (tid == 0) {
     found = 0;
@@ -473,7 +483,16 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
   };
   auto part_sum = [&](const BeamPart& p, float m) { return p.sum * exp((double)p.max - (m == -INFINITY ? 0.0 : (double)m)); };
-  if (S <= kBeamFewShares) {  // a lane each
+  if constexpr (LP != LP_NONE) {  // one row: its answers too
+    if (wave == 0) {
+      float m;
+      const RowSum r = beam_row_sum<LISTS, ONE, LP>(a, lds, req, m, lane);
+      if (tid == 0) {
+        norm(0, m, r.sum);
+        row_answer(a.answers, req, asked, own_logit, m, r, rlog[0]);
+      }
+    }
+  } else if (S <= kBeamFewShares) {  // a lane each
     if (tid < W && state[tid] == BEAM_LIVE) {
       const BeamPart* p = part + tid * S;
       float m = -INFINITY;
@@ -496,7 +515,6 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     }
   }
   __syncthreads();
-  if constexpr (LP != LP_NONE) beam_token<DT, LISTS, ONE, LP>(a, lds, req, tid);
   auto score = [&](int w, float x) { return rscore[w] + (((double)x - (double)rmax[w]) - rlog[w]); };
 
   // the parts' best scores by class; an ended beam's score counts with them

@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, c
   if (lane != 0) return;
   const int64_t t = row_token(answers, row);
   const bool asked = t >= 0 && t < vocab;
-  row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r);
+  row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r, log(r.sum));
 }
 
 int launch_score_finish(const RowAnswers& answers, const ScoreArgs& sc, int rows, int vocab, hipStream_t s) {

@@ -227,9 +227,11 @@ __device__ __forceinline__ void row_join(RowSum& r, const RowSum& part, float ma
 // logprob = (x - m) - ln S for the token's logit x, entropy = ln S - T / S (r: S and T,
 // relative to m).  Nothing left: -inf and 0; NaN or +inf among the logits: NaN; a row that
 // asks for no token: 0.
-__device__ __forceinline__ void row_answer(const RowAnswers& a, int64_t row, bool asked, float x, float m, const RowSum& r) {
+// log_sum: ln S where it is a number.
+__device__ __forceinline__ void row_answer(const RowAnswers& a, int64_t row, bool asked, float x, float m, const RowSum& r,
+                                           double log_sum) {
   const bool nan = !(r.sum < INFINITY), none = !nan && r.sum == 0.0;
-  const double ls = nan ? (double)NAN : none ? 0.0 : log(r.sum);
+  const double ls = nan ? (double)NAN : none ? 0.0 : log_sum;
   a.logprobs[row] = !asked ? 0.0f : nan ? NAN : none ? -INFINITY : (float)(((double)x - (double)m) - ls);
   const double h = nan ? (double)NAN : none ? 0.0 : fmax(ls - r.ent / r.sum, 0.0);
   if (a.entropy) a.entropy[row] = (float)h;
@@ -249,7 +251,7 @@ __device__ __forceinline__ void row_answer_from(const RowAnswers& a, const void*
                                                 float m, const RowSum& r) {
   const int64_t t = row_token(a, row);
   const bool asked = t >= 0 && t < vocab;
-  row_answer(a, row, asked, asked ? load_as_f32(logits, DT, (size_t)(at + t)) : 0.0f, m, r);
+  row_answer(a, row, asked, asked ? load_as_f32(logits, DT, (size_t)(at + t)) : 0.0f, m, r, log(r.sum));
 }
 
 }  // namespace nvjsel

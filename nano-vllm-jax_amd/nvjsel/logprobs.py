@@ -73,19 +73,28 @@ class _Differentiable(torch.autograd.Function):
         return logprobs, ent, top, ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_logprobs, grad_entropy, *_):
+        if torch.is_grad_enabled():  # with create_graph: once is all there is
+            return _once(ctx, grad_logprobs, grad_entropy)
+        return _Differentiable.gradient(ctx, grad_logprobs, grad_entropy)
+
+    @staticmethod
+    def gradient(ctx, grad_logprobs, grad_entropy):
         if grad_logprobs is None and grad_entropy is None:
             return None, None, None, None
         logits, tokens, stats = ctx.saved_tensors
         rows, vocab = logits.shape
-        g, h = (None if t is None else t.to(torch.float32).contiguous() for t in (grad_logprobs, grad_entropy))
+        g = None if grad_logprobs is None else grad_logprobs.contiguous()  # f32, as their outputs
+        h = None if grad_entropy is None else grad_entropy.contiguous()
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
         with _on_device(logits.device):
             _lib.call("nvjsel_token_logprobs_grad", logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab,
                       _row_stride(logits), tokens.data_ptr(), tokens.element_size(), stats.data_ptr(),
                       _ptr(g), _ptr(h), out.data_ptr(), vocab, _stream_handle(logits.device))
         return out, None, None, None
+
+
+_once = torch.autograd.function.once_differentiable(_Differentiable.gradient)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int = 0,
