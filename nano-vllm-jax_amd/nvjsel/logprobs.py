@@ -114,7 +114,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
 
     Differentiable in ``logits`` through ``logprobs`` and ``entropy`` (once; the
     alternatives carry no gradient).  A row whose own two gradients are 0, or one
-    with nothing left, gets a gradient of zeros."""
+    with nothing left, gets a gradient of zeros.  In a captured graph take the gradient of a
+    leaf made within the capture (``logits.detach().requires_grad_()``, ``torch.autograd.grad``)."""
     if logits.ndim < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError("token_logprobs takes logits [..., V] and one token for every row")
     if logits.numel() == 0:

@@ -26,6 +26,7 @@ def _t(*shape, dtype=B16):
     ([_t(4, 8, dtype=torch.float32)], [_t(6, 4, dtype=torch.float32)], {}, "bfloat16 or float16"),
     ([_t(4, 8)], [_t(6, 4, dtype=torch.float16)], {}, "bfloat16 or float16"),
     ([_t(513, 8)], [_t(6, 513)], {}, "at most 512"),
+    ([_t(4, 8).requires_grad_()], [_t(6, 4)], {}, "not differentiable|device tensors"),
     ([_t(4, 8)], [_t(6, 4)], {}, "device tensors"),
 ])
 def test_pack_refusals(a, b, kw, what):
