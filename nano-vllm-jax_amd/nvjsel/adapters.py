@@ -156,7 +156,7 @@ def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, 
     a = adapters.a
     dev = _require_cuda(x, base, a, adapter_ids)
     if out is None:
-        result = flat = torch.empty(base.shape, dtype=base.dtype, device=dev)
+        result = flat = torch.empty_like(base, memory_format=torch.contiguous_format)
     else:
         if out.shape != base.shape or out.dtype != base.dtype or out.device != dev:
             raise ValueError("out must have base's shape, type and device")
@@ -168,7 +168,8 @@ def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, 
             raise ValueError("out's rows must be apart by one stride") from None
     if out is not None and ((flat.stride(1) != 1 and width > 1) or _stride(flat) < width):
         raise ValueError("out's rows must be contiguous and must not overlap")
-    x, base, ids = _rows(x, rows), _rows(base, rows), adapter_ids.reshape(rows).contiguous()
+    x, base = _rows(x, rows), _rows(base, rows)
+    ids = adapter_ids if adapter_ids.ndim == 1 and adapter_ids.is_contiguous() else adapter_ids.reshape(rows).contiguous()
     if out is not None and (base.data_ptr(), _stride(base)) != (flat.data_ptr(), _stride(flat)) and _meet(base, flat):
         raise ValueError("out must be base itself or share no memory with it")
     if hidden < _MIN_HIDDEN:  # zeros beside the table's zeros

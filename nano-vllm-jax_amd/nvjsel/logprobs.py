@@ -44,13 +44,13 @@ def _forward(logits, tokens, num_top: int, entropy: bool, stats: bool):
     """Of ``logits [N, V]`` with unit token stride; and the rows' statistics for the gradient."""
     rows, vocab = logits.shape
     dev = logits.device
-    logprobs = torch.empty((rows,), dtype=torch.float32, device=dev)
+    logprobs = torch.empty_like(tokens, dtype=torch.float32)
     ent = torch.empty_like(logprobs) if entropy else None
-    kept = torch.empty((rows, 3), dtype=torch.float32, device=dev) if stats else None
+    kept = logprobs.new_empty((rows, 3)) if stats else None
     top = ids = None
     if num_top:
-        top = torch.empty((rows, num_top), dtype=torch.float32, device=dev)
-        ids = torch.empty((rows, num_top), dtype=torch.int32, device=dev)
+        top = logprobs.new_empty((rows, num_top))
+        ids = torch.empty_like(top, dtype=torch.int32)
     dt = _dtype_code(logits, "logits")
     with _on_device(dev):
         nbytes = _bytes(dev.index, dt, rows, vocab, num_top)
@@ -86,7 +86,7 @@ class _Differentiable(torch.autograd.Function):
         rows, vocab = logits.shape
         g = None if grad_logprobs is None else grad_logprobs.contiguous()  # f32, as their outputs
         h = None if grad_entropy is None else grad_entropy.contiguous()
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
         with _on_device(logits.device):
             _lib.call("nvjsel_token_logprobs_grad", logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab,
                       _row_stride(logits), tokens.data_ptr(), tokens.element_size(), stats.data_ptr(),
@@ -136,7 +136,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
         logits = logits.reshape(rows, vocab)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    tokens = tokens.reshape(rows).contiguous()
+    if tokens.ndim != 1 or not tokens.is_contiguous():
+        tokens = tokens.reshape(rows).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         lp, ent, top, ids = _Differentiable.apply(logits, tokens, num_top, bool(entropy))
     else:
@@ -210,7 +211,7 @@ def _scored(x, output_weight, tokens, entropy, weight_layout, reduce_cast):
     rc = own if reduce_cast is None else int(reduce_cast)
     if rc not in (0, own):
         return None
-    logprobs = torch.empty((x.shape[0],), dtype=torch.float32, device=dev)
+    logprobs = torch.empty_like(tokens, dtype=torch.float32)
     ent = torch.empty_like(logprobs) if entropy else None
     stream = _stream_handle(dev)
     ws = _workspace(dev, stream, "score", nbytes, 0)
