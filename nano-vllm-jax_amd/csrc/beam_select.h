@@ -388,30 +388,22 @@ struct BeamJoinLds {
   float rmax[kBeamMax];
   uint32_t best_of[kBeamClasses];  // of the parts' classes: the scores' first 32 bits in order
   uint2 early[LISTS == kBeamFew ? kBeamEarly : 1];  // every part's first candidates
+  double ent[LISTS == kBeamFew ? LISTS : 1];        // of the parts (LP_ENTROPY)
   int start[LISTS];                // of the parts that reach the bound: the number of their first candidate
   uint16_t list[LISTS];
   int found;
 };
 
 // A row's sums from its parts, by one wave.
-template <int LISTS, bool ONE, int LP>
-__device__ __forceinline__ RowSum beam_row_sum(const BeamArgs& a, const BeamJoinLds<LISTS>& lds, int row, float& m, int lane) {
-  const int S = a.shares;
+template <int LISTS, bool ENT>
+__device__ __forceinline__ RowSum beam_row_sum(const BeamJoinLds<LISTS>& lds, int parts, float& m, int lane) {
   m = -INFINITY;
-  for (int i = lane; i < S; i += 64) m = fmaxf(m, lds.part[i].max);
+  for (int i = lane; i < parts; i += 64) m = fmaxf(m, lds.part[i].max);
   m = wave_max_f32(m);
   RowSum r{0.0, 0.0};
-  for (int i = lane; i < S; i += 64) {
-    const BeamPart& p = lds.part[i];
-    RowSum own{p.sum, 0.0};
-    if constexpr (LP == LP_ENTROPY) {
-      const uint2 u = row_get<ONE>(a.ents + (size_t)row * S + i);
-      own.ent = two_words(u.x, u.y);
-    }
-    row_join(r, own, p.max, m);
-  }
+  for (int i = lane; i < parts; i += 64) row_join(r, RowSum{lds.part[i].sum, ENT ? lds.ent[i] : 0.0}, lds.part[i].max, m);
   r.sum = wave_sum_f64(r.sum);
-  if constexpr (LP == LP_ENTROPY) r.ent = wave_sum_f64(r.ent);
+  if constexpr (ENT) r.ent = wave_sum_f64(r.ent);
   return r;
 }
 
@@ -432,25 +424,23 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
   const int lane = tid & 63, wave = tid >> 6;
   const int W = a.beams, S = a.shares, k = a.k, lists = W * S;
 
-  bool asked = false;      // LP: whether the row asks for a token, and its logit
-  float own_logit = 0.0f;
-  if constexpr (LP != LP_NONE) {
-    if (tid == 0) {
-      const int64_t t = row_token(a.answers, req);
-      asked = t >= 0 && t < a.vocab;
-      if (asked) own_logit = load_as_f32(a.logits, DT, (size_t)((int64_t)req * a.batch_stride + t));
-    }
-  }
+  // LP: the last wave answers for the row, its token and the token's logit on their way beside the parts
+  const bool answers = LP != LP_NONE && wave == THREADS / 64 - 1;
+  int64_t token = -1;
+  float own_logit = 0.0f, own_max = 0.0f;
+  RowSum own_sum{0.0, 0.0};
+  if (answers) token = row_token(a.answers, req);
   if (tid < kBeamClasses) best_of[tid] = 0;
   if (tid == 0) {
     found = 0;
     taken = 0;
   }
-  // One launch: the parts' first candidates on their way with the parts, whatever of them
+  // The parts' first candidates on their way with the parts, whatever of them
   // are there, so that the ones that reach the bound need no round trip of their own
+  constexpr bool EARLY = ONE || LP != LP_NONE;
   int firsts = 0;
-  uint2 e[ONE ? kBeamEarly / THREADS : 1];
-  if constexpr (ONE) {
+  uint2 e[EARLY ? kBeamEarly / THREADS : 1];
+  if constexpr (EARLY) {
     firsts = min(kBeamEarly / lists, a.cap);
 #pragma unroll
     for (int u = 0; u < kBeamEarly / THREADS; ++u) {
@@ -464,8 +454,13 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     part[l].sum = two_words(u.x, u.y);
     part[l].max = __uint_as_float(v.x);
     part[l].count = (int)min(v.y, (uint32_t)a.cap);  // whatever is there, no candidate is read outside the workspace
+    if constexpr (LP == LP_ENTROPY) {
+      const uint2 t = row_get<ONE>(a.ents + (size_t)req * lists + l);
+      lds.ent[l] = two_words(t.x, t.y);
+    }
   }
-  if constexpr (ONE) {
+  if (token >= 0 && token < a.vocab) own_logit = load_as_f32(a.logits, DT, (size_t)((int64_t)req * a.batch_stride + token));
+  if constexpr (EARLY) {
 #pragma unroll
     for (int u = 0; u < kBeamEarly / THREADS; ++u)
       if (tid + u * THREADS < lists * firsts) lds.early[tid + u * THREADS] = e[u];
@@ -483,14 +478,13 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
   };
   auto part_sum = [&](const BeamPart& p, float m) { return p.sum * exp((double)p.max - (m == -INFINITY ? 0.0 : (double)m)); };
-  if constexpr (LP != LP_NONE) {  // one row: its answers too
+  if constexpr (LP != LP_NONE) {  // one row
     if (wave == 0) {
       float m;
-      const RowSum r = beam_row_sum<LISTS, ONE, LP>(a, lds, req, m, lane);
-      if (tid == 0) {
-        norm(0, m, r.sum);
-        row_answer(a.answers, req, asked, own_logit, m, r, rlog[0]);
-      }
+      const RowSum r = beam_row_sum<LISTS, false>(lds, S, m, lane);
+      if (tid == 0) norm(0, m, r.sum);
+    } else if (answers) {
+      own_sum = beam_row_sum<LISTS, LP == LP_ENTROPY>(lds, S, own_max, lane);
     }
   } else if (S <= kBeamFewShares) {  // a lane each
     if (tid < W && state[tid] == BEAM_LIVE) {
@@ -515,6 +509,7 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     }
   }
   __syncthreads();
+  if (answers && lane == 0) row_answer(a.answers, req, token >= 0 && token < a.vocab, own_logit, own_max, own_sum, rlog[0]);
   auto score = [&](int w, float x) { return rscore[w] + (((double)x - (double)rmax[w]) - rlog[w]); };
 
   // the parts' best scores by class; an ended beam's score counts with them
@@ -567,7 +562,7 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
         }
         of[u] = list[lo];
         const int j = i - start[lo];
-        if (N == 1 && ONE && j < firsts) c[u] = lds.early[of[u] * firsts + j];
+        if (N == 1 && EARLY && j < firsts) c[u] = lds.early[of[u] * firsts + j];
         else c[u] = row_get<ONE>(a.cand + ((size_t)req * lists + of[u]) * a.cap + j);
       }
 #pragma unroll

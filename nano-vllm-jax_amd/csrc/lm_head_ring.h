@@ -558,8 +558,8 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
   }
   // Adds a tile's logits: differences from the new maximum, so that no size of logits is far
   // off; -inf (a row past the end starts there) is 0 in both sums.  The products' registers are
-  // read, never written, by one path: copies of them spill (2048 rows 950 us; with the rounding and
-  // the rows past the end as paths of their own 1032, writing them 1209).
+  // read, never written, by one path: copies of them spill (2048 rows 950 us before a stage's reads
+  // went among its products; with the rounding and the rows past the end as paths of their own 1032, writing them 1209).
   auto score_tile = [&](int v0) NVJSEL_INLINE {
     auto logit = [&](int tv, int tb, int e) NVJSEL_INLINE { return apply_cast(acc[tv][tb][e], S::CAST ? (WT == DT_BF16 ? 1 : 2) : 0); };
 #pragma unroll

@@ -33,7 +33,7 @@ struct RowArgs {
 };
 
 // Bound: the stream and, beside it, an exponential a logit: 1000 rows of 151,936 bf16 logits (304
-// MB) 52 us, 5.8 TB/s, with entropies; 7.0 is this card's streaming read.  8 to 28 waves per CU, two to four
+// MB) 50 us, 6.1 TB/s, with entropies; 7.0 is this card's streaming read.  8 to 28 waves per CU, two to four
 // chunks in registers and chunks half as long took as much (31-33 us at 512 rows), 40 and 64 waves more (36-37).
 // A block's four waves take consecutive shares of one row, the next chunk on its way in
 // registers, lanes with a maximum and sums of their own; the waves' sums meet in LDS, and
@@ -157,7 +157,7 @@ static constexpr int kGradPieces = 4;  // 16-byte pieces of a thread
 // Elementwise: one exponential per logit, read once and written once.  p ln p is 0 where p
 // is: ln p is held above -1e30 in that product; the hardware's exp2 gives 0 below 2^-126.  A row
 // without a gradient (padding) is not read: zeros.  Bound: the reads and writes: 512 rows of 151,936 bf16
-// logits (311 MB) 54 us, 5.8 TB/s, a large copy's 5.0; 2 pieces a thread 56.
+// logits (311 MB) 54-57 us, 5.5-5.8 TB/s, a large copy's 5.0; 2 pieces a thread 56.
 template <int DT, bool ENT>
 __global__ void __launch_bounds__(256) logprobs_grad_kernel(GradArgs a) {
   using E = RowElems<DT>;
