@@ -230,3 +230,23 @@ def test_a_servers_step(kind):
     assert bool(((r.logprobs.double().cpu() - lp).abs() <= 2.0 ** -19 + lp.abs() * 2.0 ** -24).all())
     scored = nvjsel.lm_head_token_logprobs(x, head, tokens, num_top=4, entropy=True, adapters=table, adapter_ids=ids)
     assert all(torch.equal(p, q) for p, q in zip(r, scored))
+
+
+@pytest.mark.parametrize("rank", [16, 64, 512])
+def test_most_rows(rank):
+    """2^20 rows; 1000 of them have an adapter, the first and last ones too."""
+    rows, hidden, width = 1 << 20, 8, 3
+    g = torch.Generator().manual_seed(rank)
+    x = torch.randn(rows, hidden, generator=g).to(torch.bfloat16)
+    base = torch.randn(rows, width, generator=g).to(torch.bfloat16)
+    a = [(torch.randn(rank, hidden, generator=g) / math.sqrt(hidden)).to(torch.bfloat16) for _ in range(2)]
+    b = [(torch.randn(width, rank, generator=g) / math.sqrt(rank)).to(torch.bfloat16) for _ in range(2)]
+    some = torch.randperm(rows, generator=g)[:998].tolist() + [0, rows - 1]
+    ids = torch.full((rows,), -1, dtype=torch.int32)
+    ids[some] = torch.randint(0, 2, (1000,), generator=g).to(torch.int32)
+    s = torch.tensor([0.5, 1.5])
+    table = nvjsel.pack_adapters([t.cuda() for t in a], [t.cuda() for t in b], s)
+    got = nvjsel.apply_adapters(x.cuda(), base.cuda(), table, ids.cuda()).cpu()
+    assert torch.equal(got[ids < 0], base[ids < 0])
+    want, tol = oracle(x[some], base[some], a, b, s, ids[some])
+    assert bool(((got[some].double() - want).abs() <= tol).all())

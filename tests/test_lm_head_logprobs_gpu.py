@@ -222,3 +222,8 @@ def test_captured_and_again():
         eager = call()
         torch.cuda.synchronize()
         assert torch.equal(out.logprobs, eager.logprobs) and torch.equal(out.entropy, eager.entropy)
+
+
+def test_hundreds_of_row_blocks():
+    check(*make((1 << 17) + 3, 64, 130, seed=7), reduce_cast=0)
+    check(*make((1 << 15) + 33, 64, 130, "f32", "bf16", seed=8), reduce_cast=0, entropy=False)

@@ -426,3 +426,27 @@ def test_captured_training_pass():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_most_rows():
+    """2^23 rows, the most of a call: results, alternatives and gradient."""
+    rows, vocab = 1 << 23, 3
+    g = torch.Generator().manual_seed(23)
+    x = torch.randn(rows, vocab, generator=g)
+    t = torch.randint(-1, vocab, (rows,), generator=g)
+    asked = t >= 0
+    lp = torch.log_softmax(x.double(), 1)
+    want = torch.where(asked, lp.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+    leaf = x.cuda().requires_grad_()
+    r = nvjsel.token_logprobs(leaf, t.cuda())
+    plain = nvjsel.token_logprobs(leaf.detach(), t.cuda(), num_top=1)
+    for got in (r.logprobs.detach(), plain.logprobs):
+        assert bool(((got.cpu().double() - want).abs() <= SUM + want.abs() * 2.0 ** -23).all())
+    best = lp.max(1)  # torch.randn's values differ within a row
+    assert torch.equal(plain.top_ids.cpu().long()[:, 0], best.indices)
+    assert bool(((plain.top_logprobs[:, 0].cpu().double() - best.values).abs() <= SUM + best.values.abs() * 2.0 ** -23).all())
+    d, = torch.autograd.grad(r.logprobs, leaf, torch.ones(rows, device="cuda"))
+    p = lp.exp()
+    exact = torch.where(asked[:, None], torch.zeros_like(lp).scatter_(1, t.clamp(min=0)[:, None], 1.0) - p, 0.0)
+    tol = p * (SUM + 2.0 ** -22 * (2.0 + lp.abs() + (x.amax(1, keepdim=True) - x.double().logsumexp(1, keepdim=True)).abs()))
+    assert bool(((d.cpu().double() - exact).abs() <= tol + 2.0 ** -23).all())
