@@ -37,7 +37,7 @@ __device__ __forceinline__ u32x4_t shift_down8(u32x4_t w, int s) {
 // (REDUCE_CAST-rounded) logits themselves, written to out_logits; SCORE: log
 // probabilities of given tokens (and entropies), lm_head_score.hip.
 enum { MODE_GREEDY = 0, MODE_SAMPLE = 1, MODE_LOGITS = 2, MODE_SCORE = 8 };
-enum { SCORE_ENTROPY = 1, SCORE_CAST = 2 };  // added to MODE_SCORE
+enum { SCORE_ENTROPY = 1, SCORE_CAST = 2, SCORE_TERMS = 4 };  // added to MODE_SCORE
 
 struct LmArgs {
   const void* W;

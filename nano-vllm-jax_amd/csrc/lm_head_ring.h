@@ -66,6 +66,9 @@ struct RingShape {
   static constexpr bool SMP = MODE == MODE_SAMPLE;
   // scoring: with the entropy, of logits rounded to the weight's type
   static constexpr bool SCORE = MODE >= MODE_SCORE, ENT = SCORE && (MODE & SCORE_ENTROPY), CAST = SCORE && (MODE & SCORE_CAST);
+  // f32 hidden: split as it is staged, or given in its terms (scoring)
+  static constexpr bool TERMS = SCORE && (MODE & SCORE_TERMS), RAW = NS == 3 && !TERMS;
+  static_assert(!TERMS || (NS == 3 && NBR == 64), "whole loads of all waves");
   static constexpr int NW = 8;                        // waves; one block per CU
   static constexpr int BV = 256;                      // vocabulary rows of a block tile
   static constexpr int TB = NBR <= 32 || NS == 3 ? 1 : 2;  // 32-row batch tiles per wave
@@ -75,7 +78,7 @@ struct RingShape {
   // ring slots: W stages come from HBM, hidden stages from L2
   static constexpr int RW = NS == 3 ? (SMP && NBR == 64 ? 2 : 3) : SMP ? (NBR <= 64 ? 3 : 2) : NBR <= 32 ? 4 : 3;
   static constexpr int RX = NS == 3 || SMP ? 2 : NBR <= 32 ? 4 : NBR <= 128 ? 3 : 2;
-  static constexpr int LDS_RAW = NS == 3 ? NBR * kRingKC * 4 : 0;  // one stage of f32 values
+  static constexpr int LDS_RAW = RAW ? NBR * kRingKC * 4 : 0;  // one stage of f32 values
   static constexpr int LDS_RING = (RW * BV + RX * NS * NBR) * kRingKC * 2 + LDS_RAW;
   // sample mode: rows scored at a time, queue entries per wave (12 B each), and
   // per batch row the block's largest approximate score and best exact key
@@ -147,6 +150,7 @@ struct ScoreArgs {
   int shares;           // of the vocabulary
   float* token_logits;  // [B]
   RowPart* parts;       // [B][shares]
+  uint16_t* terms;      // [B][3][H]: the hidden's (SCORE_TERMS)
 };
 // Block -> (share, row block): the blocks of a share, which read the same rows of W, next to each
 // other on one XCD (blocks go to the eight in turn).
@@ -167,8 +171,8 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
   constexpr int XLANES = XBYTES >= NW * 1024 ? 64 : XBYTES / (NW * 16);  // lanes of each
   // loads a wave may leave in flight when stage s starts: those issued after
   // X(s) and W(s) (each stage issues X(s + RX - 1), then W(s + RW - 1))
-  // (NS = 3: X(s) is split already; W(s + 1) is in flight where RW = 3)
-  constexpr int LIVE = NS == 3 ? (RW - 2) * WL : (RX - 2) * (WL + XL) + (RW > RX ? WL : 0);
+  // (RAW: X(s) is split already; W(s + 1) is in flight where RW = 3)
+  constexpr int LIVE = S::RAW ? (RW - 2) * WL : (RX - 2) * (WL + XL) + (RW > RX ? WL : 0);
   static_assert(RW >= RX && RX >= 2, "W runs at least as far ahead as the hidden");
   constexpr int XRING = RW * WBYTES;  // LDS offset of the hidden's slots
   __shared__ __attribute__((aligned(1024))) char ring[S::LDS_RING + S::LDS_QUEUE];
@@ -182,7 +186,8 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     const int place = score_place(share, (int)gridDim.x);
     share = place / sc.row_blocks;
     b0 = place % sc.row_blocks * NBR;
-    hidden += (size_t)b0 * rowb * (NS == 3 ? 2 : 1);
+    if constexpr (S::TERMS) hidden = (const char*)sc.terms + (size_t)b0 * rowb * 3;
+    else hidden += (size_t)b0 * rowb * (NS == 3 ? 2 : 1);
   }
   const int B = S::SCORE ? min(NBR, a.B - b0) : a.B;
   const int nkc = a.H / kRingKC;
@@ -212,7 +217,8 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     const int p = (i * NW + wave) * XLANES + lane;  // (XL > 1: XLANES = 64)
     const int row = p >> 3;
     const int q = (p & 7) ^ ((row >> 1) & 7);
-    xoff[i] = (uint32_t)min(row, B - 1) * rowb + (uint32_t)(q * 16);
+    xoff[i] = S::TERMS ? (uint32_t)(min(row % NBR, B - 1) * 3 + row / NBR) * rowb + (uint32_t)(q * 16)
+                       : (uint32_t)min(row, B - 1) * rowb + (uint32_t)(q * 16);
   }
   auto issue_x = [&]() NVJSEL_INLINE {
     const uint32_t dst = ring0 + (uint32_t)(XRING + lx * XBYTES);
@@ -224,18 +230,18 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     lx = lx + 1 == RX ? 0 : lx + 1;
     xko = xko + kRingKC * 2 == rowb ? 0u : xko + kRingKC * 2;
   };
-  // NS = 3: the next hidden stage arrives as f32 in `raw`, each thread's 16-byte
+  // RAW: the next hidden stage arrives as f32 in `raw`, each thread's 16-byte
   // pieces (four values) where it reads them back itself, and is split into
   // the other slot in the middle of a stage
   constexpr int RL = S::LDS_RAW / (NW * 1024);  // raw loads per wave and stage
-  constexpr int RAW = XRING + RX * XBYTES;
+  constexpr int RAW0 = XRING + RX * XBYTES;
   auto issue_raw = [&]() NVJSEL_INLINE {
     const char* src = hidden + 2 * xko;
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
       const int p = (i * NW + wave) * 64 + lane;  // row p >> 4, values 4 (p & 15) .. + 3
       dma16(src, (uint32_t)min(p >> 4, B - 1) * (2 * rowb) + (uint32_t)(p & 15) * 16u,
-            ring0 + (uint32_t)(RAW + (i * NW + wave) * 1024));
+            ring0 + (uint32_t)(RAW0 + (i * NW + wave) * 1024));
     }
     xko = xko + kRingKC * 2 == rowb ? 0u : xko + kRingKC * 2;
   };
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
       const int p = (i * NW + wave) * 64 + lane, row = p >> 4, q = (p & 15) >> 1;
-      const u32x4_t r = *(const u32x4_t*)(ring + RAW + p * 16);
+      const u32x4_t r = *(const u32x4_t*)(ring + RAW0 + p * 16);
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[j]);
@@ -328,11 +334,11 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
   // one stage; `rest`: the previous stage of the tile left its last step's products
   auto stage = [&](auto rest) NVJSEL_INLINE {
     stage_barrier<LIVE>();
-    if constexpr (NS == 3)
+    if constexpr (S::RAW)
       issue_raw();
     else
       issue_x();
-    constexpr bool PARTS = S::SCORE && NS == 1;  // W's requests in two parts, among the products
+    constexpr bool PARTS = S::SCORE && !S::RAW;  // W's requests in two parts, among the products
     using Half = std::integral_constant<int, WL / 2>;
     if constexpr (!PARTS) issue_w();
     read_step(I0{}, I0{});
@@ -341,7 +347,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     if constexpr (PARTS) issue_w_part(I0{}, Half{});
     read_step(I1{}, I1{});
     multiply(I0{});
-    if constexpr (NS == 3) {
+    if constexpr (S::RAW) {
       wave_wait<WL>();  // the W stage requested behind the raw values stays in flight
       split_raw();
     }
@@ -727,7 +733,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
     load_tile_start();
     // as the loop would have left them: X(0) .. X(RX - 2), each W stage RW - RX
     // ahead of the hidden stage issued with it
-    if constexpr (NS == 3) {
+    if constexpr (S::RAW) {
       issue_raw();
       wave_wait<0>();
       split_raw();

@@ -12,6 +12,7 @@ int launch_score_f16(const LmArgs& a, const ScoreArgs& sc, const RowAnswers& w, 
                      hipStream_t s);
 int launch_score_f32(const LmArgs& a, const ScoreArgs& sc, const RowAnswers& w, int block_rows, bool entropy, bool cast,
                      hipStream_t s);
+int launch_score_split(const LmArgs& a, const ScoreArgs& sc, hipStream_t s);
 int launch_score_finish(const RowAnswers& answers, const ScoreArgs& sc, int rows, int vocab, hipStream_t s);
 
 template <int WT, int MODE, int NBR, int NS>
@@ -27,7 +28,12 @@ static int launch_score_rows(const LmArgs& a, ScoreArgs sc, const RowAnswers& an
 template <int WT, int NS, int MODE>
 static int launch_score_mode(const LmArgs& a, const ScoreArgs& sc, const RowAnswers& w, int block_rows, hipStream_t s) {
   if (block_rows == 32) return launch_score_rows<WT, MODE, 32, NS>(a, sc, w, s);
-  if constexpr (NS == 1) {
+  if constexpr (NS == 3) {
+    if (sc.terms && block_rows == 64) {
+      const int rc = launch_score_split(a, sc, s);
+      return rc != NVJSEL_OK ? rc : launch_score_rows<WT, MODE + SCORE_TERMS, 64, NS>(a, sc, w, s);
+    }
+  } else {
     if (block_rows == 128) return launch_score_rows<WT, MODE, 128, NS>(a, sc, w, s);
     if (block_rows == 256) return launch_score_rows<WT, MODE, 256, NS>(a, sc, w, s);
   }

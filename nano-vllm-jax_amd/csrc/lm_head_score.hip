@@ -12,7 +12,7 @@
 // entropies: 876-928 us by card, 1.12-1.19 PFLOP/s (a library's bare product of these sizes, which writes
 // 1 GB of logits, 919); the tiles' products without their sums 881: matrix pipes 77% busy at some 1.5 GHz of
 // 2.4.  24 rows 79 us, the stream of W (508 MB) at 6.4 TB/s.  300 f32 rows x 768 (three products each)
-// of 50,257 tokens 81-95 us, 0.73-0.86 PFLOP/s: four tiles a block, bound by the terms' reads from LDS.
+// of 50,257 tokens 77 us, 0.90 PFLOP/s: four tiles a block, three launches; 2048 x 1024, 248,320 tokens 2.62 ms, 1.19 PFLOP/s.
 #include "lm_head_score.h"
 
 namespace nvjsel {
@@ -33,6 +33,38 @@ __global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, c
   const int64_t t = row_token(answers, row);
   const bool asked = t >= 0 && t < vocab;
   row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r, log(r.sum));
+}
+
+// f32 hidden rows as their three bf16 terms, [row][term][H], eight values a thread: once for a launch, where
+// the GEMM's blocks would each split them again for every tile (calls of 300 rows x 768 and 50,257 tokens 85 -> 77
+// us, 64 x 1024 and 248,320 124 -> 108, 40 x 768 and 8000 26 -> 24, 2048 x 1024 and 248,320 3455 -> 2622).
+__global__ void __launch_bounds__(256) score_split_kernel(const float* hidden, uint16_t* terms, int H, int64_t pieces) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= pieces) return;
+  const int each = H / 8;
+  const int64_t row = i / each;
+  const int k = (int)(i - row * each) * 8;
+  const u32x4_t* x = (const u32x4_t*)(hidden + i * 8);
+  float v[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const u32x4_t r = x[h];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[h][j] = __uint_as_float(r[j]);
+  }
+#pragma unroll
+  for (int t = 0; t < 3; ++t) {
+    const uint2 lo = next_term(v[0]), hi = next_term(v[1]);
+    *(u32x4_t*)(terms + (row * 3 + t) * H + k) = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+  }
+}
+
+int launch_score_split(const LmArgs& a, const ScoreArgs& sc, hipStream_t s) {
+  const int64_t pieces = (int64_t)a.B * (a.H / 8);
+  hipLaunchKernelGGL(score_split_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, (const float*)a.hidden,
+                     sc.terms, a.H, pieces);
+  NVJSEL_CHECK_LAUNCH("score_split_kernel");
+  return NVJSEL_OK;
 }
 
 int launch_score_finish(const RowAnswers& answers, const ScoreArgs& sc, int rows, int vocab, hipStream_t s) {
@@ -75,8 +107,15 @@ static int score_row_blocks(int64_t left, int vocab, int cus) {
   return first[left];
 }
 
-static size_t score_bytes(int64_t rows, int cus) {  // parts: at most `cus` shares x row blocks of 256 rows
+// Hidden values whose terms are kept, for calls of more than 32 f32 rows.
+static constexpr int kScoreTermsHidden = 16384;
+static bool score_terms(bool f32, int64_t rows, int H) { return f32 && rows > 32 && H <= kScoreTermsHidden; }
+static size_t score_parts_bytes(int64_t rows, int cus) {  // parts: at most `cus` shares x row blocks of 256 rows
   return align_up((size_t)rows * 4, 16) + (size_t)cus * 256 * sizeof(RowPart);
+}
+static size_t score_bytes(bool f32, int64_t rows, int H, int cus) {
+  const int64_t most = rows < kScoreBlocks * 64 ? rows : kScoreBlocks * 64;  // of a launch
+  return score_parts_bytes(rows, cus) + (score_terms(f32, rows, H) ? (size_t)most * 3 * H * 2 : 0);
 }
 
 }  // namespace nvjsel
@@ -110,7 +149,7 @@ extern "C" size_t nvjsel_lm_head_token_logprobs_workspace_size(int hidden_dtype,
                                                                int64_t rows, int hidden_dim, int vocab) {
   clear_error();
   if (score_check(hidden_dtype, weight_dtype, weight_layout, rows, hidden_dim, vocab) != NVJSEL_OK) return 0;
-  return score_bytes(rows, device_cu_count());
+  return score_bytes(hidden_dtype == NVJSEL_F32, rows, hidden_dim, device_cu_count());
 }
 
 extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtype, const void* weight, int weight_dtype,
@@ -129,7 +168,8 @@ extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtyp
   if ((((uintptr_t)hidden) | ((uintptr_t)weight)) & 15)
     return fail(NVJSEL_EUNSUPPORTED, "lm_head_token_logprobs: hidden and weight must be 16-byte aligned");
   const int cus = device_cu_count();
-  const size_t need = score_bytes(rows, cus);
+  const bool f32 = hidden_dtype == NVJSEL_F32;
+  const size_t need = score_bytes(f32, rows, hidden_dim, cus);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
     set_error("lm_head_token_logprobs: workspace %zu bytes (16-byte aligned) < required %zu", workspace_bytes, need);
     return NVJSEL_EWORKSPACE;
@@ -139,7 +179,7 @@ extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtyp
   int64_t n = 0;
   for (int64_t r0 = 0; r0 < rows; r0 += n) {
     const int64_t left = rows - r0;
-    const int block_rows = score_block_rows(hidden_dtype == NVJSEL_F32, left);
+    const int block_rows = score_block_rows(f32, left);
     ScoreArgs sc{};
     // a last block that a smaller shape takes is left to the next launch
     const int64_t blocks = block_rows == 256 ? (left + 127) / 256 : (left + block_rows - 1) / block_rows;
@@ -149,6 +189,7 @@ extern "C" int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtyp
     sc.token64 = token_bytes == 8;
     sc.token_logits = (float*)workspace + r0;
     sc.parts = (RowPart*)((char*)workspace + align_up((size_t)rows * 4, 16));
+    sc.terms = score_terms(f32, rows, hidden_dim) ? (uint16_t*)((char*)workspace + score_parts_bytes(rows, cus)) : nullptr;
     LmArgs a{};
     a.W = weight;
     a.hidden = (const char*)hidden + (size_t)r0 * hidden_dim * dtype_size(hidden_dtype);
