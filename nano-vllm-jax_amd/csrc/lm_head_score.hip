@@ -21,18 +21,29 @@ __global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, c
                                                            int rows, int shares, int vocab) {
   const int row = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   if (row >= rows) return;
+  // all on their way together: the parts, the token and its logit (whatever lies there where none is asked)
+  const int64_t t = row_token(answers, row);
+  const float x = token_logits[row];
   const RowPart* p = parts + (size_t)row * shares;
+  constexpr int KEPT = 4;
+  RowPart q[KEPT];
+#pragma unroll
+  for (int u = 0; u < KEPT; ++u) q[u] = p[min(lane + 64 * u, shares - 1)];
   float m = -INFINITY;
-  for (int i = lane; i < shares; i += 64) m = fmaxf(m, p[i].max);
+#pragma unroll
+  for (int u = 0; u < KEPT; ++u) m = fmaxf(m, q[u].max);
+  for (int i = lane + 64 * KEPT; i < shares; i += 64) m = fmaxf(m, p[i].max);
   m = wave_max_f32(m);
   RowSum r{0.0, 0.0};
-  for (int i = lane; i < shares; i += 64) row_join(r, RowSum{p[i].sum, p[i].ent}, p[i].max, m);
+#pragma unroll
+  for (int u = 0; u < KEPT; ++u)
+    if (lane + 64 * u < shares) row_join(r, RowSum{q[u].sum, q[u].ent}, q[u].max, m);
+  for (int i = lane + 64 * KEPT; i < shares; i += 64) row_join(r, RowSum{p[i].sum, p[i].ent}, p[i].max, m);
   r.sum = wave_sum_f64(r.sum);
   r.ent = wave_sum_f64(r.ent);
   if (lane != 0) return;
-  const int64_t t = row_token(answers, row);
   const bool asked = t >= 0 && t < vocab;
-  row_answer(answers, row, asked, asked ? token_logits[row] : 0.0f, m, r, log(r.sum));
+  row_answer(answers, row, asked, asked ? x : 0.0f, m, r, log(r.sum));
 }
 
 // f32 hidden rows as their three bf16 terms, [row][term][H], eight values a thread: once for a launch, where
