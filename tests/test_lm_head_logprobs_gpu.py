@@ -227,3 +227,36 @@ def test_captured_and_again():
 def test_hundreds_of_row_blocks():
     check(*make((1 << 17) + 3, 64, 130, seed=7), reduce_cast=0)
     check(*make((1 << 15) + 33, 64, 130, "f32", "bf16", seed=8), reduce_cast=0, entropy=False)
+
+
+@pytest.mark.parametrize("rows,hidden", [(33, 64), (64, 16384), (65, 16384), (40, 16448), (100, 16448)])
+def test_f32_rows_as_terms_and_as_they_lie(rows, hidden):
+    """More than 32 f32 rows are split beforehand up to 16,384 hidden values, as they are staged beyond."""
+    check(*make(rows, hidden, 300, "f32", "bf16", seed=21), reduce_cast=0)
+
+
+def test_f32_terms_of_an_infinity_and_captured():
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn(150, 64, generator=g)
+    w = (torch.randn(301, 64, generator=g) * 0.02).to(torch.bfloat16)
+    w[:, 9] = -w[:, 9].abs() - 0.01
+    x[[2, 70, 149], 9] = math.inf
+    t = torch.randint(0, 301, (150,), generator=g)
+    xd, wd, td = x.cuda(), w.cuda(), t.cuda()
+    call = lambda: nvjsel.lm_head_token_logprobs(xd, wd, td, weight_layout="vh", entropy=True)  # noqa: E731
+    r = call()
+    bad = torch.zeros(150, dtype=torch.bool)
+    bad[[2, 70, 149]] = True
+    assert bool((r.logprobs.cpu()[bad] == -math.inf).all()) and bool((r.entropy.cpu()[bad] == 0.0).all())
+    lp, _, tol, _ = oracle(x[~bad], w, t[~bad])
+    assert bool(((r.logprobs.double().cpu()[~bad] - lp).abs() <= tol + SUM + lp.abs() * 2.0 ** -23).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        xd.mul_(0.5)
+        td.copy_(td.roll(k + 1))
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out.logprobs, eager.logprobs) and torch.equal(out.entropy, eager.entropy)
