@@ -137,8 +137,8 @@ __device__ __forceinline__ uint16_t adapter_term(float& v) {
 // leaves few blocks without work.  The waves split the hidden size, each with the loads of
 // kShrinkSteps steps in flight; their sums meet in LDS, in order.
 // Bound: latency of the loads, table and rows alike: 2000 f16 rows x 2560, rank 64, 11.5 us; without the
-// table's loads 7.4, without the rows' 8.1, with neither 5.5; its ranks split over two or four blocks 12.5 and 16.9.  With tables as they come ([rank, hidden], a load of
-// 16 rows) 17.
+// table's loads 7.4, without the rows' 8.1, with neither 5.5; its ranks split over two or four blocks 12.5 and
+// 16.9.  With tables as they come ([rank, hidden], a load of 16 rows) 17.
 template <int XDT, int TDT, int RG>
 __global__ void __launch_bounds__(64 * kShrinkWaves, 4) adapter_shrink_kernel(AdapterArgs a) {
   constexpr int NX = AdapterX<XDT, TDT>::NX, NT = adapter_terms(TDT), RANK = 16 * RG, S = kShrinkSteps;
