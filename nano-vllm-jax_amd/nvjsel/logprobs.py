@@ -193,7 +193,7 @@ def lm_head_token_logprobs(hidden: torch.Tensor, output_weight, tokens: torch.Te
         if r is None:
             r = _scored_by_logits(x, output_weight, tokens, num_top, entropy, weight_layout, reduce_cast, adapters,
                                   adapter_ids)
-    return TokenLogprobs(*(t if t is None else t.reshape(*shape, *t.shape[1:]) for t in r))
+    return TokenLogprobs(*(t if t is None else t.reshape((*shape, *t.shape[1:])) for t in r))
 
 
 def _scored(x, output_weight, tokens, entropy, weight_layout, reduce_cast):
