@@ -475,7 +475,7 @@ __device__ __forceinline__ void beam_join(const BeamArgs& a, BeamJoinLds<LISTS>&
     const int st = !(t < INFINITY) ? BEAM_NAN : m == -INFINITY ? BEAM_DEAD : BEAM_LIVE;  // NaN: or an infinity; the mask leaves nothing
     state[w] = st;
     rmax[w] = m;
-    rlog[w] = st == BEAM_LIVE ? log(t) : 0.0;
+    rlog[w] = st != BEAM_LIVE ? 0.0 : LP ? row_log_sum(t) : log(t);
   };
   auto part_sum = [&](const BeamPart& p, float m) { return p.sum * exp((double)p.max - (m == -INFINITY ? 0.0 : (double)m)); };
   if constexpr (LP != LP_NONE) {  // one row

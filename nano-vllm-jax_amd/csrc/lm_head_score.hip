@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(256) score_finish_kernel(RowAnswers answers, c
   r.ent = wave_sum_f64(r.ent);
   if (lane != 0) return;
   const bool asked = t >= 0 && t < vocab;
-  row_answer(answers, row, asked, asked ? x : 0.0f, m, r, log(r.sum));
+  row_answer(answers, row, asked, asked ? x : 0.0f, m, r, row_log_sum(r.sum));
 }
 
 // f32 hidden rows as their three bf16 terms, [row][term][H], eight values a thread: once for a launch, where

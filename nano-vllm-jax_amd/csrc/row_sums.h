@@ -224,6 +224,10 @@ __device__ __forceinline__ void row_join(RowSum& r, const RowSum& part, float ma
   r.sum += f * part.sum;
 }
 
+// ln S: the row's maximum is one of its terms, 1 exactly, which the hardware's exp2 and a wave's series may leave an ulp
+// or so below; no log probability is above 0.
+__device__ __forceinline__ double row_log_sum(double sum) { return log(fmax(sum, 1.0)); }
+
 // logprob = (x - m) - ln S for the token's logit x, entropy = ln S - T / S (r: S and T,
 // relative to m).  Nothing left: -inf and 0; NaN or +inf among the logits: NaN; a row that
 // asks for no token: 0.
@@ -251,7 +255,7 @@ __device__ __forceinline__ void row_answer_from(const RowAnswers& a, const void*
                                                 float m, const RowSum& r) {
   const int64_t t = row_token(a, row);
   const bool asked = t >= 0 && t < vocab;
-  row_answer(a, row, asked, asked ? load_as_f32(logits, DT, (size_t)(at + t)) : 0.0f, m, r, log(r.sum));
+  row_answer(a, row, asked, asked ? load_as_f32(logits, DT, (size_t)(at + t)) : 0.0f, m, r, row_log_sum(r.sum));
 }
 
 }  // namespace nvjsel

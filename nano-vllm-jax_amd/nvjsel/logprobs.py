@@ -104,7 +104,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
     ``logits [..., V]`` (f32, bf16 or f16), ``tokens`` int32 or int64 of the shape
     before V.  With ``entropy`` also ``-sum p ln p`` of every row; with ``num_top``
     (at most 64) the likeliest tokens and their log probabilities, the best first,
-    equal ones by token.  Sums are taken in 32 and 64 bits, results are f32.
+    equal ones by token.  Sums are taken in 32 and 64 bits, results are f32, no
+    log probability above 0.
 
     A token outside 0..V-1 (the -1 of padding) asks for nothing: its log probability is
     0 and gives no gradient.  Logits of ``-inf`` (masked) have no probability and are no
