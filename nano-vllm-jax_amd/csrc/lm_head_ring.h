@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(512) lm_head_ring_kernel(LmArgs a, int rows, S
         if constexpr (S::ENT) u += sum_tree(p);
         __builtin_amdgcn_sched_barrier(0);
       }
-      const float d = smax[tb] == -INFINITY ? 0.0f : (smax[tb] - base) * kLog2e;
+      const float d = smax[tb] == -INFINITY ? 0.0f : fmaxf((smax[tb] - base) * kLog2e, -1e30f);  // finite: 0 times it is 0
       const double f = (double)__builtin_amdgcn_exp2f(d);
       if constexpr (S::ENT) ssum[tb].ent = f * (ssum[tb].ent + ssum[tb].sum * (double)d) + (double)u;
       ssum[tb].sum = f * ssum[tb].sum + (double)s;
