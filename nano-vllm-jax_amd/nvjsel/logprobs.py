@@ -74,27 +74,35 @@ class _Differentiable(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_logprobs, grad_entropy, *_):
-        if torch.is_grad_enabled():  # with create_graph: once is all there is
-            return _once(ctx, grad_logprobs, grad_entropy)
-        return _Differentiable.gradient(ctx, grad_logprobs, grad_entropy)
-
-    @staticmethod
-    def gradient(ctx, grad_logprobs, grad_entropy):
         if grad_logprobs is None and grad_entropy is None:
             return None, None, None, None
-        logits, tokens, stats = ctx.saved_tensors
-        rows, vocab = logits.shape
         g = None if grad_logprobs is None else grad_logprobs.contiguous()  # f32, as their outputs
         h = None if grad_entropy is None else grad_entropy.contiguous()
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-        with _on_device(logits.device):
-            _lib.call("nvjsel_token_logprobs_grad", logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab,
-                      _row_stride(logits), tokens.data_ptr(), tokens.element_size(), stats.data_ptr(),
-                      _ptr(g), _ptr(h), out.data_ptr(), vocab, _stream_handle(logits.device))
-        return out, None, None, None
+        # with create_graph the gradient stands in the graph, between the logits and a refusal
+        gradient = _Once.apply if torch.is_grad_enabled() else _gradient
+        return gradient(*ctx.saved_tensors, g, h), None, None, None
 
 
-_once = torch.autograd.function.once_differentiable(_Differentiable.gradient)
+def _gradient(logits, tokens, stats, g, h):
+    rows, vocab = logits.shape
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    with _on_device(logits.device):
+        _lib.call("nvjsel_token_logprobs_grad", logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab,
+                  _row_stride(logits), tokens.data_ptr(), tokens.element_size(), stats.data_ptr(),
+                  _ptr(g), _ptr(h), out.data_ptr(), vocab, _stream_handle(logits.device))
+    return out
+
+
+class _Once(torch.autograd.Function):
+    """The gradient, whose own derivative is refused, not left out."""
+
+    @staticmethod
+    def forward(ctx, *operands):
+        return _gradient(*operands)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("token_logprobs is differentiable once: a second derivative was asked for")
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int = 0,
@@ -113,8 +121,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
     token -1; a row with nothing left has log probability ``-inf`` and entropy 0.  A NaN or
     ``+inf`` in a row makes its results NaN, its alternatives the first tokens.
 
-    Differentiable in ``logits`` through ``logprobs`` and ``entropy`` (once; the
-    alternatives carry no gradient).  A row whose own two gradients are 0, or one
+    Differentiable in ``logits`` through ``logprobs`` and ``entropy`` (once: a second derivative
+    raises; the alternatives carry no gradient).  A row whose own two gradients are 0, or one
     with nothing left, gets a gradient of zeros.  In a captured graph take the gradient of a
     leaf made within the capture (``logits.detach().requires_grad_()``, ``torch.autograd.grad``)."""
     if logits.ndim < 1 or tokens.shape != logits.shape[:-1]:
