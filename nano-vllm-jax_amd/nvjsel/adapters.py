@@ -12,6 +12,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._tensors import _TORCH_DTYPES, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
@@ -38,7 +39,16 @@ class AdapterTable:
         return int(self.a.shape[0])
 
 
+def _no_tangent(who: str, *ts) -> None:
+    """Refuses forward mode's dual tensors, whose tangents the launches would leave behind."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    if any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError(f"{who} has no forward-mode derivative: call it on tensors without a tangent")
+
+
 def _no_gradient(who: str, *ts) -> None:
+    _no_tangent(who, *ts)
     if not torch.is_grad_enabled():
         return
     if any(t is not None and t.requires_grad for t in ts):

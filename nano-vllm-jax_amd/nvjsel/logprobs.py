@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .adapters import AdapterTable, _no_gradient
+from .adapters import AdapterTable, _no_gradient, _no_tangent
 from .selection import _adapter_ids, _normed, _weight_operand, lm_head_logits_hip, reference_reduce_cast
 from .w4 import W4Weight
 from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
@@ -121,8 +121,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
     token -1; a row with nothing left has log probability ``-inf`` and entropy 0.  A NaN or
     ``+inf`` in a row makes its results NaN, its alternatives the first tokens.
 
-    Differentiable in ``logits`` through ``logprobs`` and ``entropy`` (once: a second derivative
-    raises; the alternatives carry no gradient).  A row whose own two gradients are 0, or one
+    Differentiable in ``logits`` through ``logprobs`` and ``entropy`` (backward, once: forward mode and a second
+    derivative raise; the alternatives carry no gradient).  A row whose own two gradients are 0, or one
     with nothing left, gets a gradient of zeros.  In a captured graph take the gradient of a
     leaf made within the capture (``logits.detach().requires_grad_()``, ``torch.autograd.grad``)."""
     if logits.ndim < 1 or tokens.shape != logits.shape[:-1]:
@@ -139,6 +139,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, num_top: int =
     _dtype_code(logits, "logits")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64 (got {tokens.dtype})")
+    _no_tangent("token_logprobs", logits)
     _require_cuda(logits, tokens)
     shape = tokens.shape
     if logits.ndim != 2:
