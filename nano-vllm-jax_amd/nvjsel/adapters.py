@@ -61,7 +61,7 @@ def pack_adapters(a, b, scales=None) -> AdapterTable:
 
     ``scales`` (f32 ``[L]`` or numbers; 1 where None) multiply the adapters' parts, ``alpha / R`` as
     a rule.  Ranks may differ, up to 512 (a table's ranks are laid out as its largest, rounded up to 16 or a
-    multiple of 32).  Not differentiable."""
+    multiple of 32).  Not differentiable: tensors that want a gradient, scales too, are refused."""
     if torch.is_tensor(a) and torch.is_tensor(b) and a.ndim == b.ndim == 3 and a.shape[0] == b.shape[0]:
         plain = [(a, b)]  # all of one rank: one launch each
     else:
@@ -81,7 +81,8 @@ def pack_adapters(a, b, scales=None) -> AdapterTable:
     dtype = a[0].dtype
     if dtype not in _TABLE_DTYPES or any(t.dtype != dtype for t in a + b):
         raise ValueError("adapters must be bfloat16 or float16, a and b alike")
-    _no_gradient("pack_adapters", *a, *b)
+    given = scales if isinstance(scales, (list, tuple)) else [scales]
+    _no_gradient("pack_adapters", *a, *b, *(t for t in given if torch.is_tensor(t)))
     most = max(int(t.shape[0]) for t in a)
     if most > MAX_RANK:
         raise ValueError(f"ranks must be at most {MAX_RANK} (got {most})")
