@@ -13,6 +13,7 @@ from functools import lru_cache
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._tensors import _TORCH_DTYPES, _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
@@ -194,4 +195,6 @@ def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, 
         _lib.call("nvjsel_apply_adapters", x.data_ptr(), xd, _stride(x), base.data_ptr(), od, _stride(base), a.data_ptr(),
                   adapters.b.data_ptr(), td, adapters.scales.data_ptr(), a.shape[0], adapters.rank, hidden, width,
                   ids.data_ptr(), rows, flat.data_ptr(), _stride(flat), ws.data_ptr(), nbytes, stream)
+    if out is not None:
+        increment_version(out)  # a backward pass that saved it is to notice
     return result
