@@ -397,8 +397,9 @@ int nvjsel_lm_head_token_logprobs(const void* hidden, int hidden_dtype, const vo
  * x [rows, hidden] of x_dtype, base and out [rows, width] of out_dtype (rows their strides
  * apart, out of at least width; out = base for in place, else they share no memory).  hidden at least 8
  * (NVJSEL_EUNSUPPORTED below).  Tables of bf16 or f16 from nvjsel_adapters_pack, of `rank` 16 or a multiple of
- * 32 up to 512; scales f32, ids int32.  fp32 sums, out rounded once.  A NaN or an infinity in a row of x or in
- * its adapter makes that row NaN and no other.  rows at most 2^20, hidden 2^24, width 2^28.
+ * 32 up to 512; scales f32, ids int32.  fp32 sums, out rounded once.  A NaN or an infinity in a row of x, or
+ * in its adapter's A or scale, makes that row NaN; one in B's row v leaves column v of that adapter's rows without
+ * finite values (NaN or infinite); neither reaches other values.  rows at most 2^20, hidden 2^24, width 2^28.
  * Workspace: scratch (16-byte aligned).
  *
  * nvjsel_adapters_pack lays out `count` adapters' a [rank, hidden] (which = 0) or b [width, rank] (1) of

@@ -149,7 +149,8 @@ def apply_adapters(x: torch.Tensor, base: torch.Tensor, adapters: AdapterTable, 
     outside 0..L-1 (the -1 of a row without an adapter) leaves its row as it is.  Any order and
     mixture of adapters.  Sums are fp32; the result, of ``base``'s type, is rounded once.
     ``out`` receives it (``base`` itself for in place), a new tensor where None.  A NaN or an infinity
-    in a row of ``x``, or in its own adapter, makes that row's results NaN and no other's.
+    in a row of ``x``, or in its own adapter's A or scale, makes that row's results NaN; one in row ``v`` of B leaves
+    column ``v`` of that adapter's rows NaN or infinite; neither reaches other values.
     Not differentiable."""
     rows_shape, hidden, width = adapter_ids.shape, adapters.hidden, adapters.width
     if x.ndim < 1 or base.ndim < 1 or x.shape[:-1] != rows_shape or base.shape[:-1] != rows_shape:
