@@ -26,15 +26,16 @@ static constexpr int kShrinkBlocks = 512;
 // Terms that y is kept in.
 __host__ __device__ constexpr int adapter_terms(int table_dtype) { return table_dtype == DT_BF16 ? 3 : 2; }
 
-// f32 values as the next bf16 term, which leaves the remainders.
+// f32 values as the next bf16 term, which leaves the remainders.  Cut off, not rounded: three terms hold all 24
+// bits either way, and rounded the largest finite numbers would become infinite.
 __device__ __forceinline__ u32x4_t bf16_term(float (&v)[8]) {
   uint32_t o[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = __builtin_bit_cast(uint16_t, (__bf16)v[2 * j]), hi = __builtin_bit_cast(uint16_t, (__bf16)v[2 * j + 1]);
-    o[j] = hi << 16 | lo;
-    v[2 * j] = v[2 * j] - __uint_as_float(o[j] << 16);
-    v[2 * j + 1] = v[2 * j + 1] - __uint_as_float(o[j] & 0xFFFF0000u);
+    const uint32_t lo = __float_as_uint(v[2 * j]), hi = __float_as_uint(v[2 * j + 1]) & 0xFFFF0000u;
+    o[j] = hi | lo >> 16;
+    v[2 * j] = v[2 * j] - __uint_as_float(lo & 0xFFFF0000u);
+    v[2 * j + 1] = v[2 * j + 1] - __uint_as_float(hi);
   }
   return u32x4_t{o[0], o[1], o[2], o[3]};
 }
@@ -118,7 +119,7 @@ __device__ __forceinline__ int adapter_exponent(float m) {
   const int e = 15 - __builtin_amdgcn_frexp_expf(m);
   return !(m > 0.0f && m < INFINITY) ? 0 : e < -126 ? -126 : e > 126 ? 126 : e;
 }
-// The next term of v in the tables' type, which leaves the remainder.
+// The next term of v in the tables' type, which leaves the remainder (bf16 cut off, as x's).
 template <int TDT>
 __device__ __forceinline__ uint16_t adapter_term(float& v) {
   if constexpr (TDT == DT_F16) {
@@ -126,9 +127,9 @@ __device__ __forceinline__ uint16_t adapter_term(float& v) {
     v = v - (float)h;
     return __builtin_bit_cast(uint16_t, h);
   } else {
-    const __bf16 h = (__bf16)v;
-    v = v - (float)h;
-    return __builtin_bit_cast(uint16_t, h);
+    const uint32_t h = __float_as_uint(v) & 0xFFFF0000u;
+    v = v - __uint_as_float(h);
+    return (uint16_t)(h >> 16);
   }
 }
 
