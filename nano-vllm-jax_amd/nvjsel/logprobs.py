@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .adapters import AdapterTable, _no_gradient, _no_tangent
+from .adapters import MAX_ROWS as _ADAPTER_ROWS, AdapterTable, _no_gradient, _no_tangent
 from .selection import _adapter_ids, _normed, _weight_operand, lm_head_logits_hip, reference_reduce_cast
 from .w4 import W4Weight
 from ._tensors import _dtype_code, _on_device, _require_cuda, _stream_handle, _workspace
@@ -237,7 +237,7 @@ def _score_bytes(device: int, *shape: int) -> int:
 
 def _scored_by_logits(x, output_weight, tokens, num_top, entropy, weight_layout, reduce_cast, adapters, adapter_ids):
     vocab = output_weight.vocab if isinstance(output_weight, W4Weight) else max(output_weight.shape)
-    step = max(64, _LOGIT_BYTES // (4 * vocab) // 64 * 64)
+    step = min(max(64, _LOGIT_BYTES // (4 * vocab) // 64 * 64), _ADAPTER_ROWS)
     parts = []
     for i in range(0, x.shape[0], step):
         ids = None if adapters is None else adapter_ids[i:i + step]

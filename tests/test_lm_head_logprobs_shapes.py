@@ -48,3 +48,49 @@ def test_one_hidden_vector(hidden):
         assert torch.equal(one.logprobs, row.logprobs[0]) and torch.equal(one.entropy, row.entropy[0])
         if "num_top" in kw:
             assert torch.equal(one.top_ids, row.top_ids[0]) and torch.equal(one.top_logprobs, row.top_logprobs[0])
+
+
+@pytest.mark.parametrize("vocab,rows", [(3, (1 << 20) + 5), (40, (1 << 20) + 5), (3, 100), (100_000, 3000)])
+@pytest.mark.parametrize("adapted", [True, False])
+def test_rows_of_a_step(monkeypatch, vocab, rows, adapted):
+    """Logits are formed for as many rows at a time as every call on the way takes."""
+    steps = []
+
+    def logits(x, w, *, adapters, adapter_ids, **kw):
+        assert (adapter_ids is not None) == adapted and (not adapted or adapter_ids.shape == x.shape[:1])
+        steps.append(x.shape[0])
+        return x
+
+    def scored(logits, tokens, *, num_top, entropy):
+        return nvjsel.TokenLogprobs(tokens.float(), None, None, None)
+
+    monkeypatch.setattr(module, "lm_head_logits_hip", logits)
+    monkeypatch.setattr(module, "token_logprobs", scored)
+    tokens = torch.arange(rows)
+    ids = torch.zeros(rows, dtype=torch.int32) if adapted else None
+    r = module._scored_by_logits(torch.zeros(1, 2).expand(rows, 2), torch.zeros(2, vocab), tokens, 0, False, None, None,
+                                 object() if adapted else None, ids)
+    assert torch.equal(r[0], tokens.float()) and sum(steps) == rows
+    assert max(steps) <= (1 << 20) and max(steps) * vocab * 4 <= max(1 << 28, 64 * vocab * 4)
+    assert len(steps) == -(-rows // max(steps))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_adapters_take():
+    rows = (1 << 20) + 70
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(rows, 8, generator=g).to(torch.bfloat16)
+    w = torch.randn(5, 8, generator=g).to(torch.bfloat16)
+    a, b = torch.randn(1, 2, 8, generator=g).to(torch.bfloat16), torch.randn(1, 5, 2, generator=g).to(torch.bfloat16)
+    t = torch.randint(0, 5, (rows,), generator=g)
+    table = nvjsel.pack_adapters(a.cuda(), b.cuda())
+    ids = (torch.arange(rows) % 2 - 1).to(torch.int32)
+    r = nvjsel.lm_head_token_logprobs(x.cuda(), w.cuda(), t.cuda(), weight_layout="vh", reduce_cast=0, adapters=table,
+                                      adapter_ids=ids.cuda())
+    l = x.double() @ w.double().T + (ids == 0).double()[:, None] * ((x.double() @ a[0].double().T) @ b[0].double().T)
+    want = torch.log_softmax(l, 1).gather(1, t[:, None])[:, 0]
+    # fp32 sums of 8, 8 and 2 products (each addition 2^-23 of the magnitudes), y's terms 2^-21
+    xs = x.double().abs()
+    size = xs @ w.double().abs().T + (xs @ a[0].double().abs().T) @ b[0].double().abs().T
+    off = size.amax(1) * 30 * 2.0 ** -23
+    assert bool(((r.logprobs.double().cpu() - want).abs() <= 2 * off + 2.0 ** -19 + want.abs() * 2.0 ** -24).all())
