@@ -9,10 +9,12 @@
 // ends; a share's parts are joined by a second kernel, a wave a row.
 //
 // Bound: the products, at the clock that the card's power leaves.  2048 bf16 rows x 1024, 248,320 tokens, with
-// entropies: 876-928 us by card, 1.12-1.19 PFLOP/s (a library's bare product of these sizes, which writes
-// 1 GB of logits, 919); the tiles' products without their sums 881: matrix pipes 77% busy at some 1.5 GHz of
-// 2.4.  24 rows 79 us, the stream of W (508 MB) at 6.4 TB/s.  300 f32 rows x 768 (three products each)
-// of 50,257 tokens 77 us, 0.90 PFLOP/s: four tiles a block, three launches; 2048 x 1024, 248,320 tokens 2.62 ms, 1.19 PFLOP/s.
+// entropies: 874-928 us by card, 1.12-1.19 PFLOP/s (a library's bare product of these sizes, which writes
+// 1 GB of logits, 919); the tiles' products without their sums 881: matrix pipes 67% busy of 1.51 M cycles, some 1.7 GHz of
+// 2.4.  Logits rounded to the weight's type, the default of 16-bit hidden rows, take 4% more there (920 beside 886 on one
+// card: each is rounded where it is compared, summed and taken), 1-2% for 64 and 256 rows, nothing for few.
+// 24 rows 79 us, the stream of W (508 MB) at 6.4 TB/s.  300 f32 rows x 768 (three products each)
+// of 50,257 tokens 75-77 us, 0.90 PFLOP/s: four tiles a block, three launches; 2048 x 1024, 248,320 tokens 2.62 ms, 1.19 PFLOP/s.
 #include "lm_head_score.h"
 
 namespace nvjsel {
